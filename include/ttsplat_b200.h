@@ -360,6 +360,51 @@ int tts_wsr_dense_bwd(const float* theta_u, const float* o, const float* color, 
  * step uploads and holds its targets as uint8.  src and dst 16-byte aligned. */
 int tts_unit_from_u8(const uint8_t* src, long long n, float* dst, void* stream);
 
+/* ---- table rows through slot tables -------------------------------------------------------
+ * The gather of per-gaussian rows by an (idx, valid) table, `conic[idx]` and `color_o[idx] * valid`
+ * of tools/m4_train_binned.py:203-211, for rows of any width, and its transpose.
+ * table [R] rows of C elements of `type`, table_stride elements apart; idx [N] int32 or (idx64)
+ * int64; valid [N] uint8 or NULL; weight [N] fp32 or NULL; N < 2^31, R < 2^31 - 1, C < 2^31.
+ * out[N][C] = scale * weight[n] * table[idx[n]], rounded once; a slot with valid 0 or a negative
+ * idx gives zeros, an idx >= R is not read and gives NaN. */
+#define TTS_ROW_F32 0
+#define TTS_ROW_BF16 1
+#define TTS_ROW_F16 2
+int tts_gather_rows(const void* table, long long R, long long C, long long table_stride, int type,
+                    const void* idx, int idx64, const uint8_t* valid, const float* weight,
+                    float scale, long long N, void* out, void* stream);
+/* gtable[R][C] (or NULL) = sum over n with idx[n] = v, in a fixed order, of scale * weight[n] *
+ * gout[n], zero for rows without a use; gweight[N] (or NULL; needs the table) = scale * <gout[n],
+ * table[idx[n]]>, zero for slots that look nothing up.  gout rows are gout_stride elements apart.
+ * Sums in fp32, rounded once; the workspace is needed for gtable. */
+size_t tts_gather_rows_bwd_workspace_bytes(long long N, long long R, long long C);
+int tts_gather_rows_bwd(const void* table, long long R, long long C, long long table_stride,
+                        int type, const void* idx, int idx64, const uint8_t* valid,
+                        const float* weight, float scale, long long N, const void* gout,
+                        long long gout_stride, void* gtable, float* gweight, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* ---- label scores ---------------------------------------------------------------------------
+ * Rows of C logits of `type`, row_stride elements apart (P < 2^31 rows, 1 <= C < 2^31); labels [P]
+ * int32 or (labels64) int64.  logp[P] = log softmax at the label (0 for a negative label, NaN for
+ * one >= C), entropy[P] of the softmax, the `top` (0..16) best labels' log probabilities
+ * top_logp[P][top] and ids top_ids[P][top], best first, ties to the lowest id, and stats[P][2] =
+ * (max, log of the sum of exp(x - max)) for the backward (or NULL).  Logits of -inf are masked labels: never
+ * an alternative (id -1 and -inf where there are fewer than `top`); a row of nothing else has logp
+ * -inf and entropy 0; a NaN or +inf in a row makes its results NaN. */
+int tts_label_log_probs(const void* logits, long long P, long long C, long long row_stride,
+                        int type, const void* labels, int labels64, int top, float* logp,
+                        float* entropy, float* top_logp, int64_t* top_ids, float* stats,
+                        void* stream);
+/* glogits[P][C] from the gradients of logp, entropy and top_logp (each NULL when there is none);
+ * stats, entropy and top_ids as the forward wrote them.  Zeros for a row whose gradients are all
+ * zero and for a row of masked labels only. */
+int tts_label_log_probs_bwd(const void* logits, long long P, long long C, long long row_stride,
+                            int type, const void* labels, int labels64, int top, const float* stats,
+                            const float* entropy, const int64_t* top_ids, const float* g_logp,
+                            const float* g_entropy, const float* g_top, void* glogits,
+                            void* stream);
+
 /* ---- measurement ----------------------------------------------------------------------------
  * FP32 FMA-pipe throughput probe (no counterpart in the reference): `blocks` blocks of 256
  * threads run 8 independent packed fma.rn.f32x2 chains for `iters` rounds and write one float

@@ -1,0 +1,271 @@
+"""The row lookup (binned.gather_rows) and its gradients against float64, at the sizes, masks and layouts
+where they can go wrong.
+
+Tolerances, with u = 2^-24 the fp32 rounding and r = finfo(type).eps / 2 that of the result:
+* out = round(round(scale w) t): the factor, the product and the result, 2u + r relative (r = u for fp32);
+* a gradient row adds n products of a rounded factor: each term is off by 3u (factor, product, weight
+  as given), each of the n adds by u of the running sum of magnitudes: (n + 3) u sum|f g| + r |value|;
+* a weight's gradient adds C products: (C + 3) u |scale| sum|g t|.
+fp16 results below the normal range are off by half the smallest step (2^-25) instead.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _inputs(R, C, shape, dt=torch.float32, seed=0, index=torch.int64, unused=0.2, hot=0.0, valid=True, weight=True):
+    g = torch.Generator().manual_seed(seed)
+    N = 1
+    for s in shape:
+        N *= s
+    idx = torch.randint(0, max(R, 1), (N,), generator=g)
+    idx[torch.rand(N, generator=g) < hot] = R // 2          # one row with most of the uses
+    idx[torch.rand(N, generator=g) < unused / 2] = -1
+    ok = torch.rand(N, generator=g) >= unused / 2
+    if R == 0:
+        idx.fill_(-1)
+    return dict(table=torch.randn(R, C, generator=g).to(dt).to(DEV), idx=idx.to(index).reshape(shape).to(DEV),
+                valid=ok.reshape(shape).to(DEV) if valid else None,
+                weight=(torch.rand(N, generator=g) * 2 - 0.5).reshape(shape).to(DEV) if weight else None,
+                gout=torch.randn(N, C, generator=g).to(dt).reshape(*shape, C).to(DEV))
+
+
+def _check(x, scale=1.0, gout=None):
+    from tt_splat_b200 import binned
+    table = x["table"].detach().requires_grad_(True)
+    weight = None if x["weight"] is None else x["weight"].detach().requires_grad_(True)
+    out = binned.gather_rows(table, x["idx"], valid=x["valid"], weight=weight, scale=scale)
+    gout = x["gout"] if gout is None else gout
+    grads = torch.autograd.grad(out, [table] + ([weight] if weight is not None else []), gout)
+    dt, (R, C) = table.dtype, table.shape
+    r, sub = torch.finfo(dt).eps / 2, (2.0 ** -25 if dt == torch.float16 else 0.0)
+    idx = x["idx"].reshape(-1).long()
+    use = idx >= 0 if x["valid"] is None else (idx >= 0) & x["valid"].reshape(-1)
+    f = torch.full(idx.shape, float(scale), dtype=torch.float64, device=DEV)
+    if weight is not None:
+        f = f * weight.detach().reshape(-1).double()
+    t64, n = table.detach().double(), use.nonzero()[:, 0]
+    ref = torch.zeros(idx.numel(), C, dtype=torch.float64, device=DEV)
+    ref[n] = f[n, None] * t64[idx[n]]
+    assert out.shape == (*x["idx"].shape, C) and out.dtype == dt
+    err = (out.detach().reshape(-1, C).double() - ref).abs()
+    assert (err <= ref.abs() * (r + 2.5 * U) + sub).all()
+    assert (out.detach().reshape(-1, C)[~use] == 0).all()
+
+    go = gout.reshape(-1, C).double()
+    term = f[n, None] * go[n]
+    gt = torch.zeros(R, C, dtype=torch.float64, device=DEV).index_add_(0, idx[n], term)
+    mag = torch.zeros(R, C, dtype=torch.float64, device=DEV).index_add_(0, idx[n], term.abs())
+    cnt = torch.bincount(idx[n], minlength=R)[:R, None]
+    assert grads[0].shape == table.shape and grads[0].dtype == dt
+    err = (grads[0].double() - gt).abs()
+    assert (err <= (cnt + 3) * U * mag * 1.01 + (r + U) * gt.abs() + sub).all()
+    assert (grads[0][cnt[:, 0] == 0] == 0).all()
+    if weight is not None:
+        dots = go[n] * t64[idx[n]]
+        gw, gm = torch.zeros_like(f), torch.zeros_like(f)
+        gw[n], gm[n] = scale * dots.sum(1), abs(scale) * dots.abs().sum(1)
+        assert grads[1].shape == weight.shape and grads[1].dtype == torch.float32
+        err = (grads[1].reshape(-1).double() - gw).abs()
+        assert (err <= (C + 3) * U * gm * 1.01).all()
+        assert (grads[1].reshape(-1)[~use] == 0).all()
+    return out, grads
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("C", [1, 2, 3, 4, 7, 8, 12, 16, 31, 33, 45, 64, 100, 256, 1000, 2049])
+def test_widths(C, dt):
+    _check(_inputs(37, C, (129,), dt, seed=C), scale=0.75)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("N", [1, 2, 31, 32, 33, 255, 257, 4095, 4097, 8193, 40000])
+def test_lengths(N, dt):
+    _check(_inputs(300, 13, (N,), dt, seed=N, index=torch.int32))
+
+
+@pytest.mark.parametrize("R", [1, 2, 255, 256, 257, 65535, 65536, 65537, 300000, 17000000])
+def test_table_sizes(R):
+    """Row counts on both sides of the sort's digits; the last and first row are looked up."""
+    x = _inputs(R, 2, (20000,), seed=R % 1000)
+    x["idx"][0], x["idx"][1] = R - 1, 0
+    x["valid"][:2] = True
+    _check(x)
+
+
+@pytest.mark.parametrize("hot", [0.5, 0.99, 1.0])
+@pytest.mark.parametrize("N,C", [(5000, 45), (100000, 6), (70000, 128)])
+def test_row_with_most_uses(hot, N, C):
+    _check(_inputs(1000, C, (N,), torch.bfloat16, seed=N, hot=hot))
+
+
+@pytest.mark.parametrize("valid,weight", [(False, False), (True, False), (False, True)])
+def test_without_mask_or_weight(valid, weight):
+    _check(_inputs(50, 9, (40, 16), seed=3, valid=valid, weight=weight), scale=-3.5)
+
+
+def test_nothing_looked_up():
+    from tt_splat_b200 import binned
+    x = _inputs(20, 5, (64,), unused=0.0)
+    x["valid"][:] = False
+    _check(x)
+    x["valid"][:] = True
+    x["idx"][:] = -7
+    _check(x)
+    _check(_inputs(0, 5, (64,)))                                       # a table without rows
+    t = torch.randn(20, 5, device=DEV, requires_grad=True)
+    out = binned.gather_rows(t, torch.empty(0, 3, dtype=torch.int32, device=DEV))
+    assert out.shape == (0, 3, 5)
+    assert (torch.autograd.grad(out, t, torch.empty_like(out))[0] == 0).all()
+    t = torch.randn(20, 0, device=DEV, requires_grad=True)
+    out = binned.gather_rows(t, torch.zeros(4, dtype=torch.int32, device=DEV))
+    assert out.shape == (4, 0) and torch.autograd.grad(out, t, out.detach())[0].shape == (20, 0)
+
+
+def test_shapes_of_tables_and_indices():
+    from tt_splat_b200 import binned
+    t = torch.randn(30, 15, 3, device=DEV)
+    i = torch.randint(0, 30, (2, 4, 8), device=DEV)
+    assert torch.equal(binned.gather_rows(t, i), t[i])
+    v = torch.randn(30, device=DEV)
+    assert torch.equal(binned.gather_rows(v, i), v[i])
+    assert torch.equal(binned.gather_rows(t, i[0, 0, 0]), t[i[0, 0, 0]])
+    assert torch.equal(binned.gather_rows(t, i.transpose(0, 2)), t[i.transpose(0, 2)])
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_strided_tables_and_gradients(dt):
+    """Columns of a wider table, an offset that breaks 16-byte alignment, and gradients that arrive as a
+    slice or as one expanded row or number."""
+    from tt_splat_b200 import binned
+    wide = torch.randn(40, 24, device=DEV).to(dt)
+    i = torch.randint(0, 40, (100,), device=DEV)
+    for cols in (slice(0, 8), slice(1, 9), slice(2, 5), slice(8, 24)):
+        assert torch.equal(binned.gather_rows(wide[:, cols], i), wide[i][:, cols])
+    assert torch.equal(binned.gather_rows(wide.t(), i % 24), wide.t()[i % 24])
+    x = _inputs(40, 8, (100,), dt)
+    big = torch.randn(100, 19, device=DEV).to(dt)
+    _check(x, gout=big[:, 3:11])
+    _check(x, gout=big[:1, :8].expand(100, 8))
+    _check(x, gout=big[:1, :1].expand(100, 8))
+    x["table"] = wide[:, 5:13]
+    _check(x)
+
+
+def test_bad_values_stay_out():
+    """NaN gradients and weights of unused slots, and table rows nobody uses, reach nothing; an index
+    past the table gives NaN and no gradient."""
+    from tt_splat_b200 import binned
+    x = _inputs(20, 6, (200,), unused=0.0)
+    x["valid"][::3] = False
+    x["table"][7] = float("nan")
+    x["idx"][x["idx"] == 7] = 8
+    x["gout"][::3] = float("nan")
+    y = dict(x, weight=x["weight"].clone())
+    y["weight"][::3] = float("inf")
+    from tt_splat_b200 import ops
+    gt, gw = ops.gather_rows_bwd(y["table"], 20, y["idx"], y["valid"].view(torch.uint8), y["weight"], 1.0, y["gout"],
+                                 want_weight=True)
+    assert torch.isfinite(gt).all() and torch.isfinite(gw).all() and (gw[::3] == 0).all()
+    assert torch.isfinite(binned.gather_rows(y["table"], y["idx"], y["valid"], y["weight"])).all()
+    for far in (20, 21, 2 ** 31 - 1, 2 ** 40):
+        t = torch.randn(20, 6, device=DEV, requires_grad=True)
+        w = torch.ones(3, device=DEV, requires_grad=True)
+        out = binned.gather_rows(t, torch.tensor([1, far, 1], device=DEV), weight=w)
+        assert out[1].isnan().all() and torch.equal(out[0], t[1])
+        gt, gw = torch.autograd.grad(out, [t, w], torch.ones_like(out))
+        assert torch.equal(gt[1], torch.full((6,), 2.0, device=DEV)) and gt.sum() == 12 and gw[1] == 0
+
+
+def test_offsets_past_32_bits():
+    """An output and a table whose last elements lie past 2^31 elements."""
+    from tt_splat_b200 import binned
+    C = 8192
+    R = 2 ** 31 // C + 3
+    t = torch.zeros(R, C, dtype=torch.bfloat16, device=DEV)
+    t[-1] = 1.5
+    t[0] = 0.5
+    i = torch.zeros(R, dtype=torch.int32, device=DEV)
+    i[-1] = R - 1
+    t.requires_grad_(True)
+    out = binned.gather_rows(t, i)
+    assert (out[-1] == 1.5).all() and (out[-2] == 0.5).all()
+    gout = torch.zeros_like(out)
+    gout[-1], gout[-2] = 2.0, 3.0
+    (g,) = torch.autograd.grad(out, t, gout)
+    assert (g[-1] == 2.0).all() and (g[0] == 3.0).all() and (g[1:-1] == 0).all()
+
+
+def test_same_bits_every_time():
+    a, b = (_check(_inputs(64, 40, (30000,), torch.bfloat16, hot=0.3)) for _ in range(2))
+    assert all(torch.equal(p, q) for p, q in zip(a[1], b[1]))
+
+
+def test_gradient_against_differences():
+    """The lookup is linear in the table and in the weights, so differences are exact up to rounding: the
+    change of <gout, out> along a direction d equals <gradient, d> (fp32 sums of 4000 terms, 4000 u)."""
+    from tt_splat_b200 import binned
+    x = _inputs(30, 8, (500,))
+    _, (gt, gw) = _check(x, scale=2.0)
+    value = lambda t, w: (binned.gather_rows(t, x["idx"], x["valid"], w, 2.0).double() * x["gout"].double()).sum()  # noqa: E731
+    d, e = torch.randn_like(x["table"]), torch.randn_like(x["weight"])
+    dt = value(x["table"] + d, x["weight"]) - value(x["table"], x["weight"])
+    dw = value(x["table"], x["weight"] + e) - value(x["table"], x["weight"])
+    mag = (x["gout"].double().abs().sum() * 40)
+    assert abs(dt - (gt.double() * d.double()).sum()) < 4000 * U * mag
+    assert abs(dw - (gw.double() * e.double()).sum()) < 4000 * U * mag
+
+
+def test_streams_and_graphs():
+    """On a side stream, two calls at once on two streams, and a captured forward and backward replayed on
+    new contents."""
+    from tt_splat_b200 import binned
+    x = _inputs(100, 33, (20000,), hot=0.2)
+    y = _inputs(900, 4, (9000,), torch.float16, seed=5)
+    ref = [_check(z) for z in (x, y)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for z, s in zip((x, y), streams):
+        with torch.cuda.stream(s):
+            t, w = z["table"].detach().requires_grad_(True), z["weight"].detach().requires_grad_(True)
+            out = binned.gather_rows(t, z["idx"], z["valid"], w)
+            got.append((out, torch.autograd.grad(out, [t, w], z["gout"])))
+    torch.cuda.synchronize()
+    for (o, g), (ro, rg) in zip(got, ref):
+        assert torch.equal(o, ro) and all(torch.equal(a, b) for a, b in zip(g, rg))
+
+    t, w = x["table"].clone().requires_grad_(True), x["weight"].clone().requires_grad_(True)
+    # torch ties a leaf's gradient to the stream of the graph that is alive: eager ones go before the capture
+    eager = binned.gather_rows(t, x["idx"], x["valid"], w)
+    del eager
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = binned.gather_rows(t, x["idx"], x["valid"], w)
+            grads = torch.autograd.grad(out, [t, w], x["gout"])
+        graphs.append((g, out, grads))
+    z = _inputs(100, 33, (20000,), seed=9, hot=0.1)
+    with torch.no_grad():
+        t.copy_(z["table"]), w.copy_(z["weight"])
+        x["idx"].copy_(z["idx"]), x["valid"].copy_(z["valid"]), x["gout"].copy_(z["gout"])
+    for g, _, _ in graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    ro, rg = _check(z)
+    for _, o, gr in graphs:
+        assert torch.equal(o, ro) and all(torch.equal(a, b) for a, b in zip(gr, rg))
+
+
+def test_second_derivative_is_refused():
+    from tt_splat_b200 import binned
+    t = torch.randn(5, 3, device=DEV, requires_grad=True)
+    out = binned.gather_rows(t, torch.zeros(4, dtype=torch.int64, device=DEV))
+    (g,) = torch.autograd.grad((out * out).sum(), t, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), t)

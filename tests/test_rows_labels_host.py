@@ -1,0 +1,77 @@
+"""Refusals of the row lookup and the label scores, before anything reaches a GPU: wrong types, shapes
+and ranges in Python, and the C entry points' own checks (null pointers are never touched)."""
+import pytest
+import torch
+
+
+def test_gather_rows_refusals(pkg):
+    from tt_splat_b200 import binned
+    table, idx = torch.zeros(4, 3), torch.zeros(5, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        binned.gather_rows(table, idx)
+    with pytest.raises(ValueError, match="dimension"):
+        binned.gather_rows(torch.zeros(()), idx)
+    with pytest.raises(TypeError, match="table"):
+        binned.gather_rows(table.double(), idx)
+    with pytest.raises(TypeError, match="idx"):
+        binned.gather_rows(table, idx.to(torch.int16))
+    with pytest.raises(TypeError, match="idx"):
+        binned.gather_rows(table, idx.float())
+    with pytest.raises(TypeError, match="valid"):
+        binned.gather_rows(table, idx, valid=torch.ones(5))
+    with pytest.raises(ValueError, match="valid"):
+        binned.gather_rows(table, idx, valid=torch.ones(4, dtype=torch.bool))
+    with pytest.raises(TypeError, match="weight"):
+        binned.gather_rows(table, idx, weight=torch.ones(5, dtype=torch.float64))
+    with pytest.raises(ValueError, match="weight"):
+        binned.gather_rows(table, idx, weight=torch.ones(5, 1))
+
+
+def test_label_log_probs_refusals(pkg):
+    from tt_splat_b200 import metrics
+    x, t = torch.zeros(5, 7), torch.zeros(5, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        metrics.label_log_probs(x, t)
+    with pytest.raises(ValueError, match="at least one label"):
+        metrics.label_log_probs(torch.zeros(5, 0), t)
+    with pytest.raises(TypeError, match="logits"):
+        metrics.label_log_probs(x.double(), t)
+    with pytest.raises(TypeError, match="labels"):
+        metrics.label_log_probs(x, t.float())
+    with pytest.raises(ValueError, match="labels"):
+        metrics.label_log_probs(x, t[:4])
+    for top in (-1, 17):
+        with pytest.raises(ValueError, match="top"):
+            metrics.label_log_probs(x, t, top=top)
+
+
+def test_c_entry_points_refuse(pkg):
+    from tt_splat_b200 import _lib
+    lib = _lib.lib()
+    err = lambda: lib.tts_last_error().decode()  # noqa: E731
+    gather = lambda R, C, type, N: lib.tts_gather_rows(None, R, C, C, type, None, 0, None, None, 1.0, N, None, None)  # noqa: E731
+    assert gather(4, 3, 3, 5) == 1 and "type" in err()
+    assert gather(4, 3, -1, 5) == 1 and "type" in err()
+    assert gather(4, 3, 0, 2 ** 31) == 1 and "lookups" in err()
+    assert gather(2 ** 31 - 1, 3, 0, 5) == 1 and "table rows" in err()
+    assert gather(4, 2 ** 31, 0, 5) == 1 and "width" in err()
+    assert gather(4, 3, 0, 5) == 1 and "null" in err()
+    assert gather(4, 3, 0, 0) == 0 and gather(4, 0, 0, 5) == 0       # nothing to write
+    assert lib.tts_gather_rows_bwd_workspace_bytes(1000, 100, 8) > 0
+    fake = 16                                                       # never dereferenced on the host
+    bwd = lambda **k: lib.tts_gather_rows_bwd(k.get("table"), 4, 3, 3, 0, k.get("idx"), 0, None, None, 1.0, 5,  # noqa: E731
+                                              k.get("gout"), 3, k.get("gtable"), k.get("gweight"), None, 0, None)
+    assert bwd(gtable=fake) == 1 and "null" in err()
+    assert bwd(idx=fake, gout=fake, gweight=fake) == 1 and "needs the table" in err()
+    assert bwd(idx=fake, gout=fake, gtable=fake) == 3 and "workspace" in err()
+    assert bwd(idx=fake, gout=fake) == 0                            # no gradient wanted
+    score = lambda P, C, type, top: lib.tts_label_log_probs(None, P, C, C, type, None, 0, top, None, None, None, None,  # noqa: E731
+                                                            None, None)
+    assert score(5, 7, 9, 0) == 1 and "type" in err()
+    assert score(5, 0, 0, 0) == 1 and "labels" in err()
+    assert score(2 ** 31, 7, 0, 0) == 1 and "rows" in err()
+    assert score(5, 7, 0, 17) == 1 and "top" in err()
+    assert score(5, 7, 0, 0) == 1 and "null" in err()
+    assert score(0, 7, 0, 0) == 0
+    assert lib.tts_label_log_probs_bwd(None, 5, 7, 7, 0, None, 0, 0, None, None, None, None, None, None, None, None) == 1
+    assert "null" in err()

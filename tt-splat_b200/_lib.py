@@ -81,6 +81,11 @@ SIGNATURES = {
     "tts_phi_theta_bwd": (I, [P, P, P, LL, LL, P, P, P, SZ, I, P]),
     "tts_poly_splat_wgeo": (I, [P, LL, LL, D, P, P, P, I, P]),
     "tts_unit_from_u8": (I, [P, LL, P, P]),
+    "tts_gather_rows": (I, [P, LL, LL, LL, I, P, I, P, P, F, LL, P, P]),
+    "tts_gather_rows_bwd_workspace_bytes": (SZ, [LL, LL, LL]),
+    "tts_gather_rows_bwd": (I, [P, LL, LL, LL, I, P, I, P, P, F, LL, P, LL, P, P, P, SZ, P]),
+    "tts_label_log_probs": (I, [P, LL, LL, LL, I, P, I, I, P, P, P, P, P, P]),
+    "tts_label_log_probs_bwd": (I, [P, LL, LL, LL, I, P, I, I, P, P, P, P, P, P, P, P]),
     "tts_fma_probe_flops": (LL, [I, I]),
     "tts_fma_probe": (I, [I, I, P, P]),
     "tts_wsr_dense_fwd": (I, [P, P, P, P, P, P, P, I, I, P, P, P]),

@@ -4,10 +4,14 @@
   ``theta_u_gathered`` (:130-143, the theta kernel in that function's op order, differentiable);
 - ``_operands(model, cam, tmap, R, K)`` (:189-212): geometry, activations, binning and the
   per-tile operand gather, differentiable in the model parameters;
+- ``gather_rows(table, idx, valid, weight, scale)``: the gather through those tables for rows of any
+  width (``conic[idx]``, ``color_o[idx] * valid`` of :203-211, features, label logits, shared
+  codebooks, embeddings), with its gradients;
 - ``_DevRenderBinned.apply(theta_u, color_o, o_col, w_b, Phi, gidx, c_b, H, W)`` (:154-186):
   the per-tile WSR forward and backward on operands in the reference's layout.
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._lib import on_device
 from . import ops
@@ -80,6 +84,68 @@ def theta_u_gathered(conic_t, mu_t, origins, k):
     reference function's op order; differentiable in conic_t and mu_t."""
     with on_device(conic_t):
         return _ThetaGathered.apply(conic_t, mu_t, origins, float(k))
+
+
+class _GatherRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, weight, idx, valid, scale):
+        keep = table if weight is not None and ctx.needs_input_grad[1] else None
+        ctx.save_for_backward(keep, weight, idx, valid)
+        ctx.scale, ctx.R = scale, table.shape[0]
+        return ops.gather_rows(table, idx, valid, weight, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gout):
+        table, weight, idx, valid = ctx.saved_tensors
+        with on_device(gout):
+            gt, gw = ops.gather_rows_bwd(table, ctx.R, idx, valid, weight, ctx.scale, ops.rows2d(gout, gout.shape[1]),
+                                         want_table=ctx.needs_input_grad[0], want_weight=ctx.needs_input_grad[1])
+        return gt, gw, None, None, None
+
+
+def gather_rows(table, idx, valid=None, weight=None, scale=1.0):
+    """Rows of ``table`` [R, ...] by ``idx`` [...] -> [*idx.shape, *table.shape[1:]]: slot n gets
+    scale * weight[n] * table[idx[n]], rounded once to the table's type.
+
+    ``idx`` is int32 or int64: the tables of ``assign_bins`` with their ``valid`` mask, those of
+    ``bin_tables`` (-1 in unused slots), or any ids.  A slot that is not valid, or whose id is
+    negative, gets zeros; an id past the last row is never read and gets NaN.  ``weight`` is
+    float32 with idx's shape.  The table is float32, bfloat16 or float16 with any row stride.
+
+    Differentiable once in ``table`` and ``weight``: a row's gradient is the sum over its uses in a
+    fixed order (fp32 sums, the same bits on every run), [R, ...] in full with zeros for rows that
+    nothing looks up.  To capture a training step in a CUDA graph, take its gradients with
+    ``torch.autograd.grad`` and drop the outputs of eager calls on the same leaves first: torch ties
+    a leaf's gradient to the stream of the graph that is still alive, and the capture fails."""
+    if table.dim() < 1:
+        raise ValueError("table must have at least one dimension")
+    ops.row_type(table, "table")
+    ops.index_type(idx, "idx")
+    shape = idx.shape
+    if valid is not None:
+        if valid.dtype not in (torch.bool, torch.uint8):
+            raise TypeError(f"valid must be bool or uint8, got {valid.dtype}")
+        if valid.shape != shape:
+            raise ValueError(f"valid must have the shape of idx {tuple(shape)}, got {tuple(valid.shape)}")
+        valid = valid.contiguous().view(torch.uint8).reshape(-1)
+    if weight is not None:
+        if weight.dtype != torch.float32:
+            raise TypeError(f"weight must be float32, got {weight.dtype}")
+        if weight.shape != shape:
+            raise ValueError(f"weight must have the shape of idx {tuple(shape)}, got {tuple(weight.shape)}")
+        weight = weight.contiguous().view(-1)
+    width = 1
+    for n in table.shape[1:]:
+        width *= n
+    with on_device(table):
+        rows = ops.rows2d(table, width) if width else table.reshape(table.shape[0], 0)
+        flat = idx.contiguous().view(-1)
+        if torch.is_grad_enabled() and (rows.requires_grad or (weight is not None and weight.requires_grad)):
+            out = _GatherRows.apply(rows, weight, flat, valid, float(scale))
+        else:
+            out = ops.gather_rows(rows, flat, valid, weight, float(scale))
+    return out.view(*shape, *table.shape[1:])
 
 
 class _Operands(torch.autograd.Function):

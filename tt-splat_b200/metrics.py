@@ -2,8 +2,12 @@
 
 ``loss_fn`` runs the fused L1 + SSIM kernel, which returns the loss and its gradient in one
 pass; the autograd backward scales the stored gradient.  Images are [H,W,3] (or [V,H,W,3]).
+``label_log_probs`` scores rows of label logits (a render's [H,W,C], a batch's [N,C]).
 """
+from typing import NamedTuple
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._lib import on_device
 from . import ops
@@ -47,3 +51,63 @@ def ssim(pred, gt, win_size=11):
     the loss 1 - SSIM)."""
     return 1.0 - ops.loss_l1_ssim(pred.detach().float().contiguous(), gt.float().contiguous().to(pred.device),
                                   1.0, 1.0)["loss"].sum()
+
+
+class LabelLogProbs(NamedTuple):
+    logp: torch.Tensor        # [...] log probability of the given label
+    entropy: torch.Tensor     # [...] entropy of the row's distribution
+    top_logp: torch.Tensor    # [..., top] log probabilities of the best labels, best first
+    top_ids: torch.Tensor     # [..., top] their ids (int64)
+
+
+class _LabelLogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, top):
+        logp, entropy, top_logp, top_ids, stats = ops.label_log_probs(logits, labels, top)
+        ctx.save_for_backward(logits, labels, stats, entropy, top_ids)
+        ctx.mark_non_differentiable(top_ids)
+        ctx.set_materialize_grads(False)
+        return logp, entropy, top_logp, top_ids
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_logp, g_entropy, g_top, _):
+        logits, labels, stats, entropy, top_ids = ctx.saved_tensors
+        f = lambda g: None if g is None else g.contiguous()  # noqa: E731
+        with on_device(logits):
+            return ops.label_log_probs_bwd(logits, labels, stats, entropy, top_ids, f(g_logp), f(g_entropy),
+                                           f(g_top)), None, None
+
+
+def label_log_probs(logits, labels, top=0):
+    """Log probabilities of ``labels`` [...] under the softmax of ``logits`` [..., C], with the
+    entropy of each row and its ``top`` (0 to 16) best labels -> ``LabelLogProbs`` in fp32.
+
+    Logits are float32, bfloat16 or float16 with any row stride; labels int32 or int64.  A negative
+    label is unlabelled (log probability 0, no gradient), one past the last gives NaN.  Logits of
+    -inf are masked labels: never among the best (id -1, log probability -inf where fewer are
+    left), and a row of nothing else has log probability -inf, entropy 0 and no gradient.  Ties go
+    to the lowest id.  A row with NaN or +inf has NaN results.
+
+    Differentiable once in the logits through all three; a row whose incoming gradients are zero
+    gets zeros whatever it holds.  To capture a training step in a CUDA graph, take its gradients
+    with ``torch.autograd.grad`` and drop the outputs of eager calls on the same leaves first: torch
+    ties a leaf's gradient to the stream of the graph that is still alive, and the capture fails."""
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits must be [..., C] with at least one label, got {tuple(logits.shape)}")
+    ops.row_type(logits, "logits")
+    ops.index_type(labels, "labels")
+    shape = logits.shape[:-1]
+    if labels.shape != shape:
+        raise ValueError(f"labels must have the shape {tuple(shape)}, got {tuple(labels.shape)}")
+    if not 0 <= int(top) <= 16:
+        raise ValueError(f"top must be 0 to 16, got {top}")
+    top = int(top)
+    with on_device(logits):
+        x = ops.rows2d(logits, logits.shape[-1])
+        t = labels.contiguous().view(-1)
+        if torch.is_grad_enabled() and x.requires_grad:
+            logp, entropy, top_logp, top_ids = _LabelLogProbs.apply(x, t, top)
+        else:
+            logp, entropy, top_logp, top_ids, _ = ops.label_log_probs(x, t, top, want_stats=False)
+    return LabelLogProbs(logp.view(shape), entropy.view(shape), top_logp.view(*shape, top), top_ids.view(*shape, top))

@@ -333,6 +333,101 @@ def unit_from_u8(src, out=None):
     return out
 
 
+_ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_INDEX_TYPES = {torch.int32: 0, torch.int64: 1}
+
+
+def row_type(t, what):
+    """Type code (TTS_ROW_*) of a tensor of rows."""
+    if t.dtype not in _ROW_TYPES:
+        raise TypeError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
+    return _ROW_TYPES[t.dtype]
+
+
+def index_type(t, what):
+    if t.dtype not in _INDEX_TYPES:
+        raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
+    return _INDEX_TYPES[t.dtype]
+
+
+def rows2d(t, width):
+    """[n, width] view of a tensor's rows with unit stride along them (the kernels take any distance
+    between rows, an expanded one included); a copy where no such view exists."""
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
+    return t if width <= 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _dev_rows(*ts):
+    """As _dev, for row tensors that need not be contiguous."""
+    for t in ts:
+        if t is not None:
+            if not t.is_cuda:
+                raise RuntimeError("tt-splat B200 ops need CUDA tensors (no CPU fallback)")
+            if t.device.index != torch.cuda.current_device():
+                raise ValueError(f"tensor on {t.device} but the current device is cuda:{torch.cuda.current_device()}: "
+                                 "call under torch.cuda.device(...) of the tensors' device")
+
+
+def gather_rows(table, idx, valid=None, weight=None, scale=1.0):
+    """out[n] = scale * weight[n] * table[idx[n]] for table [R, C] (unit stride along the rows) and flat
+    contiguous idx, valid (uint8) and weight (float32) of N entries."""
+    _dev_rows(table)
+    _dev(idx, valid, weight)
+    R, C = table.shape
+    N = idx.numel()
+    out = torch.empty(N, C, dtype=table.dtype, device=table.device)
+    call("tts_gather_rows", ptr(table), R, C, table.stride(0), row_type(table, "table"), ptr(idx),
+         index_type(idx, "idx"), ptr(valid), ptr(weight), scale, N, ptr(out), stream())
+    return out
+
+
+def gather_rows_bwd(table, R, idx, valid, weight, scale, gout, want_table=True, want_weight=False):
+    """Gradients of gather_rows from gout [N, C]: gtable [R, C] in gout's type and gweight [N] (each
+    None when not wanted); ``table`` is read for the weight gradient only and may be None without it."""
+    _dev_rows(table, gout)
+    _dev(idx, valid, weight)
+    N, C = gout.shape
+    dev = gout.device
+    gtable = torch.empty(R, C, dtype=gout.dtype, device=dev) if want_table else None
+    gweight = torch.empty(N, device=dev) if want_weight else None
+    nbytes = lib().tts_gather_rows_bwd_workspace_bytes(N, R, C) if want_table else 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if want_table else None
+    call("tts_gather_rows_bwd", ptr(table), R, C, 0 if table is None else table.stride(0), row_type(gout, "gout"),
+         ptr(idx), index_type(idx, "idx"), ptr(valid), ptr(weight), scale, N, ptr(gout), gout.stride(0), ptr(gtable),
+         ptr(gweight), ptr(ws), nbytes, stream())
+    return gtable, gweight
+
+
+def label_log_probs(logits, labels, top=0, want_stats=True):
+    """-> (logp [P], entropy [P], top_logp [P, top], top_ids [P, top] int64, stats [P, 2]) of logits [P, C]
+    (unit stride along the rows) and flat contiguous labels; stats, which only the backward needs, is
+    None when not wanted."""
+    _dev_rows(logits)
+    _dev(labels)
+    P, C = logits.shape
+    dev = logits.device
+    logp, entropy = torch.empty(P, device=dev), torch.empty(P, device=dev)
+    top_logp = torch.empty(P, top, device=dev)
+    top_ids = torch.empty(P, top, dtype=torch.int64, device=dev)
+    stats = torch.empty(P, 2, device=dev) if want_stats else None
+    call("tts_label_log_probs", ptr(logits), P, C, logits.stride(0), row_type(logits, "logits"), ptr(labels),
+         index_type(labels, "labels"), top, ptr(logp), ptr(entropy), ptr(top_logp), ptr(top_ids), ptr(stats), stream())
+    return logp, entropy, top_logp, top_ids, stats
+
+
+def label_log_probs_bwd(logits, labels, stats, entropy, top_ids, g_logp=None, g_entropy=None, g_top=None):
+    """Gradient of label_log_probs in the logits, [P, C] contiguous; absent gradients count as zero."""
+    _dev_rows(logits)
+    _dev(labels, stats, entropy, top_ids, g_logp, g_entropy, g_top)
+    P, C = logits.shape
+    gx = torch.empty(P, C, dtype=logits.dtype, device=logits.device)
+    call("tts_label_log_probs_bwd", ptr(logits), P, C, logits.stride(0), row_type(logits, "logits"), ptr(labels),
+         index_type(labels, "labels"), top_ids.shape[1], ptr(stats), ptr(entropy), ptr(top_ids), ptr(g_logp),
+         ptr(g_entropy), ptr(g_top), ptr(gx), stream())
+    return gx
+
+
 def read_status():
     """Read and clear the device status word (bounded waits that gave up); synchronous."""
     import ctypes
