@@ -385,7 +385,7 @@ int tts_gather_rows_bwd(const void* table, long long R, long long C, long long t
                         size_t workspace_bytes, void* stream);
 
 /* ---- label scores ---------------------------------------------------------------------------
- * Rows of C logits of `type`, row_stride elements apart (P < 2^31 rows, 1 <= C < 2^31); labels [P]
+ * Rows of C logits of `type`, row_stride elements apart (P < 2^31 rows, 1 <= C <= 2^27); labels [P]
  * int32 or (labels64) int64.  logp[P] = log softmax at the label (0 for a negative label, NaN for
  * one >= C), entropy[P] of the softmax, the `top` (0..16) best labels' log probabilities
  * top_logp[P][top] and ids top_ids[P][top], best first, ties to the lowest id, and stats[P][2] =

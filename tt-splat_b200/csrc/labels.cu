@@ -11,145 +11,583 @@
 // the last one gives NaN and reads nothing.  A row whose incoming gradients are all zero gets zeros.
 //
 // stats[r] = (m, log S); log S = -inf marks a row of masked labels only (a real one is at least 0).
+//
+// The running maximum starts at -FLT_MAX, so that x - m is -inf and never NaN for a masked label, and
+// x - m is clamped at D_MIN, where exp is 0 in fp32 already: 0 * D_MIN is 0 in A.  S = 0 then says that
+// nothing was there.  The maximum keeps NaN (max.NaN), so m tells a bad row without a test per element.
+#include <cooperative_groups.h>
 #include <math_constants.h>
 
 #include "rowtype.cuh"
 
 namespace tts {
 
-constexpr int TOP_MAX = 16;
+namespace cg = cooperative_groups;
 
-__device__ __forceinline__ float warp_sum(float x) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-  return x;
+constexpr int TOP_MAX = 16;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float F_LOWEST = -3.402823466e38f;
+constexpr float D_MIN = -500.f;
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// 2^x: at most 2^-22 off relative to the result, results below 2^-126 are 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
+// Part of a row's softmax: the sums are relative to m.
+struct Soft {
+  float m, S, A;
+  __device__ __forceinline__ void init() { m = F_LOWEST, S = 0.f, A = 0.f; }
+  // The sums relative to m2 >= m (or NaN).
+  __device__ __forceinline__ void rebase(float m2) {
+    const float d = fmaxf(m - m2, D_MIN), c = exp2_fast(d * LOG2E);
+    A = c * fmaf(d, S, A);
+    S *= c;
+    m = m2;
+  }
+  __device__ __forceinline__ void add(float x) {
+    const float d = fmaxf(x - m, D_MIN), e = exp2_fast(d * LOG2E);
+    S += e;
+    A = fmaf(e, d, A);
+  }
+  __device__ __forceinline__ void merge(Soft o) {
+    const float m2 = max_nan(m, o.m);
+    rebase(m2);
+    o.rebase(m2);
+    S += o.S;
+    A += o.A;
+  }
+  __device__ __forceinline__ bool bad() const { return !(m < CUDART_INF_F); }
+};
+
+struct ScoreArgs {
+  const void* labels;
+  float* logp;
+  float* entropy;
+  float* top_logp;
+  long long* top_ids;
+  float2* stats;
+  long long C;
+  int labels64, top;
+};
+
+// A row's results but the alternatives; x is the row (global or shared memory).
 template <class T>
-__global__ void __launch_bounds__(256) k_label_scores(const T* __restrict__ logits, long long P, long long C,
-                                                      long long stride, const void* __restrict__ labels, int labels64,
-                                                      int top, float* __restrict__ logp, float* __restrict__ entropy,
-                                                      float* __restrict__ top_logp, long long* __restrict__ top_ids,
-                                                      float2* __restrict__ stats) {
-  const int lane = threadIdx.x & 31;
-  const long long warps = (long long)gridDim.x * (blockDim.x >> 5);
-  for (long long r = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; r < P; r += warps) {
-    const T* x = logits + r * stride;
-    float m = -CUDART_INF_F;
-    bool bad = false;
-    for (long long j = lane; j < C; j += 32) {
-      const float v = to_f32(x[j]);
-      bad |= !(v < CUDART_INF_F);
-      m = fmaxf(m, v);
+__device__ __forceinline__ float2 write_scores(const ScoreArgs& a, long long r, const Soft& s, const T* x) {
+  const bool bad = s.bad(), empty = !bad && s.S == 0.f;
+  const float nan = CUDART_NAN_F;
+  const float m = bad ? nan : (empty ? 0.f : s.m), logS = bad ? nan : (empty ? -CUDART_INF_F : logf(s.S));
+  const long long t = load_index(a.labels, a.labels64, r);
+  float lp = 0.f;
+  if (t >= a.C)
+    lp = nan;
+  else if (t >= 0)
+    lp = empty ? -CUDART_INF_F : (to_f32(x[t]) - m) - logS;
+  a.logp[r] = lp;
+  a.entropy[r] = bad ? nan : (empty ? 0.f : logS - s.A / s.S);
+  if (a.stats) a.stats[r] = make_float2(m, logS);
+  return make_float2(m, logS);
+}
+
+// Alternative k of row r: id -1 where there is none.
+__device__ __forceinline__ void write_top(const ScoreArgs& a, long long r, int k, float v, long long id, float2 st) {
+  a.top_ids[r * a.top + k] = id;
+  a.top_logp[r * a.top + k] = st.y != st.y ? CUDART_NAN_F : (id < 0 ? -CUDART_INF_F : (v - st.x) - st.y);
+}
+
+// ---- vectors of 16 bytes -----------------------------------------------------------------------
+template <class T>
+struct Vec16 {
+  static constexpr int N = 16 / sizeof(T);
+  uint4 w;
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w);
+    } else {
+      const unsigned p = i < 2 ? w.x : i < 4 ? w.y : i < 6 ? w.z : w.w;
+      const unsigned short h = (unsigned short)((i & 1) ? p >> 16 : p & 0xffffu);
+      T t;
+      memcpy(&t, &h, 2);
+      return to_f32(t);
     }
+  }
+  __device__ __forceinline__ void set(int i, float f) {
+    const T t = from_f32<T>(f);
+    unsigned& p = sizeof(T) == 4 ? (i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w)
+                                 : (i < 2 ? w.x : i < 4 ? w.y : i < 6 ? w.z : w.w);
+    if constexpr (sizeof(T) == 4) {
+      p = __float_as_uint(f);
+    } else {
+      unsigned short h;
+      memcpy(&h, &t, 2);
+      p = (i & 1) ? (p & 0xffffu) | ((unsigned)h << 16) : (p & 0xffff0000u) | h;
+    }
+  }
+};
+
+// A row of C elements as `head` single ones up to the first 16-byte boundary, nv vectors and a tail.
+template <class T>
+struct RowSplit {
+  int head, tail;
+  long long nv;
+  __device__ __forceinline__ RowSplit(const T* x, long long C) {
+    const int off = (int)(reinterpret_cast<uintptr_t>(x) & 15u);
+    const long long h = off ? (16 - off) / (int)sizeof(T) : 0;
+    head = (int)(h < C ? h : C);
+    nv = (C - head) / Vec16<T>::N;
+    tail = (int)(C - head - nv * Vec16<T>::N);
+  }
+};
+
+// ---- one block (or a cluster of blocks) per row: many labels -------------------------------------
+constexpr int SB_THREADS = 256;
+constexpr int SB_CAND = 256;      // candidates for the alternatives held in shared memory
+constexpr int SB_CLUSTER = 8;
+
+struct BlockTop {
+  float v[TOP_MAX];
+  long long id[TOP_MAX];
+  int n;
+};
+
+// Whether (v, id) comes before (w, jd): the larger value, among equal ones the lower id.
+__device__ __forceinline__ bool before(float v, long long id, float w, long long jd) {
+  return v > w || (v == w && id < jd);
+}
+
+// The `top` best labels of the block's part of the row, best first.  Threads are 8 to a group; the k-th
+// largest of the 32 groups' maxima is a bound that at least k elements reach and few more (about 1.4 k
+// for distinct random values), and only threads whose own maximum reaches it hold any: their elements
+// alone are read again.  More candidates than fit (long runs of equal values): one pass for each
+// alternative.
+template <class T>
+__device__ void block_top(const T* x, const RowSplit<T>& rs, long long lo, long long hi, bool ends, float tmax, int top,
+                          BlockTop* out) {
+  constexpr int N = Vec16<T>::N;
+  __shared__ float s_g[32];
+  __shared__ float s_T;
+  __shared__ int s_nq, s_nc;
+  __shared__ unsigned char s_q[SB_THREADS];
+  __shared__ float s_v[SB_CAND];
+  __shared__ long long s_id[SB_CAND];
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  float g = tmax;
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    bad = __any_sync(0xffffffffu, bad);
-    const bool empty = !bad && m == -CUDART_INF_F;
-    float S = 0.f, A = 0.f;
-    if (!bad && !empty)
-      for (long long j = lane; j < C; j += 32) {
-        const float d = to_f32(x[j]) - m, e = expf(d);
-        S += e;
-        if (e > 0.f) A = fmaf(e, d, A);
+  for (int d = 4; d > 0; d >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, d));
+  if ((lane & 7) == 0) s_g[wid * 4 + (lane >> 3)] = g;
+  if (tid == 0) s_nq = s_nc = 0;
+  __syncthreads();
+  if (wid == 0) {
+    const float mine = s_g[lane];
+    int rank = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) rank += before(s_g[i], i, mine, lane);
+    if (rank == top - 1) s_T = mine;
+  }
+  __syncthreads();
+  const float T0 = s_T;
+  if (tmax >= T0) s_q[atomicAdd(&s_nq, 1)] = (unsigned char)tid;
+  __syncthreads();
+  auto consider = [&](float v, long long id) {
+    if (v >= T0) {
+      const int c = atomicAdd(&s_nc, 1);
+      if (c < SB_CAND) {
+        s_v[c] = v;
+        s_id[c] = id;
       }
-    S = warp_sum(S);
-    A = warp_sum(A);
-    const float nan = CUDART_NAN_F;
-    const float logS = bad ? nan : (empty ? -CUDART_INF_F : logf(S));
-    const float base = bad ? nan : (empty ? 0.f : m);
-    if (lane == 0) {
-      const long long t = load_index(labels, labels64, r);
-      float lp = 0.f;
-      if (t >= C)
-        lp = nan;
-      else if (t >= 0)
-        lp = bad ? nan : (empty ? -CUDART_INF_F : (to_f32(x[t]) - base) - logS);
-      logp[r] = lp;
-      entropy[r] = bad ? nan : (empty ? 0.f : logS - A / S);
-      if (stats) stats[r] = make_float2(base, logS);
     }
-    // the k-th best is the best of those behind the (k-1)-th in the order (value down, id up)
-    float pv = CUDART_INF_F;
-    long long pi = -1;
-    for (int k = 0; k < top; ++k) {
-      float bv = -CUDART_INF_F;
-      long long bi = C;
-      if (!bad)
-        for (long long j = lane; j < C; j += 32) {
-          const float v = to_f32(x[j]);
-          if ((v < pv || (v == pv && j > pi)) && v > bv) {
-            bv = v;
-            bi = j;
-          }
-        }
+  };
+  const int rounds = (int)((hi - lo + SB_THREADS - 1) / SB_THREADS);
+  const long long work = (long long)s_nq * rounds;
+  const uint4* xv = reinterpret_cast<const uint4*>(x + rs.head);
+  for (long long p = tid; p < work; p += SB_THREADS) {
+    const int q = (int)(p / rounds);
+    const long long v = lo + s_q[q] + (p - (long long)q * rounds) * SB_THREADS;
+    if (v >= hi) continue;
+    const Vec16<T> w{__ldg(xv + v)};
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) {
+    for (int e = 0; e < N; ++e) consider(w.get(e), rs.head + v * N + e);
+  }
+  const long long t0 = rs.head + rs.nv * N;
+  if (ends && tid < rs.head) consider(to_f32(x[tid]), tid);
+  if (ends && tid < rs.tail) consider(to_f32(x[t0 + tid]), t0 + tid);
+  __syncthreads();
+  const int nc = s_nc;
+  if (nc <= SB_CAND) {
+    if (tid < nc) {
+      const float v = s_v[tid];
+      const long long id = s_id[tid];
+      int rank = 0;
+      for (int i = 0; i < nc; ++i) rank += before(s_v[i], s_id[i], v, id);
+      if (rank < top) {
+        out->v[rank] = v;
+        out->id[rank] = id;
+      }
+    }
+    if (tid == 0) out->n = nc < top ? nc : top;
+    __syncthreads();
+    return;
+  }
+  float pv = CUDART_INF_F;
+  long long pid = -1;
+  int k = 0;
+  for (; k < top; ++k) {
+    float bv = -CUDART_INF_F;
+    long long bi = -1;
+    auto look = [&](float v, long long id) {
+      if (before(pv, pid, v, id) && v > bv) bv = v, bi = id;
+    };
+    if (ends && tid < rs.head) look(to_f32(x[tid]), tid);
+    for (long long v = lo + tid; v < hi; v += SB_THREADS) {
+      const Vec16<T> w{__ldg(xv + v)};
+#pragma unroll
+      for (int e = 0; e < N; ++e) look(w.get(e), rs.head + v * N + e);
+    }
+    if (ends && tid < rs.tail) look(to_f32(x[t0 + tid]), t0 + tid);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+      const float ov = __shfl_xor_sync(0xffffffffu, bv, d);
+      const long long oi = __shfl_xor_sync(0xffffffffu, bi, d);
+      if (oi >= 0 && (bi < 0 || before(ov, oi, bv, bi))) bv = ov, bi = oi;
+    }
+    __syncthreads();
+    if (lane == 0) s_v[wid] = bv, s_id[wid] = bi;
+    __syncthreads();
+    bv = s_v[0], bi = s_id[0];
+    for (int w = 1; w < SB_THREADS / 32; ++w)
+      if (s_id[w] >= 0 && (bi < 0 || before(s_v[w], s_id[w], bv, bi))) bv = s_v[w], bi = s_id[w];
+    if (bi < 0) break;
+    if (tid == 0) out->v[k] = bv, out->id[k] = bi;
+    pv = bv;
+    pid = bi;
+  }
+  if (tid == 0) out->n = k;
+  __syncthreads();
+}
+
+// One pass over the row with each thread's own running maximum and sums (UNROLL vectors in flight), then
+// one merge; the blocks of a cluster take a part of the row each and the first one merges theirs through
+// distributed shared memory.
+template <class T>
+__global__ void __launch_bounds__(SB_THREADS) k_scores_block(const T* __restrict__ logits, long long stride, int cs,
+                                                             ScoreArgs a) {
+  constexpr int N = Vec16<T>::N, UNROLL = 4;
+  __shared__ Soft s_soft[SB_THREADS / 32];
+  __shared__ Soft s_all;
+  __shared__ BlockTop s_top;
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  const long long r = blockIdx.x / cs;
+  const int rank = blockIdx.x % cs;
+  const T* x = logits + r * stride;
+  const RowSplit<T> rs(x, a.C);
+  const long long lo = rs.nv * rank / cs, hi = rs.nv * (rank + 1) / cs;
+  const uint4* xv = reinterpret_cast<const uint4*>(x + rs.head);
+  Soft s;
+  s.init();
+  if (rank == 0) {
+    float h = -CUDART_INF_F, t = -CUDART_INF_F;
+    if (tid < rs.head) h = to_f32(x[tid]);
+    if (tid < rs.tail) t = to_f32(x[rs.head + rs.nv * N + tid]);
+    s.m = max_nan(s.m, max_nan(h, t));
+    s.add(h);
+    s.add(t);
+  }
+  for (long long v0 = lo + tid; v0 < hi; v0 += UNROLL * SB_THREADS) {
+    Vec16<T> w[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const long long v = v0 + u * SB_THREADS;
+      if (v < hi) w[u].w = __ldg(xv + v);
+    }
+    float m = s.m;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (v0 + u * SB_THREADS < hi) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) m = max_nan(m, w[u].get(e));
+      }
+    if (!(m == s.m)) s.rebase(m);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (v0 + u * SB_THREADS < hi) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) s.add(w[u].get(e));
+      }
+  }
+  const float tmax = s.m;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    Soft o;
+    o.m = __shfl_xor_sync(0xffffffffu, s.m, d);
+    o.S = __shfl_xor_sync(0xffffffffu, s.S, d);
+    o.A = __shfl_xor_sync(0xffffffffu, s.A, d);
+    s.merge(o);
+  }
+  if (lane == 0) s_soft[wid] = s;
+  __syncthreads();
+  s = s_soft[0];
+#pragma unroll
+  for (int w = 1; w < SB_THREADS / 32; ++w) s.merge(s_soft[w]);
+  if (tid == 0) {
+    s_all = s;
+    s_top.n = 0;
+  }
+  __syncthreads();
+  if (a.top > 0 && !s.bad()) block_top<T>(x, rs, lo, hi, rank == 0, tmax, a.top, &s_top);
+  if (cs == 1) {
+    float2 st;
+    if (tid == 0) {
+      s_all = s;
+      st = write_scores(a, r, s, x);
+      s_soft[0].m = st.x, s_soft[0].S = st.y;
+    }
+    if (a.top > 0) {
+      __syncthreads();
+      if (tid < a.top)
+        write_top(a, r, tid, s_top.v[tid], tid < s_top.n ? s_top.id[tid] : -1, make_float2(s_soft[0].m, s_soft[0].S));
+    }
+    return;
+  }
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  if (rank == 0 && wid == 0) {
+    Soft all = s;
+    for (int b = 1; b < cs; ++b) all.merge(*cluster.map_shared_rank(&s_all, b));
+    float2 st;
+    if (lane == 0) st = write_scores(a, r, all, x);
+    st.x = __shfl_sync(0xffffffffu, st.x, 0);
+    st.y = __shfl_sync(0xffffffffu, st.y, 0);
+    const BlockTop* mine = lane < cs ? cluster.map_shared_rank(&s_top, lane) : &s_top;
+    const int n = lane < cs && !all.bad() ? mine->n : 0;
+    int at = 0;
+    for (int k = 0; k < a.top; ++k) {
+      float bv = at < n ? mine->v[at] : -CUDART_INF_F;
+      long long bi = at < n ? mine->id[at] : -1;
+      const long long own = bi;
+#pragma unroll
+      for (int d = SB_CLUSTER / 2; d > 0; d >>= 1) {
         const float ov = __shfl_xor_sync(0xffffffffu, bv, d);
         const long long oi = __shfl_xor_sync(0xffffffffu, bi, d);
-        if (ov > bv || (ov == bv && oi < bi)) {
-          bv = ov;
-          bi = oi;
-        }
+        if (oi >= 0 && (bi < 0 || before(ov, oi, bv, bi))) bv = ov, bi = oi;
       }
-      if (lane == 0) {
-        top_ids[r * top + k] = bi < C ? bi : -1;
-        top_logp[r * top + k] = bad ? nan : (bi < C ? (bv - base) - logS : -CUDART_INF_F);
-      }
-      pv = bv;
-      pi = bi;
+      bv = __shfl_sync(0xffffffffu, bv, 0);
+      bi = __shfl_sync(0xffffffffu, bi, 0);
+      if (bi >= 0 && own == bi) ++at;
+      if (lane == 0) write_top(a, r, k, bv, bi, st);
     }
+  }
+  cluster.sync();
+}
+
+// ---- one warp per row ----------------------------------------------------------------------------
+template <class T>
+__global__ void __launch_bounds__(256) k_scores_warp(const T* __restrict__ logits, long long P, long long stride,
+                                                     ScoreArgs a) {
+  const int lane = threadIdx.x & 31;
+  const long long r = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  if (r >= P) return;
+  const T* x = logits + r * stride;
+  const int C = (int)a.C;
+  Soft s;
+  s.init();
+  for (int j = lane; j < C; j += 32) s.m = max_nan(s.m, to_f32(x[j]));
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) s.m = max_nan(s.m, __shfl_xor_sync(0xffffffffu, s.m, d));
+  for (int j = lane; j < C; j += 32) s.add(to_f32(x[j]));
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    s.S += __shfl_xor_sync(0xffffffffu, s.S, d);
+    s.A += __shfl_xor_sync(0xffffffffu, s.A, d);
+  }
+  float2 st;
+  if (lane == 0) st = write_scores(a, r, s, x);
+  st.x = __shfl_sync(0xffffffffu, st.x, 0);
+  st.y = __shfl_sync(0xffffffffu, st.y, 0);
+  // the k-th best is the best of those behind the (k-1)-th in the order (value down, id up)
+  float pv = CUDART_INF_F;
+  int pid = -1;
+  for (int k = 0; k < a.top; ++k) {
+    float bv = -CUDART_INF_F;
+    int bi = C;
+    if (!s.bad())
+      for (int j = lane; j < C; j += 32) {
+        const float v = to_f32(x[j]);
+        if (before(pv, pid, v, j) && v > bv) bv = v, bi = j;
+      }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+      const float ov = __shfl_xor_sync(0xffffffffu, bv, d);
+      const int oi = __shfl_xor_sync(0xffffffffu, bi, d);
+      if (before(ov, oi, bv, bi)) bv = ov, bi = oi;
+    }
+    if (lane == 0) write_top(a, r, k, bv, bi < C ? bi : -1, st);
+    pv = bv;
+    pid = bi;
+  }
+}
+
+// ---- the gradient -----------------------------------------------------------------------------------
+struct GradArgs {
+  const void* labels;
+  const float2* stats;
+  const float* entropy;
+  const long long* top_ids;
+  const float* g_logp;
+  const float* g_entropy;
+  const float* g_top;
+  long long C;
+  int labels64, top;
+};
+
+// With d = x - m:  dx = p (alpha - g_H d),  p = exp(d - log S),  alpha = -total - g_H (H - log S).
+struct RowGrad {
+  float m, c, alpha, gh, gl;
+  long long t;
+  bool zero;      // nothing comes in: zeros, whatever the row holds
+  bool empty;     // masked labels only: zeros
+  __device__ __forceinline__ RowGrad(const GradArgs& a, long long r) {
+    const float2 st = a.stats[r];
+    gh = a.g_entropy ? a.g_entropy[r] : 0.f;
+    t = load_index(a.labels, a.labels64, r);
+    gl = 0.f;
+    if (a.g_logp && t >= 0) gl = t < a.C ? a.g_logp[r] : CUDART_NAN_F;
+    float total = gl;
+    if (a.g_top)
+      for (int k = 0; k < a.top; ++k)
+        if (a.top_ids[r * a.top + k] >= 0) total += a.g_top[r * a.top + k];
+    m = st.x;
+    c = -st.y * LOG2E;
+    alpha = st.y != st.y ? CUDART_NAN_F : -total - gh * (a.entropy[r] - st.y);
+    zero = total == 0.f && gh == 0.f;
+    empty = st.y == -CUDART_INF_F;
+    if (empty) gl = 0.f;
+    if (zero || empty) m = 0.f, c = 0.f, alpha = 0.f, gh = 0.f;
+  }
+  __device__ __forceinline__ float operator()(float x) const {
+    const float d = fmaxf(x - m, D_MIN);
+    return exp2_fast(fmaf(d, LOG2E, c)) * fmaf(-gh, d, alpha);
+  }
+  // The gradient at label j, which the given label or alternatives hit.
+  __device__ __forceinline__ float special(const GradArgs& a, long long r, long long j, float x) const {
+    float g = zero || empty ? 0.f : (*this)(x);
+    if (j == t) g += gl;
+    if (a.g_top && !empty)
+      for (int k = 0; k < a.top; ++k)
+        if (a.top_ids[r * a.top + k] == j) g += a.g_top[r * a.top + k];
+    return g;
+  }
+};
+
+constexpr int GB_THREADS = 256;
+constexpr int GB_UNROLL = 4;
+
+// Blocks of one row each (blockIdx.x: row, blockIdx.y: part of its vectors); the labels whose gradient has
+// a term of its own are stored last, behind a barrier.
+template <class T, bool SAME>
+__global__ void __launch_bounds__(GB_THREADS) k_scores_grad_block(const T* __restrict__ logits, long long stride, GradArgs a,
+                                                                  T* __restrict__ glogits) {
+  constexpr int N = Vec16<T>::N;
+  const long long r = blockIdx.x;
+  const T* x = logits + r * stride;
+  T* gx = glogits + r * a.C;
+  const RowGrad g(a, r);
+  const bool none = g.zero || g.empty;
+  const RowSplit<T> rs(gx, a.C);
+  const long long per = (long long)GB_THREADS * GB_UNROLL;
+  const long long lo = blockIdx.y * per, hi = lo + per < rs.nv ? lo + per : rs.nv;
+  const long long j0 = blockIdx.y == 0 ? 0 : rs.head + lo * N;
+  const long long j1 = blockIdx.y == gridDim.y - 1 ? a.C : rs.head + hi * N;
+  const uint4* xv = reinterpret_cast<const uint4*>(x + rs.head);
+  uint4* gv = reinterpret_cast<uint4*>(gx + rs.head);
+  Vec16<T> w[GB_UNROLL];
+#pragma unroll
+  for (int u = 0; u < GB_UNROLL; ++u) {
+    const long long v = lo + u * GB_THREADS + threadIdx.x;
+    if (v < hi && !none) {
+      if constexpr (SAME) {
+        w[u].w = __ldcs(xv + v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[u].set(e, to_f32(x[rs.head + v * N + e]));
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < GB_UNROLL; ++u) {
+    const long long v = lo + u * GB_THREADS + threadIdx.x;
+    if (v < hi) {
+      Vec16<T> o;
+#pragma unroll
+      for (int e = 0; e < N; ++e) o.set(e, none ? 0.f : g(w[u].get(e)));
+      __stcs(gv + v, o.w);
+    }
+  }
+  if (blockIdx.y == 0 && threadIdx.x < rs.head)
+    gx[threadIdx.x] = from_f32<T>(none ? 0.f : g(to_f32(x[threadIdx.x])));
+  if (blockIdx.y == gridDim.y - 1 && threadIdx.x < rs.tail) {
+    const long long j = a.C - rs.tail + threadIdx.x;
+    gx[j] = from_f32<T>(none ? 0.f : g(to_f32(x[j])));
+  }
+  __syncthreads();
+  if (threadIdx.x <= (a.g_top ? a.top : 0)) {
+    const long long j = threadIdx.x == 0 ? g.t : a.top_ids[r * a.top + threadIdx.x - 1];
+    if (j >= j0 && j < j1) gx[j] = from_f32<T>(g.special(a, r, j, to_f32(x[j])));
   }
 }
 
 template <class T>
-__global__ void __launch_bounds__(256) k_label_scores_bwd(const T* __restrict__ logits, long long P, long long C,
-                                                          long long stride, const void* __restrict__ labels, int labels64,
-                                                          int top, const float2* __restrict__ stats,
-                                                          const float* __restrict__ entropy,
-                                                          const long long* __restrict__ top_ids,
-                                                          const float* __restrict__ g_logp,
-                                                          const float* __restrict__ g_entropy,
-                                                          const float* __restrict__ g_top, T* __restrict__ glogits) {
+__global__ void __launch_bounds__(256) k_scores_grad_warp(const T* __restrict__ logits, long long P, long long stride,
+                                                          GradArgs a, T* __restrict__ glogits) {
   const int lane = threadIdx.x & 31;
-  const long long warps = (long long)gridDim.x * (blockDim.x >> 5);
-  for (long long r = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; r < P; r += warps) {
-    const T* x = logits + r * stride;
-    T* gx = glogits + r * C;
-    const float2 st = stats[r];
-    const float H = entropy[r], gh = g_entropy ? g_entropy[r] : 0.f;
-    const long long t = load_index(labels, labels64, r);
-    float gl = 0.f;
-    if (g_logp && t >= 0) gl = t < C ? g_logp[r] : CUDART_NAN_F;
-    float total = gl;
-    if (g_top)
-      for (int k = 0; k < top; ++k)
-        if (top_ids[r * top + k] >= 0) total += g_top[r * top + k];
-    const bool zero = st.y == -CUDART_INF_F, plain = total == 0.f && gh == 0.f;
-    for (long long j = lane; j < C; j += 32) {
-      float g = 0.f;
-      if (!plain) {
-        const float lp = (to_f32(x[j]) - st.x) - st.y, p = expf(lp);
-        g = p == 0.f ? 0.f : p * (-total - gh * (lp + H));
-      }
-      if (j == t) g += gl;
-      if (g_top)
-        for (int k = 0; k < top; ++k)
-          if (top_ids[r * top + k] == j) g += g_top[r * top + k];
-      gx[j] = from_f32<T>(zero ? 0.f : g);
-    }
+  const long long r = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  if (r >= P) return;
+  const T* x = logits + r * stride;
+  T* gx = glogits + r * a.C;
+  const RowGrad g(a, r);
+  const bool none = g.zero || g.empty;
+  const int C = (int)a.C;
+  for (int j = lane; j < C; j += 32) gx[j] = from_f32<T>(none ? 0.f : g(to_f32(x[j])));
+  __syncwarp();
+  if (lane <= (a.g_top ? a.top : 0)) {
+    const long long j = lane == 0 ? g.t : a.top_ids[r * a.top + lane - 1];
+    if (j >= 0 && j < C) gx[j] = from_f32<T>(g.special(a, r, j, to_f32(x[j])));
   }
 }
 
-static unsigned warp_grid(long long items) {
-  long long b = (items + 7) / 8;
-  return (unsigned)(b < 148 * 64 ? b : 148 * 64);
-}
+constexpr long long WARP_ROW_MAX = 1024;      // labels up to which a warp takes a row
+
 static int check_labels(long long P, long long C, int type, int top) {
   TTS_REQUIRE(type >= TTS_ROW_F32 && type <= TTS_ROW_F16, "unknown row type");
   TTS_REQUIRE(P >= 0 && P < (1ll << 31), "the number of rows must be below 2^31");
-  TTS_REQUIRE(C >= 1 && C < (1ll << 31), "the number of labels must be at least 1 and below 2^31");
+  TTS_REQUIRE(C >= 1 && C <= (1ll << 27), "the number of labels must be 1 to 2^27");
   TTS_REQUIRE(top >= 0 && top <= TOP_MAX, "top must be 0 to 16");
+  return TTS_OK;
+}
+
+template <class T>
+static int launch_scores_block(const T* x, long long P, long long stride, const ScoreArgs& a, cudaStream_t st) {
+  // few rows: a cluster of blocks for each, as long as that fills the SMs and leaves every block 2048 labels
+  int cs = 1;
+  while (cs < SB_CLUSTER && P * cs * 2 <= 148 * 4 && a.C / (cs * 2) >= 2048) cs *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(P * cs));
+  cfg.blockDim = dim3(SB_THREADS);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cs;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cs > 1 ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, k_scores_block<T>, x, stride, cs, a) != cudaSuccess)
+    return check_launch("label_log_probs (block per row)");
   return TTS_OK;
 }
 
@@ -164,11 +602,16 @@ extern "C" int tts_label_log_probs(const void* logits, long long P, long long C,
   if (P == 0) return TTS_OK;
   TTS_REQUIRE(logits && labels && logp && entropy && (top == 0 || (top_logp && top_ids)),
               "null label_log_probs argument");
+  const ScoreArgs a{labels, logp, entropy, top_logp, reinterpret_cast<long long*>(top_ids), reinterpret_cast<float2*>(stats),
+                    C, labels64, top};
   return with_row_type(type, [&](auto t) {
     using T = decltype(t);
-    k_label_scores<T><<<warp_grid(P), 256, 0, as_stream(stream)>>>(
-        static_cast<const T*>(logits), P, C, row_stride, labels, labels64, top, logp, entropy, top_logp,
-        reinterpret_cast<long long*>(top_ids), reinterpret_cast<float2*>(stats));
+    const T* x = static_cast<const T*>(logits);
+    if (C <= WARP_ROW_MAX) {
+      k_scores_warp<T><<<(unsigned)((P + 7) / 8), 256, 0, as_stream(stream)>>>(x, P, row_stride, a);
+    } else if (int rc = launch_scores_block<T>(x, P, row_stride, a, as_stream(stream))) {
+      return rc;
+    }
     return check_launch("label_log_probs");
   });
 }
@@ -181,11 +624,26 @@ extern "C" int tts_label_log_probs_bwd(const void* logits, long long P, long lon
   if (P == 0) return TTS_OK;
   TTS_REQUIRE(logits && labels && stats && entropy && glogits && (!g_top || top == 0 || top_ids),
               "null label_log_probs_bwd argument");
+  const GradArgs a{labels, reinterpret_cast<const float2*>(stats), entropy, reinterpret_cast<const long long*>(top_ids),
+                   g_logp, g_entropy, top > 0 ? g_top : nullptr, C, labels64, top};
+  cudaStream_t st = as_stream(stream);
   return with_row_type(type, [&](auto t) {
     using T = decltype(t);
-    k_label_scores_bwd<T><<<warp_grid(P), 256, 0, as_stream(stream)>>>(
-        static_cast<const T*>(logits), P, C, row_stride, labels, labels64, top, reinterpret_cast<const float2*>(stats),
-        entropy, reinterpret_cast<const long long*>(top_ids), g_logp, g_entropy, g_top, static_cast<T*>(glogits));
+    const T* x = static_cast<const T*>(logits);
+    T* gx = static_cast<T*>(glogits);
+    if (C <= WARP_ROW_MAX) {
+      k_scores_grad_warp<T><<<(unsigned)((P + 7) / 8), 256, 0, st>>>(x, P, row_stride, a, gx);
+    } else {
+      // the logits' 16-byte vectors line up with the gradient's when both start on the same offset in every row
+      const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(gx)) & 15u) == 0 &&
+                        (row_stride - C) * (long long)sizeof(T) % 16 == 0;
+      const long long vecs = C / Vec16<T>::N, per = (long long)GB_THREADS * GB_UNROLL;
+      const dim3 grid((unsigned)P, (unsigned)((vecs + per - 1) / per));
+      if (same)
+        k_scores_grad_block<T, true><<<grid, GB_THREADS, 0, st>>>(x, row_stride, a, gx);
+      else
+        k_scores_grad_block<T, false><<<grid, GB_THREADS, 0, st>>>(x, row_stride, a, gx);
+    }
     return check_launch("label_log_probs_bwd");
   });
 }
