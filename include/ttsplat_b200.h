@@ -54,7 +54,8 @@ const char* tts_last_error(void);
 
 /* Device status word written by kernels instead of trapping (bounded waits that gave up):
  * 1 = a bulk-copy wait of the forward, 2 = a relocation grid barrier, 4 = a peer barrier;
- * 8 = a cached binning table that spreads a gaussian over more than its stencil.
+ * 8 = a cached binning table that spreads a gaussian over more than its stencil;
+ * 16 = a wait of the row gradient's sort.
  * Synchronous read + clear.  A non-zero word means a step skipped work: the Python train step
  * reads it at check_status / check_replicas and at the end of fit / train_mcmc, and raises. */
 int tts_read_status(int* status_host);
@@ -364,7 +365,7 @@ int tts_unit_from_u8(const uint8_t* src, long long n, float* dst, void* stream);
  * The gather of per-gaussian rows by an (idx, valid) table, `conic[idx]` and `color_o[idx] * valid`
  * of tools/m4_train_binned.py:203-211, for rows of any width, and its transpose.
  * table [R] rows of C elements of `type`, table_stride elements apart; idx [N] int32 or (idx64)
- * int64; valid [N] uint8 or NULL; weight [N] fp32 or NULL; N < 2^31, R < 2^31 - 1, C < 2^31.
+ * int64; valid [N] uint8 or NULL; weight [N] fp32 or NULL; N < 2^30, R < 2^31 - 1, C <= 2^22.
  * out[N][C] = scale * weight[n] * table[idx[n]], rounded once; a slot with valid 0 or a negative
  * idx gives zeros, an idx >= R is not read and gives NaN. */
 #define TTS_ROW_F32 0

@@ -5,6 +5,7 @@ The library is loaded on first use from this package directory (it is built in-t
 tensor raises.  Every call passes the current torch CUDA stream, so the ops order with torch
 work and can be captured in CUDA graphs.
 """
+import contextlib
 import ctypes as C
 import os
 
@@ -138,19 +139,21 @@ def stream(device=None):
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+_NO_CONTEXT = contextlib.nullcontext()
+
+
 def on_device(t):
-    """Context selecting a CUDA tensor's device (a no-op for anything else: the ops then raise)."""
-    import contextlib
-    if isinstance(t, torch.Tensor) and t.is_cuda:
+    """Context selecting a CUDA tensor's device (a no-op where that is the current one already, and for
+    anything else: the ops then raise)."""
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.device.index != torch.cuda.current_device():
         return torch.cuda.device(t.device)
-    return contextlib.nullcontext()
+    return _NO_CONTEXT
 
 
 def device_ctx(device):
     """Context selecting a torch CUDA device (a no-op for any other device)."""
-    import contextlib
     device = torch.device(device)
-    return torch.cuda.device(device) if device.type == "cuda" else contextlib.nullcontext()
+    return torch.cuda.device(device) if device.type == "cuda" else _NO_CONTEXT
 
 
 def require_cuda():

@@ -88,20 +88,26 @@ def theta_u_gathered(conic_t, mu_t, origins, k):
 
 class _GatherRows(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, table, weight, idx, valid, scale):
-        keep = table if weight is not None and ctx.needs_input_grad[1] else None
-        ctx.save_for_backward(keep, weight, idx, valid)
-        ctx.scale, ctx.R = scale, table.shape[0]
-        return ops.gather_rows(table, idx, valid, weight, scale)
+    def forward(ctx, table, weight, idx, valid, scale, row_shape):
+        ctx.save_for_backward(table if ctx.needs_input_grad[1] else None, weight, idx, valid)
+        ctx.scale, ctx.R, ctx.row_shape = scale, table.shape[0], row_shape
+        return ops.gather_rows(table, idx, valid, weight, scale, row_shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
         table, weight, idx, valid = ctx.saved_tensors
+        width = 1
+        for n in ctx.row_shape:
+            width *= n
+        if width:
+            gout = ops.rows2d(gout, width)
+        else:
+            gout = gout.reshape(idx.numel(), 0)
         with on_device(gout):
-            gt, gw = ops.gather_rows_bwd(table, ctx.R, idx, valid, weight, ctx.scale, ops.rows2d(gout, gout.shape[1]),
+            gt, gw = ops.gather_rows_bwd(table, ctx.R, idx, valid, weight, ctx.scale, gout,
                                          want_table=ctx.needs_input_grad[0], want_weight=ctx.needs_input_grad[1])
-        return gt, gw, None, None, None
+        return gt, gw, None, None, None, None
 
 
 def gather_rows(table, idx, valid=None, weight=None, scale=1.0):
@@ -122,30 +128,28 @@ def gather_rows(table, idx, valid=None, weight=None, scale=1.0):
         raise ValueError("table must have at least one dimension")
     ops.row_type(table, "table")
     ops.index_type(idx, "idx")
-    shape = idx.shape
+    shape, row_shape = idx.shape, tuple(table.shape[1:])
+    idx = idx.contiguous()
     if valid is not None:
         if valid.dtype not in (torch.bool, torch.uint8):
             raise TypeError(f"valid must be bool or uint8, got {valid.dtype}")
         if valid.shape != shape:
             raise ValueError(f"valid must have the shape of idx {tuple(shape)}, got {tuple(valid.shape)}")
-        valid = valid.contiguous().view(torch.uint8).reshape(-1)
+        valid = valid.contiguous()
     if weight is not None:
         if weight.dtype != torch.float32:
             raise TypeError(f"weight must be float32, got {weight.dtype}")
         if weight.shape != shape:
             raise ValueError(f"weight must have the shape of idx {tuple(shape)}, got {tuple(weight.shape)}")
-        weight = weight.contiguous().view(-1)
+        weight = weight.contiguous()
     width = 1
-    for n in table.shape[1:]:
+    for n in row_shape:
         width *= n
     with on_device(table):
-        rows = ops.rows2d(table, width) if width else table.reshape(table.shape[0], 0)
-        flat = idx.contiguous().view(-1)
+        rows = ops.rows2d(table, width)
         if torch.is_grad_enabled() and (rows.requires_grad or (weight is not None and weight.requires_grad)):
-            out = _GatherRows.apply(rows, weight, flat, valid, float(scale))
-        else:
-            out = ops.gather_rows(rows, flat, valid, weight, float(scale))
-    return out.view(*shape, *table.shape[1:])
+            return _GatherRows.apply(rows, weight, idx, valid, float(scale), row_shape)
+        return ops.gather_rows(rows, idx, valid, weight, float(scale), row_shape)
 
 
 class _Operands(torch.autograd.Function):

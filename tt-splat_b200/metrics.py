@@ -103,11 +103,9 @@ def label_log_probs(logits, labels, top=0):
     if not 0 <= int(top) <= 16:
         raise ValueError(f"top must be 0 to 16, got {top}")
     top = int(top)
+    labels = labels.contiguous()
     with on_device(logits):
         x = ops.rows2d(logits, logits.shape[-1])
-        t = labels.contiguous().view(-1)
         if torch.is_grad_enabled() and x.requires_grad:
-            logp, entropy, top_logp, top_ids = _LabelLogProbs.apply(x, t, top)
-        else:
-            logp, entropy, top_logp, top_ids, _ = ops.label_log_probs(x, t, top, want_stats=False)
-    return LabelLogProbs(logp.view(shape), entropy.view(shape), top_logp.view(*shape, top), top_ids.view(*shape, top))
+            return LabelLogProbs(*_LabelLogProbs.apply(x, labels, top))
+        return LabelLogProbs(*ops.label_log_probs(x, labels, top, want_stats=False)[:4])

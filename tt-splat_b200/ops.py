@@ -354,77 +354,96 @@ def rows2d(t, width):
     """[n, width] view of a tensor's rows with unit stride along them (the kernels take any distance
     between rows, an expanded one included); a copy where no such view exists."""
     if t.dim() != 2:
-        t = t.reshape(-1, width)
+        t = t.reshape(-1, width) if width else t.reshape(t.shape[0], 0)
     return t if width <= 1 or t.stride(1) == 1 else t.contiguous()
 
 
-def _dev_rows(*ts):
-    """As _dev, for row tensors that need not be contiguous."""
-    for t in ts:
+def _addr(t):
+    """Device address of a tensor that has passed _dev or _dev_rows, or was allocated here."""
+    return None if t is None else t.data_ptr()
+
+
+def _stream(index):
+    """Current stream of the current device ``index``."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _dev_rows(rows, *flat):
+    """As _dev, with a first tensor of rows that need not be contiguous; returns the device index."""
+    if not rows.is_cuda:
+        raise RuntimeError("tt-splat B200 ops need CUDA tensors (no CPU fallback)")
+    cur = torch.cuda.current_device()
+    for t in (rows, *flat):
         if t is not None:
             if not t.is_cuda:
                 raise RuntimeError("tt-splat B200 ops need CUDA tensors (no CPU fallback)")
-            if t.device.index != torch.cuda.current_device():
-                raise ValueError(f"tensor on {t.device} but the current device is cuda:{torch.cuda.current_device()}: "
+            if t is not rows and not t.is_contiguous():
+                raise ValueError("tensors must be contiguous")
+            if t.device.index != cur:
+                raise ValueError(f"tensor on {t.device} but the current device is cuda:{cur}: "
                                  "call under torch.cuda.device(...) of the tensors' device")
+    return cur
 
 
-def gather_rows(table, idx, valid=None, weight=None, scale=1.0):
-    """out[n] = scale * weight[n] * table[idx[n]] for table [R, C] (unit stride along the rows) and flat
-    contiguous idx, valid (uint8) and weight (float32) of N entries."""
-    _dev_rows(table)
-    _dev(idx, valid, weight)
+def gather_rows(table, idx, valid=None, weight=None, scale=1.0, row_shape=None):
+    """out[n] = scale * weight[n] * table[idx[n]] for table [R, C] (unit stride along the rows) and
+    contiguous idx, valid (uint8 or bool) and weight (float32) of one shape -> [*idx.shape, *row_shape]
+    (row_shape: the C elements of a row, (C,) when not given)."""
+    dev = _dev_rows(table, idx, valid, weight)
     R, C = table.shape
-    N = idx.numel()
-    out = torch.empty(N, C, dtype=table.dtype, device=table.device)
-    call("tts_gather_rows", ptr(table), R, C, table.stride(0), row_type(table, "table"), ptr(idx),
-         index_type(idx, "idx"), ptr(valid), ptr(weight), scale, N, ptr(out), stream())
+    out = torch.empty(idx.shape + ((C,) if row_shape is None else row_shape), dtype=table.dtype, device=table.device)
+    call("tts_gather_rows", _addr(table), R, C, table.stride(0), row_type(table, "table"), _addr(idx),
+         index_type(idx, "idx"), _addr(valid), _addr(weight), scale, idx.numel(), _addr(out), _stream(dev))
     return out
 
 
-def gather_rows_bwd(table, R, idx, valid, weight, scale, gout, want_table=True, want_weight=False):
-    """Gradients of gather_rows from gout [N, C]: gtable [R, C] in gout's type and gweight [N] (each
-    None when not wanted); ``table`` is read for the weight gradient only and may be None without it."""
-    _dev_rows(table, gout)
-    _dev(idx, valid, weight)
+def gather_rows_bwd(table, R, idx, valid, weight, scale, gout, want_table=True, want_weight=False, row_shape=None):
+    """Gradients of gather_rows from gout [N, C] (unit stride along the rows): gtable [R, *row_shape] in
+    gout's type and gweight of idx's shape (each None when not wanted); ``table`` is read for the weight
+    gradient only and may be None without it."""
+    dev = _dev_rows(gout, idx, valid, weight)
+    if table is not None:
+        _dev_rows(table)
     N, C = gout.shape
-    dev = gout.device
-    gtable = torch.empty(R, C, dtype=gout.dtype, device=dev) if want_table else None
-    gweight = torch.empty(N, device=dev) if want_weight else None
-    nbytes = lib().tts_gather_rows_bwd_workspace_bytes(N, R, C) if want_table else 0
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if want_table else None
-    call("tts_gather_rows_bwd", ptr(table), R, C, 0 if table is None else table.stride(0), row_type(gout, "gout"),
-         ptr(idx), index_type(idx, "idx"), ptr(valid), ptr(weight), scale, N, ptr(gout), gout.stride(0), ptr(gtable),
-         ptr(gweight), ptr(ws), nbytes, stream())
+    gtable = gweight = ws = None
+    nbytes = 0
+    if want_table:
+        gtable = torch.empty((R, C) if row_shape is None else (R,) + row_shape, dtype=gout.dtype, device=gout.device)
+        nbytes = lib().tts_gather_rows_bwd_workspace_bytes(N, R, C)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=gout.device)
+    if want_weight:
+        gweight = torch.empty(idx.shape, dtype=torch.float32, device=gout.device)
+    call("tts_gather_rows_bwd", _addr(table), R, C, 0 if table is None else table.stride(0), row_type(gout, "gout"),
+         _addr(idx), index_type(idx, "idx"), _addr(valid), _addr(weight), scale, N, _addr(gout), gout.stride(0),
+         _addr(gtable), _addr(gweight), _addr(ws), nbytes, _stream(dev))
     return gtable, gweight
 
 
 def label_log_probs(logits, labels, top=0, want_stats=True):
-    """-> (logp [P], entropy [P], top_logp [P, top], top_ids [P, top] int64, stats [P, 2]) of logits [P, C]
-    (unit stride along the rows) and flat contiguous labels; stats, which only the backward needs, is
-    None when not wanted."""
-    _dev_rows(logits)
-    _dev(labels)
+    """-> (logp, entropy, top_logp [..., top], top_ids [..., top] int64, stats [P, 2]) of logits [P, C] (unit
+    stride along the rows) and contiguous labels [...] of P entries; stats, which only the backward needs,
+    is None when not wanted."""
+    dev = _dev_rows(logits, labels)
     P, C = logits.shape
-    dev = logits.device
-    logp, entropy = torch.empty(P, device=dev), torch.empty(P, device=dev)
-    top_logp = torch.empty(P, top, device=dev)
-    top_ids = torch.empty(P, top, dtype=torch.int64, device=dev)
-    stats = torch.empty(P, 2, device=dev) if want_stats else None
-    call("tts_label_log_probs", ptr(logits), P, C, logits.stride(0), row_type(logits, "logits"), ptr(labels),
-         index_type(labels, "labels"), top, ptr(logp), ptr(entropy), ptr(top_logp), ptr(top_ids), ptr(stats), stream())
+    on = dict(dtype=torch.float32, device=logits.device)
+    logp, entropy = torch.empty(labels.shape, **on), torch.empty(labels.shape, **on)
+    top_logp = torch.empty(labels.shape + (top,), **on)
+    top_ids = torch.empty(labels.shape + (top,), dtype=torch.int64, device=logits.device)
+    stats = torch.empty((P, 2), **on) if want_stats else None
+    call("tts_label_log_probs", _addr(logits), P, C, logits.stride(0), row_type(logits, "logits"), _addr(labels),
+         index_type(labels, "labels"), top, _addr(logp), _addr(entropy), _addr(top_logp), _addr(top_ids), _addr(stats),
+         _stream(dev))
     return logp, entropy, top_logp, top_ids, stats
 
 
 def label_log_probs_bwd(logits, labels, stats, entropy, top_ids, g_logp=None, g_entropy=None, g_top=None):
     """Gradient of label_log_probs in the logits, [P, C] contiguous; absent gradients count as zero."""
-    _dev_rows(logits)
-    _dev(labels, stats, entropy, top_ids, g_logp, g_entropy, g_top)
+    dev = _dev_rows(logits, labels, stats, entropy, top_ids, g_logp, g_entropy, g_top)
     P, C = logits.shape
-    gx = torch.empty(P, C, dtype=logits.dtype, device=logits.device)
-    call("tts_label_log_probs_bwd", ptr(logits), P, C, logits.stride(0), row_type(logits, "logits"), ptr(labels),
-         index_type(labels, "labels"), top_ids.shape[1], ptr(stats), ptr(entropy), ptr(top_ids), ptr(g_logp),
-         ptr(g_entropy), ptr(g_top), ptr(gx), stream())
+    gx = torch.empty((P, C), dtype=logits.dtype, device=logits.device)
+    call("tts_label_log_probs_bwd", _addr(logits), P, C, logits.stride(0), row_type(logits, "logits"), _addr(labels),
+         index_type(labels, "labels"), top_ids.shape[-1], _addr(stats), _addr(entropy), _addr(top_ids), _addr(g_logp),
+         _addr(g_entropy), _addr(g_top), _addr(gx), _stream(dev))
     return gx
 
 
