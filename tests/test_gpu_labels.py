@@ -251,16 +251,22 @@ def test_layouts(dt):
         s = metrics.label_log_probs(leaf, lab, top=2)
         flat, gx = _check(y.contiguous().reshape(60, 13), lab.reshape(60), top=2, grads=("logp",))
         assert s.logp.shape == (6, 10) and s.top_ids.shape == (6, 10, 2)
-        assert torch.equal(s.logp.reshape(-1), flat.logp) and torch.equal(s.top_ids.reshape(60, 2), flat.top_ids)
+        # another layout may add in another order: each result is within its bound of the exact one
+        R = _reference(y.reshape(60, 13), lab.reshape(60), 2)
+        tol = 2 * R["elp"].gather(1, lab.reshape(60).clamp(min=0)[:, None])[:, 0]
+        assert _close(s.logp.detach().reshape(-1), flat.logp.detach().double(), tol)
+        assert torch.equal(s.top_ids.reshape(60, 2), flat.top_ids)
         two = y[0].detach().requires_grad_(True)
         s2 = metrics.label_log_probs(two, lab[0])
         (g2,) = torch.autograd.grad(s2.logp.sum(), two)
-        assert torch.equal(s2.logp, flat.logp[:10]) and g2.shape == two.shape
+        assert _close(s2.logp.detach(), flat.logp[:10].detach().double(), tol[:10]) and g2.shape == two.shape
     one = img[0, 0, :13]
     s = metrics.label_log_probs(one, lab[0, 0])
     assert s.logp.shape == ()
     e = metrics.label_log_probs(one.expand(7, 13), torch.arange(7, device=DEV))
-    assert torch.equal(e.logp, metrics.label_log_probs(one[None].repeat(7, 1), torch.arange(7, device=DEV)).logp)
+    x7 = one[None].repeat(7, 1)
+    tol = 2 * _reference(x7, torch.arange(7, device=DEV), 0)["elp"][torch.arange(7), torch.arange(7)]
+    assert _close(e.logp, metrics.label_log_probs(x7, torch.arange(7, device=DEV)).logp.double(), tol)
     tr = img[0, :, :].t()[:13]
     s = metrics.label_log_probs(tr, torch.zeros(13, dtype=torch.int64, device=DEV), top=1)
     assert torch.equal(s.logp, metrics.label_log_probs(tr.contiguous(), torch.zeros(13, dtype=torch.int64, device=DEV)).logp)

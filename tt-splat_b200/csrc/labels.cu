@@ -18,6 +18,8 @@
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
+#include <type_traits>
+
 #include "rowtype.cuh"
 
 namespace tts {
@@ -386,6 +388,100 @@ __global__ void __launch_bounds__(SB_THREADS) k_scores_block(const T* __restrict
   cluster.sync();
 }
 
+// ---- one thread per row: few labels ----------------------------------------------------------------
+// A block's rows are one contiguous run of bytes: one bulk copy brings it into shared memory and, for the
+// gradient, one takes it back out, so the memory sees nothing but full lines whatever the row size.  A thread
+// then owns a row and nothing is shuffled.  Threads walk their rows in 4-byte words (two 16-bit logits) where
+// rows are whole words; with an even number of words to a row each thread starts one word further, so that
+// the warp's accesses fall into different banks.
+struct TileWalk {
+  int n, at;        // units of a row; the next one
+  __device__ __forceinline__ TileWalk(int n_) : n(n_), at((n_ & 1) ? 0 : (int)threadIdx.x % n_) {}
+  __device__ __forceinline__ int next() {
+    const int j = at;
+    at = at + 1 == n ? 0 : at + 1;
+    return j;
+  }
+};
+
+template <class T, int VB>
+struct TileUnit {
+  static constexpr int E = VB / (int)sizeof(T);
+  union {
+    typename std::conditional<VB == 4, unsigned, unsigned short>::type w;
+    T t[E];
+  };
+  __device__ __forceinline__ TileUnit() {}
+};
+
+// Copies rows [r0, r0 + n) into s (16-byte pieces by the bulk copy, the few bytes behind them by threads);
+// false when the copy did not arrive (recorded in the status word).
+template <class T>
+__device__ __forceinline__ bool load_tile(const T* logits, long long first, int count, T* s, uint64_t* bar) {
+  const unsigned bytes = (unsigned)count * (unsigned)sizeof(T), whole = bytes & ~15u;
+  if (threadIdx.x == 0) {
+    mbar_init(bar, 1);
+    if (whole > 0) {
+      mbar_expect_tx(bar, whole);
+      bulk_g2s(s, logits + first, whole, bar);
+    }
+  }
+  for (int i = (int)(whole / sizeof(T)) + threadIdx.x; i < count; i += blockDim.x) s[i] = logits[first + i];
+  __syncthreads();
+  return whole == 0 || mbar_wait_bounded(bar, 0);
+}
+
+template <class T, int VB>
+__global__ void __launch_bounds__(128) k_scores_tile(const T* __restrict__ logits, long long P, ScoreArgs a) {
+  using U = TileUnit<T, VB>;
+  extern __shared__ __align__(16) char smem[];
+  __shared__ __align__(8) uint64_t bar;
+  const int C = (int)a.C, units = C / U::E;
+  const long long r0 = (long long)blockIdx.x * blockDim.x;
+  const int rows = (int)(P - r0 < blockDim.x ? P - r0 : blockDim.x);
+  T* s = reinterpret_cast<T*>(smem);
+  if (!load_tile(logits, r0 * C, rows * C, s, &bar)) return;
+  if (threadIdx.x >= rows) return;
+  T* x = s + threadIdx.x * C;
+  U* xu = reinterpret_cast<U*>(x);
+  Soft f;
+  f.init();
+  TileWalk w(units);
+#pragma unroll 4
+  for (int i = 0; i < units; ++i) {
+    const U u = xu[w.next()];
+#pragma unroll
+    for (int e = 0; e < U::E; ++e) f.m = max_nan(f.m, to_f32(u.t[e]));
+  }
+#pragma unroll 4
+  for (int i = 0; i < units; ++i) {
+    const U u = xu[w.next()];
+#pragma unroll
+    for (int e = 0; e < U::E; ++e) f.add(to_f32(u.t[e]));
+  }
+  const long long r = r0 + threadIdx.x;
+  const float2 st = write_scores(a, r, f, x);
+  // the best label left, taken out of the tile after each round
+  for (int k = 0; k < a.top; ++k) {
+    float bv = -CUDART_INF_F;
+    int bi = -1;
+    if (!f.bad())
+#pragma unroll 4
+      for (int i = 0; i < units; ++i) {
+        const int j = w.next();
+        const U u = xu[j];
+#pragma unroll
+        for (int e = 0; e < U::E; ++e) {
+          const float v = to_f32(u.t[e]);
+          const int id = j * U::E + e;
+          if (v > bv || (v == bv && id < bi)) bv = v, bi = id;
+        }
+      }
+    if (bi >= 0) x[bi] = from_f32<T>(-CUDART_INF_F);
+    write_top(a, r, k, bv, bi, st);
+  }
+}
+
 // ---- one warp per row ----------------------------------------------------------------------------
 template <class T>
 __global__ void __launch_bounds__(256) k_scores_warp(const T* __restrict__ logits, long long P, long long stride,
@@ -561,6 +657,65 @@ __global__ void __launch_bounds__(256) k_scores_grad_warp(const T* __restrict__ 
   }
 }
 
+template <class T, int VB>
+__global__ void __launch_bounds__(128) k_scores_grad_tile(const T* __restrict__ logits, long long P, GradArgs a,
+                                                          T* __restrict__ glogits) {
+  using U = TileUnit<T, VB>;
+  extern __shared__ __align__(16) char smem[];
+  __shared__ __align__(8) uint64_t bar;
+  const int C = (int)a.C, units = C / U::E;
+  const long long r0 = (long long)blockIdx.x * blockDim.x;
+  const int rows = (int)(P - r0 < blockDim.x ? P - r0 : blockDim.x);
+  T* s = reinterpret_cast<T*>(smem);
+  if (!load_tile(logits, r0 * C, rows * C, s, &bar)) return;
+  if (threadIdx.x < rows) {
+    const long long r = r0 + threadIdx.x;
+    T* x = s + threadIdx.x * C;
+    U* xu = reinterpret_cast<U*>(x);
+    const RowGrad g(a, r);
+    const bool none = g.zero || g.empty;
+    // the labels with a term of their own, before their logits are overwritten
+    const int extra = 1 + (a.g_top ? a.top : 0);
+    float own[1 + TOP_MAX];
+    for (int k = 0; k < extra; ++k) {
+      const long long j = k == 0 ? g.t : a.top_ids[r * a.top + k - 1];
+      own[k] = j >= 0 && j < C ? g.special(a, r, j, to_f32(x[j])) : 0.f;
+    }
+    TileWalk w(units);
+#pragma unroll 4
+    for (int i = 0; i < units; ++i) {
+      const int j = w.next();
+      U u = xu[j];
+#pragma unroll
+      for (int e = 0; e < U::E; ++e) u.t[e] = from_f32<T>(none ? 0.f : g(to_f32(u.t[e])));
+      xu[j] = u;
+    }
+    for (int k = 0; k < extra; ++k) {
+      const long long j = k == 0 ? g.t : a.top_ids[r * a.top + k - 1];
+      if (j >= 0 && j < C) x[j] = from_f32<T>(own[k]);
+    }
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
+  const int count = rows * C;
+  const unsigned whole = ((unsigned)count * (unsigned)sizeof(T)) & ~15u;
+  if (threadIdx.x == 0 && whole > 0) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(glogits + r0 * C), "r"(smem_u32(s)),
+                 "r"(whole)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  }
+  for (int i = (int)(whole / sizeof(T)) + threadIdx.x; i < count; i += blockDim.x) glogits[r0 * C + i] = s[i];
+}
+
+// Rows of up to TILE_ROW_BYTES that lie one behind the other from a 16-byte boundary on take a thread each.
+constexpr long long TILE_ROW_BYTES = 512;
+static bool tile_rows(long long C, size_t elem, long long stride, const void* x, const void* gx) {
+  return C * (long long)elem <= TILE_ROW_BYTES && stride == C && aligned16(x) && aligned16(gx);
+}
+static int tile_threads(long long C, size_t elem) { return C * (long long)elem <= 128 ? 128 : 64; }
+
 constexpr long long WARP_ROW_MAX = 1024;      // labels up to which a warp takes a row
 
 static int check_labels(long long P, long long C, int type, int top) {
@@ -607,7 +762,15 @@ extern "C" int tts_label_log_probs(const void* logits, long long P, long long C,
   return with_row_type(type, [&](auto t) {
     using T = decltype(t);
     const T* x = static_cast<const T*>(logits);
-    if (C <= WARP_ROW_MAX) {
+    if (tile_rows(C, sizeof(T), row_stride, x, nullptr)) {
+      const int n = tile_threads(C, sizeof(T));
+      const size_t bytes = (size_t)n * C * sizeof(T);
+      const unsigned grid = (unsigned)((P + n - 1) / n);
+      if (C * sizeof(T) % 4 == 0)
+        k_scores_tile<T, 4><<<grid, n, bytes, as_stream(stream)>>>(x, P, a);
+      else
+        k_scores_tile<T, sizeof(T)><<<grid, n, bytes, as_stream(stream)>>>(x, P, a);
+    } else if (C <= WARP_ROW_MAX) {
       k_scores_warp<T><<<(unsigned)((P + 7) / 8), 256, 0, as_stream(stream)>>>(x, P, row_stride, a);
     } else if (int rc = launch_scores_block<T>(x, P, row_stride, a, as_stream(stream))) {
       return rc;
@@ -631,7 +794,15 @@ extern "C" int tts_label_log_probs_bwd(const void* logits, long long P, long lon
     using T = decltype(t);
     const T* x = static_cast<const T*>(logits);
     T* gx = static_cast<T*>(glogits);
-    if (C <= WARP_ROW_MAX) {
+    if (tile_rows(C, sizeof(T), row_stride, x, gx)) {
+      const int n = tile_threads(C, sizeof(T));
+      const size_t bytes = (size_t)n * C * sizeof(T);
+      const unsigned grid = (unsigned)((P + n - 1) / n);
+      if (C * sizeof(T) % 4 == 0)
+        k_scores_grad_tile<T, 4><<<grid, n, bytes, st>>>(x, P, a, gx);
+      else
+        k_scores_grad_tile<T, sizeof(T)><<<grid, n, bytes, st>>>(x, P, a, gx);
+    } else if (C <= WARP_ROW_MAX) {
       k_scores_grad_warp<T><<<(unsigned)((P + 7) / 8), 256, 0, st>>>(x, P, row_stride, a, gx);
     } else {
       // the logits' 16-byte vectors line up with the gradient's when both start on the same offset in every row
