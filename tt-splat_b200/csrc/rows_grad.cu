@@ -2,19 +2,20 @@
 //
 //   gtable_v = sum over the uses n of row v, ascending, of f_n gout_n,   gweight_n = scale <gout_n, table_v>
 //
-// A group of lanes takes L consecutive sorted uses, so rows with many uses and rows with few cost the same.
-// It keeps the running row in fp32 registers and writes it when the row changes.  A row that begins before
-// the group's uses or goes on behind them is left as a partial sum, and a second kernel adds a row's partial
-// sums in order.  Gradient rows are read once, in units of up to 16 bytes, several uses in flight.
+// A group of lanes takes a chunk of L consecutive sorted uses, so that rows with many uses and rows with few
+// cost the same.  It keeps the running row in fp32 registers and writes it when the row changes.  A row
+// belongs to the chunk in which it begins, which follows it into the next chunk; the next one skips that
+// part.  Only a row that goes on behind the next chunk too is split: every chunk leaves its part of it as a
+// partial sum, and a second kernel adds the parts in order.  Gradient rows are read once, in units of up to
+// 16 bytes, several uses in flight, the next uses' (row, use) pairs one step ahead.
 #include "rows.cuh"
 
 namespace tts {
 
 constexpr int GT = 256;
-constexpr int CHUNK_MIN = 32;
 
-// Uses per group; the partial sums take 2 rows of C floats for each.
-static long long chunk_len(long long N) { return N <= (1 << 19) ? CHUNK_MIN : (N <= (1 << 22) ? 2 * CHUNK_MIN : 4 * CHUNK_MIN); }
+// Uses of a chunk: few where there are few, so that they still spread over the SMs.
+static int chunk_len(long long N) { return N <= (1 << 14) ? 8 : (N <= (1 << 17) ? 16 : (N <= (1 << 20) ? 32 : 64)); }
 static long long chunks_of(long long N) { return (N + chunk_len(N) - 1) / chunk_len(N); }
 
 struct GradShape {
@@ -39,7 +40,35 @@ struct GradArgs {
   long long C, table_stride, gout_stride, chunks, group_blocks;
   int L, lanes, units;
   float* gweight;
-  float* partial;        // [2 * chunks][C]: the chunk's first row, begun before it; its last, which goes on
+  float* partial;        // [2 * chunks][C]: the chunk's part of a split row begun before it; of one begun in it
+};
+
+// What a chunk has to do with the rows at its ends.
+struct ChunkEnds {
+  long long i0, i1;
+  unsigned first, last;
+  bool skip;       // its first row belongs to the chunk before
+  bool open;       // its first row is split and began before it
+  bool split;      // its last row is split and goes on behind it
+  bool follow;     // its last row goes on in the next chunk and ends there
+  __device__ __forceinline__ ChunkEnds(const GradArgs& a, long long chunk) {
+    const long long N = a.u.N, L = a.L;
+    const unsigned R = (unsigned)a.u.R;
+    i0 = chunk * L;
+    i1 = i0 + L < N ? i0 + L : N;
+    first = __ldg(&a.s[i0].x);
+    last = __ldg(&a.s[i1 - 1].x);
+    const unsigned before = i0 > 0 ? __ldg(&a.s[i0 - 1].x) : R, far = i0 > L ? __ldg(&a.s[i0 - L - 1].x) : R;
+    const unsigned after = i1 < N ? __ldg(&a.s[i1].x) : R, farther = i1 + L < N ? __ldg(&a.s[i1 + L].x) : R;
+    const bool begun = first < R && before == first;             // the first row began before the chunk,
+    const bool through = begun && last == first && after == first;  // and goes on behind it
+    const bool longer = begun && far == first;                   // or began before the last one already
+    open = begun && (through || longer);
+    skip = begun && !open;
+    const bool on = last < R && after == last;
+    split = on && (through || farther == last);
+    follow = on && !split;
+  }
 };
 
 template <class T, int VB, int PL, bool GW>
@@ -68,9 +97,9 @@ __global__ void __launch_bounds__(GT) k_rows_grad(GradArgs a, const T* __restric
   const long long N = a.u.N;
   const unsigned R = (unsigned)a.u.R;
   const bool live = chunk < a.chunks;
-  const long long i0 = live ? chunk * a.L : N, i1 = i0 + a.L < N ? i0 + a.L : N;
-  unsigned cur = live ? a.s[i0].x : R;
-  bool open = live && i0 > 0 && a.s[i0 - 1].x == cur;      // the running row began in an earlier chunk
+  const ChunkEnds c(a, live ? chunk : 0);
+  unsigned cur = c.first;
+  bool open = c.open;
   float acc[PL * E], row[GW ? PL * E : 1];
   auto start = [&](unsigned v) {
     cur = v;
@@ -88,9 +117,9 @@ __global__ void __launch_bounds__(GT) k_rows_grad(GradArgs a, const T* __restric
       }
     }
   };
-  auto flush = [&](bool goes_on) {
-    if (cur >= R) return;
-    if (open || goes_on) {
+  auto flush = [&](bool split) {
+    if (cur >= R || (c.skip && cur == c.first)) return;
+    if (open || split) {
       float* p = a.partial + (2 * chunk + (open ? 0 : 1)) * a.C;
 #pragma unroll
       for (int k = 0; k < PL; ++k)
@@ -109,18 +138,29 @@ __global__ void __launch_bounds__(GT) k_rows_grad(GradArgs a, const T* __restric
         }
     }
   };
-  if (!GW && cur >= R) return;
+  // uses of the chunk, and behind it those of a last row that it follows
+  const uint2 none = make_uint2(0xffffffffu, 0xffffffffu);
+  auto use = [&](long long i) {
+    if (!live || i >= N || (i >= c.i1 && !c.follow)) return none;
+    const uint2 p = __ldg(a.s + i);
+    return i < c.i1 || p.x == c.last ? p : none;
+  };
+  uint2 next[UN];
+#pragma unroll
+  for (int j = 0; j < UN; ++j) next[j] = use(c.i0 + j);
   start(cur);
   // every group of a warp takes the same steps (the weights' sums shuffle)
-  for (long long s = 0; s < a.L; s += UN) {
+  for (long long i = c.i0;; i += UN) {
     uint2 p[UN];
     float f[UN];
     U g[UN][PL];
 #pragma unroll
-    for (int j = 0; j < UN; ++j) p[j] = i0 + s + j < i1 ? __ldg(a.s + i0 + s + j) : make_uint2(0xffffffffu, 0);
+    for (int j = 0; j < UN; ++j) p[j] = next[j];
+    if (!__any_sync(0xffffffffu, p[0].y != none.y)) break;
 #pragma unroll
     for (int j = 0; j < UN; ++j) {
-      const bool in = p[j].x < R;
+      // (a place past the end only after a wait of the sort that ran out)
+      const bool in = p[j].x < R && p[j].y < N && !(c.skip && p[j].x == c.first);
       f[j] = in ? factor_of(a.u, p[j].y) : 0.f;
       const W* src = reinterpret_cast<const W*>(gout + (long long)p[j].y * a.gout_stride);
 #pragma unroll
@@ -128,8 +168,10 @@ __global__ void __launch_bounds__(GT) k_rows_grad(GradArgs a, const T* __restric
         if (in && u0 + k * a.lanes < a.units) g[j][k].w = __ldg(src + u0 + k * a.lanes);
     }
 #pragma unroll
+    for (int j = 0; j < UN; ++j) next[j] = use(i + UN + j);
+#pragma unroll
     for (int j = 0; j < UN; ++j) {
-      const bool here = i0 + s + j < i1, in = p[j].x < R;
+      const bool here = p[j].y < N, in = here && p[j].x < R && !(c.skip && p[j].x == c.first);
       if (here && p[j].x != cur) {
         flush(false);
         open = false;
@@ -148,103 +190,95 @@ __global__ void __launch_bounds__(GT) k_rows_grad(GradArgs a, const T* __restric
             }
       if constexpr (GW) {
         for (int d = a.lanes / 2; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-        if (here && gl == 0) a.gweight[p[j].y] = in ? a.u.scale * dot : 0.f;
+        if (here && gl == 0 && (in || p[j].x >= R)) a.gweight[p[j].y] = in ? a.u.scale * dot : 0.f;
       }
     }
   }
-  if (live) flush(i1 < N && a.s[i1].x == cur);
+  if (live) flush(c.split);
 }
 
-// Rows over several chunks: the chunk in which a row begins owns it.  A lane tests a chunk; the warp adds the
-// partial sums of each row found, lanes over columns (narrow rows: lanes over columns and sums, joined in a
-// fixed order), or, for many sums, the warps of the block take a part each.
-constexpr int FIX_MANY = 64;
-constexpr int FIX_WARPS = GT / 32;
-constexpr int FIX_PARTS = 32;       // column parts of a block's grid row
+// Split rows: the chunk in which a row begins adds its parts, its own and then those of the chunks behind, a
+// lane for each column.  Rows over more than JOIN_MANY chunks are left to the whole block: its warps (and, for
+// narrow rows, lanes) take every so many-th part each, joined in a fixed order.
+constexpr int JOIN_MANY = 64;
+constexpr int JOIN_WARPS = GT / 32;
 
-struct FixItem {
+struct JoinItem {
   long long chunk, last;
   unsigned row;
 };
 
-// Column c of the sums partial(first), first + 1, ... behind the owner's own, by lanes `q` of `nq`.
-__device__ __forceinline__ float add_partials(const float* p, long long C, long long from, long long to, int step) {
+// Column p of the parts of chunks from, from + step, ... below to.
+__device__ __forceinline__ float add_parts(const float* p, long long C, long long from, long long to, int step) {
   float acc = 0.f;
   long long i = from;
-  for (; i + 3 * step < to; i += 4 * step) {
-    const float a = p[2 * i * C], b = p[2 * (i + step) * C], c = p[2 * (i + 2 * step) * C], d = p[2 * (i + 3 * step) * C];
-    acc += a;
-    acc += b;
-    acc += c;
-    acc += d;
+  for (; i + 7ll * step < to; i += 8ll * step) {
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = __ldg(p + 2 * (i + (long long)k * step) * C);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc += x[k];
   }
-  for (; i < to; i += step) acc += p[2 * i * C];
+  for (; i < to; i += step) acc += __ldg(p + 2 * i * C);
   return acc;
 }
 
 template <class T>
-__global__ void __launch_bounds__(GT) k_rows_join(GradArgs a, T* __restrict__ gtable) {
-  __shared__ FixItem s_many[GT];
+__global__ void __launch_bounds__(GT) k_rows_join(GradArgs a, int lanes, T* __restrict__ gtable) {
+  __shared__ JoinItem s_many[GT];
   __shared__ int s_n;
-  __shared__ float s_sum[FIX_WARPS][32];
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const long long N = a.u.N, C = a.C;
-  const int cols = C < 32 ? (C <= 1 ? 1 : C <= 2 ? 2 : C <= 4 ? 4 : C <= 8 ? 8 : C <= 16 ? 16 : 32) : 32;
-  const int nq = 32 / cols, q = lane / cols, cl = lane % cols;
+  __shared__ float s_sum[JOIN_WARPS][32];
+  const long long N = a.u.N, C = a.C, L = a.L;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, gl = threadIdx.x % lanes;
+  const long long chunk = ((long long)blockIdx.x * GT + threadIdx.x) / lanes;
+  const long long c0 = (long long)blockIdx.y * lanes, cstep = (long long)gridDim.y * lanes;
   if (threadIdx.x == 0) s_n = 0;
   __syncthreads();
-  const long long chunk = (long long)blockIdx.x * GT + threadIdx.x;
-  FixItem it{0, 0, 0};
-  bool found = false;
-  if (chunk < a.chunks && (chunk + 1) * a.L < N) {
-    const long long i0 = chunk * a.L, i1 = i0 + a.L;
-    const unsigned v = a.s[i1 - 1].x;
-    if (v < (unsigned)a.u.R && a.s[i1].x == v && !(i0 > 0 && a.s[i0].x == v && a.s[i0 - 1].x == v)) {
-      // the last use of row v
-      long long lo = i1, hi = N;
+  if (chunk < a.chunks) {
+    const ChunkEnds c(a, chunk);
+    if (c.split && !(c.open && c.last == c.first)) {
+      // the row's last use
+      long long lo = c.i1 + L, hi = N;
+      for (long long w = L; lo < N; w *= 2) {      // behind a few chunks for most rows
+        const long long at = lo + w < N ? lo + w : N;
+        if (at == N || a.s[at].x > c.last) {
+          hi = at;
+          break;
+        }
+        lo = at + 1;
+      }
       while (lo < hi) {
         const long long mid = (lo + hi) >> 1;
-        if (a.s[mid].x <= v)
+        if (a.s[mid].x <= c.last)
           lo = mid + 1;
         else
           hi = mid;
       }
-      it = FixItem{chunk, (lo - 1) / a.L, v};
-      found = true;
-      if (it.last - it.chunk > FIX_MANY) {
-        s_many[atomicAdd(&s_n, 1)] = it;
-        found = false;
+      const long long last = (lo - 1) / L;
+      if (last - chunk > JOIN_MANY) {
+        if (gl == 0) s_many[atomicAdd(&s_n, 1)] = JoinItem{chunk, last, c.last};
+      } else {
+        for (long long b = c0 + gl; b < C; b += cstep)
+          gtable[(long long)c.last * C + b] =
+              from_f32<T>(a.partial[(2 * chunk + 1) * C + b] + add_parts(a.partial + b, C, chunk + 1, last + 1, 1));
       }
     }
   }
-  unsigned todo = __ballot_sync(0xffffffffu, found);
-  while (todo) {
-    const int src = __ffs(todo) - 1;
-    todo &= todo - 1;
-    const long long c0 = __shfl_sync(0xffffffffu, it.chunk, src), c1 = __shfl_sync(0xffffffffu, it.last, src);
-    const unsigned v = __shfl_sync(0xffffffffu, it.row, src);
-    for (long long b = (long long)blockIdx.y * cols; b < C; b += (long long)gridDim.y * cols) {
-      const long long c = b + cl;
-      float sum = 0.f;
-      if (c < C) sum = add_partials(a.partial + c, C, c0 + 1 + q, c1 + 1, nq);
-      for (int d = 16; d >= cols; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      if (c < C && q == 0) gtable[(long long)v * C + c] = from_f32<T>(a.partial[(2 * c0 + 1) * C + c] + sum);
-    }
-  }
   __syncthreads();
-  for (int m = 0; m < s_n; ++m) {
-    const FixItem f = s_many[m];
-    for (long long b = (long long)blockIdx.y * cols; b < C; b += (long long)gridDim.y * cols) {
-      const long long c = b + cl;
+  const int nq = 32 / lanes, q = lane / lanes, n = s_n;
+  for (int m = 0; m < n; ++m) {
+    const JoinItem f = s_many[m];
+    for (long long b = c0; b < C; b += cstep) {
+      const long long col = b + gl;
       float sum = 0.f;
-      if (c < C) sum = add_partials(a.partial + c, C, f.chunk + 1 + wid * nq + q, f.last + 1, nq * FIX_WARPS);
-      for (int d = 16; d >= cols; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (col < C) sum = add_parts(a.partial + col, C, f.chunk + 1 + wid * nq + q, f.last + 1, nq * JOIN_WARPS);
+      for (int d = 16; d >= lanes; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
       s_sum[wid][lane] = sum;
       __syncthreads();
-      if (wid == 0 && q == 0 && c < C) {
-        sum = a.partial[(2 * f.chunk + 1) * C + c];
-        for (int w = 0; w < FIX_WARPS; ++w) sum += s_sum[w][lane];
-        gtable[(long long)f.row * C + c] = from_f32<T>(sum);
+      if (wid == 0 && q == 0 && col < C) {
+        sum = a.partial[(2 * f.chunk + 1) * C + col];
+        for (int w = 0; w < JOIN_WARPS; ++w) sum += s_sum[w][lane];
+        gtable[(long long)f.row * C + col] = from_f32<T>(sum);
       }
       __syncthreads();
     }
@@ -274,7 +308,13 @@ int rows_grad(const RowUses& u, const uint2* sorted, const uint8_t* used, const 
               cudaStream_t st) {
   const void* t = gweight ? table : nullptr;
   const int vb = grad_unit(type, t, table_stride, C, gout, gout_stride, gtable);
-  const GradShape g = grad_shape(C, elem_bytes(type), vb);
+  GradShape g = grad_shape(C, elem_bytes(type), vb);
+  // few chunks of wide rows: one unit a lane, more column parts
+  if (!gweight && g.per_lane > 1 && chunks_of(u.N) * g.lanes < 148 * 512) {
+    g.per_lane = 1;
+    g.parts = (int)((g.units + g.lanes - 1) / g.lanes);
+    if (g.parts > 65535) g = grad_shape(C, elem_bytes(type), vb);
+  }
   GradArgs a;
   a.u = u;
   a.s = sorted;
@@ -283,7 +323,7 @@ int rows_grad(const RowUses& u, const uint2* sorted, const uint8_t* used, const 
   a.table_stride = table_stride;
   a.gout_stride = gout_stride;
   a.chunks = chunks_of(u.N);
-  a.L = (int)chunk_len(u.N);
+  a.L = chunk_len(u.N);
   a.lanes = g.lanes;
   a.units = (int)g.units;
   a.gweight = gweight;
@@ -313,10 +353,12 @@ int rows_grad(const RowUses& u, const uint2* sorted, const uint8_t* used, const 
       else
         k_rows_grad<T, VB, 4, false><<<grid, GT, 0, st>>>(a, tb, go, gt);
     }
-    if (a.chunks > 1) {
-      const long long cols = (C + 31) / 32;
-      const dim3 jg((unsigned)((a.chunks + GT - 1) / GT), (unsigned)(cols < FIX_PARTS ? cols : FIX_PARTS));
-      k_rows_join<T><<<jg, GT, 0, st>>>(a, gt);
+    if (a.chunks > 2) {      // a split row covers a chunk whole
+      int lanes = 1;
+      while (lanes < 32 && lanes < C) lanes *= 2;
+      const long long cols = (C + lanes - 1) / lanes;
+      const dim3 jg((unsigned)((a.chunks * lanes + GT - 1) / GT), (unsigned)(cols < 32 ? cols : 32));
+      k_rows_join<T><<<jg, GT, 0, st>>>(a, lanes, gt);
     }
     return check_launch("row gradient");
   });

@@ -13,7 +13,7 @@
 
 namespace tts {
 
-constexpr int ST = 256;                       // threads of a tile
+constexpr int ST = 512;                       // threads of a tile
 constexpr int SW = ST / 32;
 constexpr int SI = 16;                        // entries per thread
 constexpr int TILE = ST * SI;
@@ -21,6 +21,8 @@ constexpr int MAX_BITS = 10;
 constexpr int MAX_DIGITS = 1 << MAX_BITS;
 constexpr int MAX_PASSES = 4;
 constexpr int BACK = 8;                       // earlier tiles that a wait looks at in one go
+constexpr int PER = MAX_DIGITS / ST;          // neighbouring digits of a thread, their states one word pair
+static_assert(PER == 2, "a thread's digits are one 8-byte word of states and one 4-byte word of counts");
 constexpr int STATUS_SORT_TIMEOUT = 16;
 // tile states: what is published, in the top two bits of a word whose rest is the count (N < 2^30)
 constexpr unsigned HAVE_COUNT = 1u << 30, HAVE_SUM = 2u << 30, VALUE = (1u << 30) - 1;
@@ -54,43 +56,55 @@ __device__ __forceinline__ unsigned same_digit(unsigned d, int bits, bool in) {
   return m;
 }
 
-// Digit counts of every pass, and the flags of the rows that are looked up.
-__global__ void __launch_bounds__(256) k_sort_digits(RowUses u, Digits dg, unsigned* __restrict__ counts,
-                                                     uint8_t* __restrict__ used) {
+// Digit counts of every pass, and the flags of the rows that are looked up.  One block per SM, so that few
+// blocks add their counts to the same words.
+constexpr int DT = 1024;
+__global__ void __launch_bounds__(DT) k_sort_digits(RowUses u, Digits dg, unsigned* __restrict__ counts,
+                                                    uint8_t* __restrict__ used) {
   __shared__ unsigned h[MAX_PASSES * MAX_DIGITS];
+  constexpr int UN = 4;
   const int D = 1 << dg.bits, all = dg.passes * D;
-  for (int i = threadIdx.x; i < all; i += 256) h[i] = 0;
+  for (int i = threadIdx.x; i < all; i += DT) h[i] = 0;
   __syncthreads();
-  for (long long n = (long long)blockIdx.x * 256 + threadIdx.x; n < u.N; n += (long long)gridDim.x * 256) {
-    const unsigned k = key_of(u, n);
-    if (k < (unsigned)u.R) used[k] = 1;
-    for (int p = 0; p < dg.passes; ++p) atomicAdd(&h[p * D + ((k >> dg.shift(p)) & (D - 1))], 1u);
+  const long long step = (long long)gridDim.x * DT;
+  for (long long n0 = (long long)blockIdx.x * DT + threadIdx.x; n0 < u.N; n0 += UN * step) {
+    unsigned k[UN];
+#pragma unroll
+    for (int i = 0; i < UN; ++i) k[i] = n0 + i * step < u.N ? key_of(u, n0 + i * step) : 0u;
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      if (n0 + i * step >= u.N) break;
+      if (k[i] < (unsigned)u.R) used[k[i]] = 1;
+      for (int p = 0; p < dg.passes; ++p) atomicAdd(&h[p * D + ((k[i] >> dg.shift(p)) & (D - 1))], 1u);
+    }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < all; i += 256)
+  for (int i = threadIdx.x; i < all; i += DT)
     if (h[i]) atomicAdd(counts + i, h[i]);
 }
 
-__device__ __forceinline__ unsigned load_state(const unsigned* p) {
-  unsigned v;
-  asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+__device__ __forceinline__ uint2 load_state(const unsigned* p) {
+  uint2 v;
+  asm volatile("ld.relaxed.gpu.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
   return v;
 }
-__device__ __forceinline__ void store_state(unsigned* p, unsigned v) {
-  asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+__device__ __forceinline__ void store_state(unsigned* p, uint2 v) {
+  asm volatile("st.relaxed.gpu.global.v2.u32 [%0], {%1, %2};" ::"l"(p), "r"(v.x), "r"(v.y) : "memory");
 }
+// The published words of both digits, which arrive each by itself: ready when both are there.
+__device__ __forceinline__ bool ready(uint2 s) { return (s.x >> 30) != 0 && (s.y >> 30) != 0; }
 
 __global__ void __launch_bounds__(ST) k_sort_pass(RowUses u, const uint2* __restrict__ src, Digits dg, int pass,
                                                   const unsigned* __restrict__ counts, unsigned* __restrict__ ticket,
                                                   unsigned* __restrict__ states, uint2* __restrict__ dst) {
-  __shared__ unsigned short s_warp[SW][MAX_DIGITS];     // counts of each warp, then of the warps before it
+  __shared__ __align__(16) unsigned short s_warp[SW][MAX_DIGITS];     // counts of each warp, then of the warps before it
   __shared__ unsigned s_base[MAX_DIGITS];               // where the tile's first entry of a digit goes
   __shared__ unsigned s_scan[SW];
   __shared__ unsigned s_tile;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int D = 1 << dg.bits, shift = dg.shift(pass);
   if (tid == 0) s_tile = atomicAdd(ticket, 1u);
-  for (int i = tid; i < SW * D; i += ST) s_warp[i / D][i % D] = 0;
+  for (int i = tid; i < SW * MAX_DIGITS / 8; i += ST) reinterpret_cast<uint4*>(s_warp)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
   const unsigned tile = s_tile;
   const long long base = (long long)tile * TILE + wid * (32 * SI);
@@ -114,32 +128,27 @@ __global__ void __launch_bounds__(ST) k_sort_pass(RowUses u, const uint2* __rest
     __syncwarp();
   }
   __syncthreads();
-  // the tile's counts, published before anything is waited for
-  constexpr int PER = MAX_DIGITS / ST;
-  unsigned count[PER];
+  // the tile's counts (two digits to a word), published before anything is waited for
+  const int d0 = tid * PER;
+  uint2 count = make_uint2(0, 0);
+  if (d0 < D) {
+    unsigned run = 0;
 #pragma unroll
-  for (int q = 0; q < PER; ++q) {
-    const int d = q * ST + tid;
-    count[q] = 0;
-    if (d < D) {
-      for (int w = 0; w < SW; ++w) {
-        const unsigned c = s_warp[w][d];
-        s_warp[w][d] = (unsigned short)count[q];
-        count[q] += c;
-      }
-      if (tile > 0) store_state(states + (long long)tile * D + d, HAVE_COUNT | count[q]);
+    for (int w = 0; w < SW; ++w) {
+      unsigned* p = reinterpret_cast<unsigned*>(&s_warp[w][d0]);
+      const unsigned c = *p;
+      *p = run;
+      run += c;
     }
+    count = make_uint2(run & 0xffffu, run >> 16);
+    if (tile > 0) store_state(states + (long long)tile * D + d0, make_uint2(HAVE_COUNT | count.x, HAVE_COUNT | count.y));
   }
+  uint2 before = make_uint2(0, 0);
   if (tile == 0) {
     // the first tile starts each digit behind the smaller ones
-    unsigned c[PER], sum = 0;
-#pragma unroll
-    for (int q = 0; q < PER; ++q) {
-      const int d = tid * PER + q;
-      c[q] = d < D ? counts[d] : 0;
-      sum += c[q];
-    }
-    unsigned incl = sum;
+    uint2 c = make_uint2(0, 0);
+    if (d0 < D) c = make_uint2(counts[d0], counts[d0 + 1]);
+    unsigned incl = c.x + c.y;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned y = __shfl_up_sync(0xffffffffu, incl, o);
@@ -147,47 +156,50 @@ __global__ void __launch_bounds__(ST) k_sort_pass(RowUses u, const uint2* __rest
     }
     if (lane == 31) s_scan[wid] = incl;
     __syncthreads();
-    unsigned run = incl - sum;
-    for (int w = 0; w < wid; ++w) run += s_scan[w];
+    before.x = incl - c.x - c.y;
+    for (int w = 0; w < wid; ++w) before.x += s_scan[w];
+    before.y = before.x + c.x;
+  } else if (d0 < D) {
+    long long t = (long long)tile - 1;
+    int tries = 0;
+    bool done = false;
+    while (!done && tries < (1 << 20)) {
+      // a few tiles at once, the nearest first; stop at one that has not published yet
+      uint2 s[BACK];
 #pragma unroll
-    for (int q = 0; q < PER; ++q) {
-      if (tid * PER + q < D) s_base[tid * PER + q] = run;
-      run += c[q];
-    }
-    __syncthreads();
+      for (int j = 0; j < BACK; ++j) s[j] = t - j >= 0 ? load_state(states + (t - j) * D + d0) : make_uint2(0, 0);
+      bool go = true;
+      int seen = 0;
 #pragma unroll
-    for (int q = 0; q < PER; ++q)
-      if (q * ST + tid < D) store_state(states + q * ST + tid, HAVE_SUM | (s_base[q * ST + tid] + count[q]));
-  } else {
-    for (int q = 0; q < PER && q * ST + tid < D; ++q) {
-      const int d = q * ST + tid;
-      unsigned before = 0;
-      long long t = (long long)tile - 1;
-      int tries = 0;
-      bool done = false;
-      while (!done && tries < (1 << 20)) {
-        // a few tiles at once, the nearest first; stop at one that has published nothing yet
-        unsigned st[BACK];
-#pragma unroll
-        for (int j = 0; j < BACK; ++j) st[j] = t - j >= 0 ? load_state(states + (t - j) * D + d) : 0u;
-        bool ready = true;
-        int seen = 0;
-#pragma unroll
-        for (int j = 0; j < BACK; ++j) {
-          ready = ready && !done && (st[j] & (HAVE_COUNT | HAVE_SUM)) != 0;
-          if (ready) {
-            before += st[j] & VALUE;
+      for (int j = 0; j < BACK; ++j) {
+        go = go && !done && ready(s[j]);
+        if (go) {
+          // a sum counts where both words hold one; a tile that is just turning its counts into sums is read
+          // again in the next round
+          const bool sx = (s[j].x & HAVE_SUM) != 0, sy = (s[j].y & HAVE_SUM) != 0;
+          if (sx != sy) {
+            go = false;
+          } else {
+            before.x += s[j].x & VALUE;
+            before.y += s[j].y & VALUE;
             ++seen;
-            done = (st[j] & HAVE_SUM) != 0;
+            done = sx;
           }
         }
-        t -= seen;
-        if (seen == 0) ++tries;
       }
-      if (!done) atomicOr(&g_status, STATUS_SORT_TIMEOUT);
-      s_base[d] = done ? before : 0xffffffffu;
-      store_state(states + (long long)tile * D + d, HAVE_SUM | ((before + count[q]) & VALUE));
+      t -= seen;
+      if (seen == 0) ++tries;
     }
+    if (!done) {
+      atomicOr(&g_status, STATUS_SORT_TIMEOUT);
+      before = make_uint2(VALUE, VALUE);
+    }
+  }
+  if (d0 < D) {
+    store_state(states + (long long)tile * D + d0,
+                make_uint2(HAVE_SUM | ((before.x + count.x) & VALUE), HAVE_SUM | ((before.y + count.y) & VALUE)));
+    s_base[d0] = before.x;
+    s_base[d0 + 1] = before.y;
   }
   __syncthreads();
 #pragma unroll
@@ -346,9 +358,9 @@ int sort_uses(const RowUses& u, const SortSpace& s, void* clear, size_t clear_by
   unsigned* tickets = reinterpret_cast<unsigned*>(s.zeroed);
   unsigned* counts = tickets + MAX_PASSES;
   unsigned* states = reinterpret_cast<unsigned*>(s.zeroed + align256((size_t)(MAX_PASSES + (size_t)dg.passes * D) * sizeof(unsigned)));
-  long long blocks = (u.N + 4095) / 4096;
-  if (blocks > 148 * 4) blocks = 148 * 4;
-  k_sort_digits<<<(unsigned)blocks, 256, 0, st>>>(u, dg, counts, s.used);
+  long long blocks = (u.N + DT - 1) / DT;
+  if (blocks > 148) blocks = 148;
+  k_sort_digits<<<(unsigned)blocks, DT, 0, st>>>(u, dg, counts, s.used);
   for (int p = 0; p < dg.passes; ++p) {
     // the last pass writes `sorted`, the ones before alternate so that none reads what it writes
     const bool to_sorted = (dg.passes - 1 - p) % 2 == 0;
