@@ -365,7 +365,8 @@ int tts_unit_from_u8(const uint8_t* src, long long n, float* dst, void* stream);
  * The gather of per-gaussian rows by an (idx, valid) table, `conic[idx]` and `color_o[idx] * valid`
  * of tools/m4_train_binned.py:203-211, for rows of any width, and its transpose.
  * table [R] rows of C elements of `type`, table_stride elements apart; idx [N] int32 or (idx64)
- * int64; valid [N] uint8 or NULL; weight [N] fp32 or NULL; N < 2^30, R < 2^31 - 1, C <= 2^22.
+ * int64; valid [N] uint8 or NULL; weight [N] fp32 or NULL; N < 2^30, R < 2^31 - 1, C <= 2^22,
+ * strides below 2^30.
  * out[N][C] = scale * weight[n] * table[idx[n]], rounded once; a slot with valid 0 or a negative
  * idx gives zeros, an idx >= R is not read and gives NaN. */
 #define TTS_ROW_F32 0

@@ -97,11 +97,12 @@ __global__ void __launch_bounds__(256) k_weight_grad(RowUses u, const T* __restr
   if (lane == 0) gweight[n] = u.scale * acc;
 }
 
-static int check_rows(long long R, long long C, int type, long long N) {
+static int check_rows(long long R, long long C, int type, long long N, long long stride) {
   TTS_REQUIRE(type >= TTS_ROW_F32 && type <= TTS_ROW_F16, "unknown row type");
   TTS_REQUIRE(N >= 0 && N < (1ll << 30), "the number of lookups must be below 2^30");
   TTS_REQUIRE(R >= 0 && R < (1ll << 31) - 1, "the number of table rows must be below 2^31 - 1");
   TTS_REQUIRE(C >= 0 && C <= (1ll << 22), "the row width must be at most 2^22");
+  TTS_REQUIRE(stride >= 0 && stride < (1ll << 30), "the distance between rows must be below 2^30");
   return TTS_OK;
 }
 static size_t elem(int type) { return type == TTS_ROW_F32 ? 4 : 2; }
@@ -113,7 +114,7 @@ using namespace tts;
 extern "C" int tts_gather_rows(const void* table, long long R, long long C, long long table_stride, int type,
                                const void* idx, int idx64, const uint8_t* valid, const float* weight, float scale,
                                long long N, void* out, void* stream) {
-  if (int rc = check_rows(R, C, type, N)) return rc;
+  if (int rc = check_rows(R, C, type, N, table_stride)) return rc;
   if (N == 0 || C == 0) return TTS_OK;
   TTS_REQUIRE((table || R == 0) && idx && out, "null gather_rows argument");
   const RowUses u{idx, valid, weight, scale, idx64, N, R};
@@ -140,7 +141,8 @@ extern "C" int tts_gather_rows_bwd(const void* table, long long R, long long C, 
                                    const void* idx, int idx64, const uint8_t* valid, const float* weight, float scale,
                                    long long N, const void* gout, long long gout_stride, void* gtable, float* gweight,
                                    void* workspace, size_t workspace_bytes, void* stream) {
-  if (int rc = check_rows(R, C, type, N)) return rc;
+  if (int rc = check_rows(R, C, type, N, table_stride)) return rc;
+  if (int rc = check_rows(R, C, type, N, gout_stride)) return rc;
   TTS_REQUIRE(N == 0 || (idx && (gout || C == 0)), "null gather_rows_bwd argument");
   TTS_REQUIRE(!gweight || table || R == 0 || C == 0, "the weight gradient needs the table");
   if (R == 0 || C == 0) gtable = nullptr;      // nothing to write

@@ -82,17 +82,17 @@ struct SortSpace {
   uint2* other;        // [N] the pass before the last (large sorts)
   char* zeroed;        // cleared before a large sort: digit counts, tickets, tile states, row flags
   size_t zeroed_bytes;
-  uint8_t* used;       // [R] rows that are looked up (large sorts)
+  uint8_t* used;       // [R] flags for the rows that are looked up, cleared (large sorts)
 };
 
 size_t sort_space(long long N, long long R, void* base, SortSpace* s);
 // Launches the sort.  Up to SORT_SMALL uses it clears the `clear_bytes` at `clear` as well (the whole
-// gradient); beyond, it leaves `used` flags instead and the caller writes the rows that have none.
+// gradient); beyond, it clears the `used` flags instead, for the caller to find the rows without a use.
 int sort_uses(const RowUses& u, const SortSpace& s, void* clear, size_t clear_bytes, cudaStream_t st);
 
 // ---- the sums over the sorted uses ---------------------------------------------------------------
 size_t grad_space(long long N, long long C);
-int rows_grad(const RowUses& u, const uint2* sorted, const uint8_t* used, const void* table, long long table_stride, int type,
+int rows_grad(const RowUses& u, const uint2* sorted, uint8_t* used, const void* table, long long table_stride, int type,
               long long C, const void* gout, long long gout_stride, void* gtable, float* gweight, float* partial,
               cudaStream_t st);
 // Whether rows_grad can write the weights' gradient on its way (a row fits a warp's registers).

@@ -6,17 +6,26 @@
 // cost the same.  It keeps the running row in fp32 registers and writes it when the row changes.  A row
 // belongs to the chunk in which it begins, which follows it into the next chunk; the next one skips that
 // part.  Only a row that goes on behind the next chunk too is split: every chunk leaves its part of it as a
-// partial sum, and a second kernel adds the parts in order.  Gradient rows are read once, in units of up to
-// 16 bytes, several uses in flight, the next uses' (row, use) pairs one step ahead.
+// partial sum, and a second kernel adds the parts in order.  A block brings its chunks' (row, use) pairs and
+// factors into shared memory first, so that nothing but gradient rows is waited for afterwards; they are read
+// once, in units of up to 16 bytes, several uses in flight.
 #include "rows.cuh"
 
 namespace tts {
 
 constexpr int GT = 256;
 
-// Uses of a chunk: few where there are few, so that they still spread over the SMs.
-static int chunk_len(long long N) { return N <= (1 << 14) ? 8 : (N <= (1 << 17) ? 16 : (N <= (1 << 20) ? 32 : 64)); }
-static long long chunks_of(long long N) { return (N + chunk_len(N) - 1) / chunk_len(N); }
+// Uses of a chunk: few where there are few, so that they still spread over the SMs, and at most 8 for each lane
+// of the smallest group that rows of this width can have, which bounds a block's uses by BLOCK_USES.
+constexpr int L_MAX = 64;
+constexpr int BLOCK_USES = 8 * GT;
+static int chunk_len(long long N, long long C) {
+  int lanes = 1;
+  while (lanes < 32 && lanes * 8 < C) lanes *= 2;
+  const int l = N <= (1 << 14) ? 8 : (N <= (1 << 17) ? 16 : (N <= (1 << 20) ? 32 : L_MAX));
+  return l < 8 * lanes ? l : 8 * lanes;
+}
+static long long chunks_of(long long N, long long C) { return (N + chunk_len(N, C) - 1) / chunk_len(N, C); }
 
 struct GradShape {
   long long units;        // of a row
@@ -36,14 +45,14 @@ static GradShape grad_shape(long long C, int elem, int vb) {
 struct GradArgs {
   RowUses u;
   const uint2* s;
-  const uint8_t* used;
-  long long C, table_stride, gout_stride, chunks, group_blocks;
-  int L, lanes, units;
+  uint8_t* used;
+  long long C, table_stride, gout_stride, chunks;
+  int L, lanes, units, unit;
   float* gweight;
   float* partial;        // [2 * chunks][C]: the chunk's part of a split row begun before it; of one begun in it
 };
 
-// What a chunk has to do with the rows at its ends.
+// What a chunk has to do with the rows at its ends; key(i) is the row of sorted use i, R outside 0 .. N - 1.
 struct ChunkEnds {
   long long i0, i1;
   unsigned first, last;
@@ -51,156 +60,197 @@ struct ChunkEnds {
   bool open;       // its first row is split and began before it
   bool split;      // its last row is split and goes on behind it
   bool follow;     // its last row goes on in the next chunk and ends there
-  __device__ __forceinline__ ChunkEnds(const GradArgs& a, long long chunk) {
-    const long long N = a.u.N, L = a.L;
-    const unsigned R = (unsigned)a.u.R;
+  template <class K>
+  __device__ __forceinline__ ChunkEnds(long long chunk, long long N, long long L, unsigned R, K key) {
     i0 = chunk * L;
     i1 = i0 + L < N ? i0 + L : N;
-    first = __ldg(&a.s[i0].x);
-    last = __ldg(&a.s[i1 - 1].x);
-    const unsigned before = i0 > 0 ? __ldg(&a.s[i0 - 1].x) : R, far = i0 > L ? __ldg(&a.s[i0 - L - 1].x) : R;
-    const unsigned after = i1 < N ? __ldg(&a.s[i1].x) : R, farther = i1 + L < N ? __ldg(&a.s[i1 + L].x) : R;
-    const bool begun = first < R && before == first;             // the first row began before the chunk,
+    first = key(i0);
+    last = key(i1 - 1);
+    const unsigned after = key(i1);
+    const bool begun = first < R && key(i0 - 1) == first;           // the first row began before the chunk,
     const bool through = begun && last == first && after == first;  // and goes on behind it
-    const bool longer = begun && far == first;                   // or began before the last one already
+    const bool longer = begun && key(i0 - L - 1) == first;          // or began before the last one already
     open = begun && (through || longer);
     skip = begun && !open;
     const bool on = last < R && after == last;
-    split = on && (through || farther == last);
+    split = on && (through || key(i1 + L) == last);
     follow = on && !split;
   }
 };
+
+// Sums v[0 .. 7] over the group's lanes (8 or more, named by mask): each step adds and halves what a lane holds,
+// 7 shuffles and the plain steps behind them instead of 8 for each value.  Returns the sum of value j in the
+// lanes whose top three bits (of their number in the group) spell j.
+__device__ __forceinline__ float sum8(float (&v)[8], int gl, int lanes, unsigned mask) {
+  int d = lanes / 2;
+#pragma unroll
+  for (int n = 4; n > 0; n >>= 1, d >>= 1) {
+    const bool up = gl & d;
+#pragma unroll
+    for (int j = 0; j < n; ++j) {
+      const float send = up ? v[j] : v[j + n];
+      const float keep = up ? v[j + n] : v[j];
+      v[j] = keep + __shfl_xor_sync(mask, send, d);
+    }
+  }
+  for (; d > 0; d >>= 1) v[0] += __shfl_xor_sync(mask, v[0], d);
+  return v[0];
+}
 
 template <class T, int VB, int PL, bool GW>
 __global__ void __launch_bounds__(GT) k_rows_grad(GradArgs a, const T* __restrict__ table, const T* __restrict__ gout,
                                                   T* __restrict__ gtable) {
   using U = Unit<T, VB>;
   using W = typename U::W;
-  constexpr int E = U::E, UN = PL == 1 ? 8 : 4;
-  const int gl = threadIdx.x % a.lanes;
-  const int u0 = blockIdx.y * a.lanes * PL + gl;
-  if (blockIdx.x >= a.group_blocks) {
-    // rows that nothing looks up
-    const long long row = ((long long)(blockIdx.x - a.group_blocks) * GT + threadIdx.x) / a.lanes;
-    if (row < a.u.R && !__ldg(a.used + row)) {
-      W* g = reinterpret_cast<W*>(gtable + row * a.C);
-      U z;
-#pragma unroll
-      for (int e = 0; e < E; ++e) z.t[e] = from_f32<T>(0.f);
-#pragma unroll
-      for (int k = 0; k < PL; ++k)
-        if (u0 + k * a.lanes < a.units) g[u0 + k * a.lanes] = z.w;
-    }
-    return;
-  }
-  const long long chunk = ((long long)blockIdx.x * GT + threadIdx.x) / a.lanes;
+  constexpr int E = U::E, UN = PL * VB > 32 ? 4 : 8;
+  constexpr int SPAN = BLOCK_USES + 2 * L_MAX + 2;
+  __shared__ unsigned s_key[SPAN], s_use[SPAN];
+  __shared__ float s_f[SPAN];
   const long long N = a.u.N;
   const unsigned R = (unsigned)a.u.R;
-  const bool live = chunk < a.chunks;
-  const ChunkEnds c(a, live ? chunk : 0);
-  unsigned cur = c.first;
-  bool open = c.open;
-  float acc[PL * E], row[GW ? PL * E : 1];
-  auto start = [&](unsigned v) {
-    cur = v;
-#pragma unroll
-    for (int k = 0; k < PL * E; ++k) acc[k] = 0.f;
-    if constexpr (GW) {
-      const W* t = reinterpret_cast<const W*>(table + (long long)v * a.table_stride);
-#pragma unroll
-      for (int k = 0; k < PL; ++k) {
-        U x;
-        const bool in = v < R && u0 + k * a.lanes < a.units;
-        if (in) x.w = __ldg(t + u0 + k * a.lanes);
-#pragma unroll
-        for (int e = 0; e < E; ++e) row[k * E + e] = in ? to_f32(x.t[e]) : 0.f;
-      }
+  // the block's uses, and as many beside them as a chunk looks at
+  const int groups = GT / a.lanes, first = a.L + 1, behind = first + groups * a.L;
+  const long long at = (long long)blockIdx.x * groups * a.L - first;
+  for (int k = threadIdx.x; k < behind + first; k += GT) {
+    const long long i = at + k;
+    uint2 p = make_uint2(R, 0xffffffffu);
+    if (i >= 0 && i < N) p = __ldg(a.s + i);
+    // (a row or use past the end only after a wait of the sort that ran out)
+    const bool in = p.x < R && p.y < N;
+    s_key[k] = in ? p.x : R;
+    s_use[k] = p.y;
+    s_f[k] = in ? factor_of(a.u, p.y) : 0.f;
+    if (GW && !in && p.y < N && k >= first && k < behind) a.gweight[p.y] = 0.f;
+  }
+  __syncthreads();
+  if (a.used && blockIdx.y == 0)
+    for (int k = first + threadIdx.x; k < behind; k += GT)
+      if (s_key[k] < R && s_key[k] != s_key[k - 1]) a.used[s_key[k]] = 1;
+  const int group = threadIdx.x / a.lanes, gl = threadIdx.x % a.lanes;
+  const long long chunk = (long long)blockIdx.x * groups + group;
+  if (chunk >= a.chunks) return;
+  const ChunkEnds c(chunk, N, a.L, R, [&](long long i) { return s_key[i - at]; });
+  // the chunk's uses, without those of a first row that it skips, with those of a last row that it follows,
+  // and without unused slots, which lie at the end
+  auto first_at_least = [&](int lo, int hi, unsigned v) {
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (s_key[mid] < v)
+        lo = mid + 1;
+      else
+        hi = mid;
     }
+    return lo;
   };
+  int j = (int)(c.i0 - at), end = (int)(c.i1 - at);
+  if (c.skip) j = first_at_least(j, end, c.first + 1);
+  if (c.follow)
+    end = first_at_least(end, end + a.L, c.last + 1);
+  else if (c.last >= R)
+    end = first_at_least(j, end, R);
+  const int u0 = blockIdx.y * a.lanes * PL + gl;
+  bool col[PL];
+#pragma unroll
+  for (int k = 0; k < PL; ++k) col[k] = u0 + k * a.lanes < a.units;
+  const unsigned mask = a.lanes == 32 ? 0xffffffffu : ((1u << a.lanes) - 1) << ((threadIdx.x & 31) / a.lanes * a.lanes);
+  const char* gbase = reinterpret_cast<const char*>(gout) + (long long)u0 * VB;
+  const char* tbase = reinterpret_cast<const char*>(table) + (long long)u0 * VB;
+  const unsigned gstep = (unsigned)(a.gout_stride * sizeof(T)), tstep = (unsigned)(a.table_stride * sizeof(T));
+  constexpr unsigned NOTHING = 0xffffffffu;
+  unsigned cur = NOTHING;
+  float acc[PL * E], row[GW ? PL * E : 1];
   auto flush = [&](bool split) {
-    if (cur >= R || (c.skip && cur == c.first)) return;
+    const bool open = c.open && cur == c.first;
     if (open || split) {
-      float* p = a.partial + (2 * chunk + (open ? 0 : 1)) * a.C;
+      float* p = a.partial + (2 * chunk + (open ? 0 : 1)) * a.C + (long long)u0 * E;
 #pragma unroll
       for (int k = 0; k < PL; ++k)
-        if (u0 + k * a.lanes < a.units)
+        if (col[k])
 #pragma unroll
-          for (int e = 0; e < E; ++e) p[(u0 + k * a.lanes) * E + e] = acc[k * E + e];
+          for (int e = 0; e < E; ++e) p[k * a.lanes * E + e] = acc[k * E + e];
     } else {
-      W* g = reinterpret_cast<W*>(gtable + (long long)cur * a.C);
+      W* g = reinterpret_cast<W*>(gtable + (long long)cur * a.C) + u0;
 #pragma unroll
       for (int k = 0; k < PL; ++k)
-        if (u0 + k * a.lanes < a.units) {
+        if (col[k]) {
           U x;
 #pragma unroll
           for (int e = 0; e < E; ++e) x.t[e] = from_f32<T>(acc[k * E + e]);
-          g[u0 + k * a.lanes] = x.w;
+          g[k * a.lanes] = x.w;
         }
     }
   };
-  // uses of the chunk, and behind it those of a last row that it follows
-  const uint2 none = make_uint2(0xffffffffu, 0xffffffffu);
-  auto use = [&](long long i) {
-    if (!live || i >= N || (i >= c.i1 && !c.follow)) return none;
-    const uint2 p = __ldg(a.s + i);
-    return i < c.i1 || p.x == c.last ? p : none;
-  };
-  uint2 next[UN];
+  for (; j < end; j += UN) {
+    U g[UN][PL], t[GW ? UN : 1][GW ? PL : 1];
+    unsigned key[UN];
 #pragma unroll
-  for (int j = 0; j < UN; ++j) next[j] = use(c.i0 + j);
-  start(cur);
-  // every group of a warp takes the same steps (the weights' sums shuffle)
-  for (long long i = c.i0;; i += UN) {
-    uint2 p[UN];
-    float f[UN];
-    U g[UN][PL];
-#pragma unroll
-    for (int j = 0; j < UN; ++j) p[j] = next[j];
-    if (!__any_sync(0xffffffffu, p[0].y != none.y)) break;
-#pragma unroll
-    for (int j = 0; j < UN; ++j) {
-      // (a place past the end only after a wait of the sort that ran out)
-      const bool in = p[j].x < R && p[j].y < N && !(c.skip && p[j].x == c.first);
-      f[j] = in ? factor_of(a.u, p[j].y) : 0.f;
-      const W* src = reinterpret_cast<const W*>(gout + (long long)p[j].y * a.gout_stride);
-#pragma unroll
-      for (int k = 0; k < PL; ++k)
-        if (in && u0 + k * a.lanes < a.units) g[j][k].w = __ldg(src + u0 + k * a.lanes);
-    }
-#pragma unroll
-    for (int j = 0; j < UN; ++j) next[j] = use(i + UN + j);
-#pragma unroll
-    for (int j = 0; j < UN; ++j) {
-      const bool here = p[j].y < N, in = here && p[j].x < R && !(c.skip && p[j].x == c.first);
-      if (here && p[j].x != cur) {
-        flush(false);
-        open = false;
-        start(p[j].x);
-      }
-      float dot = 0.f;
-      if (in)
+    for (int q = 0; q < UN; ++q)
+      if (j + q < end) {
+        key[q] = s_key[j + q];
+        const W* src = reinterpret_cast<const W*>(gbase + (unsigned long long)s_use[j + q] * gstep);
 #pragma unroll
         for (int k = 0; k < PL; ++k)
-          if (u0 + k * a.lanes < a.units)
+          if (col[k]) g[q][k].w = __ldg(src + k * a.lanes);
+        if constexpr (GW) {
+          if (key[q] != (q == 0 ? cur : key[q > 0 ? q - 1 : 0])) {
+            const W* tr = reinterpret_cast<const W*>(tbase + (unsigned long long)key[q] * tstep);
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-              const float x = to_f32(g[j][k].t[e]);
-              acc[k * E + e] = fmaf(f[j], x, acc[k * E + e]);
-              if constexpr (GW) dot = fmaf(x, row[k * E + e], dot);
-            }
-      if constexpr (GW) {
-        for (int d = a.lanes / 2; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-        if (here && gl == 0 && (in || p[j].x >= R)) a.gweight[p[j].y] = in ? a.u.scale * dot : 0.f;
+            for (int k = 0; k < PL; ++k)
+              if (col[k]) t[q][k].w = __ldg(tr + k * a.lanes);
+          }
+        }
+      }
+    float dot[UN];
+#pragma unroll
+    for (int q = 0; q < UN; ++q) {
+      dot[q] = 0.f;
+      if (j + q < end) {
+        if (key[q] != cur) {
+          if (cur != NOTHING) flush(false);
+          cur = key[q];
+#pragma unroll
+          for (int k = 0; k < PL * E; ++k) acc[k] = 0.f;
+          if constexpr (GW)
+#pragma unroll
+            for (int k = 0; k < PL; ++k)
+#pragma unroll
+              for (int e = 0; e < E; ++e) row[k * E + e] = to_f32(t[q][k].t[e]);
+        }
+        const float f = s_f[j + q];
+#pragma unroll
+        for (int k = 0; k < PL; ++k)
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const float x = to_f32(g[q][k].t[e]);
+            acc[k * E + e] = fmaf(f, x, acc[k * E + e]);
+            if constexpr (GW)
+              if (col[k]) dot[q] = fmaf(x, row[k * E + e], dot[q]);
+          }
+      }
+    }
+    if constexpr (GW) {
+      if (UN == 8 && a.lanes >= 8) {
+        if constexpr (UN == 8) {
+          const float sum = sum8(dot, gl, a.lanes, mask);
+          const int q = gl / (a.lanes / 8);
+          if (gl % (a.lanes / 8) == 0 && j + q < end) a.gweight[s_use[j + q]] = a.u.scale * sum;
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < UN; ++q) {
+          for (int d = a.lanes / 2; d > 0; d >>= 1) dot[q] += __shfl_xor_sync(mask, dot[q], d);
+          if (gl == 0 && j + q < end) a.gweight[s_use[j + q]] = a.u.scale * dot[q];
+        }
       }
     }
   }
-  if (live) flush(c.split);
+  if (cur != NOTHING) flush(c.split);
 }
 
 // Split rows: the chunk in which a row begins adds its parts, its own and then those of the chunks behind, a
 // lane for each column.  Rows over more than JOIN_MANY chunks are left to the whole block: its warps (and, for
 // narrow rows, lanes) take every so many-th part each, joined in a fixed order.
-constexpr int JOIN_MANY = 64;
+constexpr int JOIN_MANY = 32;
 constexpr int JOIN_WARPS = GT / 32;
 
 struct JoinItem {
@@ -223,19 +273,55 @@ __device__ __forceinline__ float add_parts(const float* p, long long C, long lon
   return acc;
 }
 
+// Zeros for the rows without a use, a group of lanes for each; the bits of 0 are the same in every type.
+template <class W>
+__device__ __forceinline__ void zero_rows(const GradArgs& a, void* gtable, long long block, long long blocks) {
+  constexpr int UN = 4;
+  const int gl = threadIdx.x % a.lanes;
+  const long long groups = blocks * GT / a.lanes;
+  W* g = static_cast<W*>(gtable);
+  W z;
+  memset(&z, 0, sizeof z);
+  for (long long v = (block * GT + threadIdx.x) / a.lanes; v < a.u.R; v += UN * groups) {
+    bool hit[UN];
+#pragma unroll
+    for (int i = 0; i < UN; ++i) hit[i] = v + i * groups < a.u.R && !__ldg(a.used + v + i * groups);
+#pragma unroll
+    for (int i = 0; i < UN; ++i)
+      if (hit[i])
+        for (long long k = gl; k < a.units; k += a.lanes) g[(v + i * groups) * a.units + k] = z;
+  }
+}
+
+// A lane tests a chunk for a split row that begins in it; the warp then adds what the lanes found, one row after
+// the other.  The blocks behind these write the rows that nothing looks up.
+constexpr int JOIN_TEST = 8;        // chunks of a warp
+
 template <class T>
-__global__ void __launch_bounds__(GT) k_rows_join(GradArgs a, int lanes, T* __restrict__ gtable) {
-  __shared__ JoinItem s_many[GT];
+__global__ void __launch_bounds__(GT) k_rows_join(GradArgs a, int lanes, unsigned join_blocks, T* __restrict__ gtable) {
+  __shared__ JoinItem s_many[JOIN_TEST * JOIN_WARPS];
   __shared__ int s_n;
   __shared__ float s_sum[JOIN_WARPS][32];
   const long long N = a.u.N, C = a.C, L = a.L;
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, gl = threadIdx.x % lanes;
-  const long long chunk = ((long long)blockIdx.x * GT + threadIdx.x) / lanes;
-  const long long c0 = (long long)blockIdx.y * lanes, cstep = (long long)gridDim.y * lanes;
+  const unsigned R = (unsigned)a.u.R;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  if (blockIdx.x >= join_blocks) {
+    if (blockIdx.y > 0) return;
+    if (a.unit == 16)
+      zero_rows<uint4>(a, gtable, blockIdx.x - join_blocks, gridDim.x - join_blocks);
+    else if (a.unit == 4)
+      zero_rows<unsigned>(a, gtable, blockIdx.x - join_blocks, gridDim.x - join_blocks);
+    else
+      zero_rows<unsigned short>(a, gtable, blockIdx.x - join_blocks, gridDim.x - join_blocks);
+    return;
+  }
   if (threadIdx.x == 0) s_n = 0;
   __syncthreads();
-  if (chunk < a.chunks) {
-    const ChunkEnds c(a, chunk);
+  const long long chunk = ((long long)blockIdx.x * JOIN_WARPS + wid) * JOIN_TEST + lane;
+  JoinItem it{0, 0, 0};
+  bool found = false;
+  if (lane < JOIN_TEST && chunk < a.chunks) {
+    const ChunkEnds c(chunk, N, L, R, [&](long long i) { return i >= 0 && i < N ? __ldg(&a.s[i].x) : R; });
     if (c.split && !(c.open && c.last == c.first)) {
       // the row's last use
       long long lo = c.i1 + L, hi = N;
@@ -254,18 +340,29 @@ __global__ void __launch_bounds__(GT) k_rows_join(GradArgs a, int lanes, T* __re
         else
           hi = mid;
       }
-      const long long last = (lo - 1) / L;
-      if (last - chunk > JOIN_MANY) {
-        if (gl == 0) s_many[atomicAdd(&s_n, 1)] = JoinItem{chunk, last, c.last};
-      } else {
-        for (long long b = c0 + gl; b < C; b += cstep)
-          gtable[(long long)c.last * C + b] =
-              from_f32<T>(a.partial[(2 * chunk + 1) * C + b] + add_parts(a.partial + b, C, chunk + 1, last + 1, 1));
-      }
+      it = JoinItem{chunk, (lo - 1) / L, c.last};
+      found = it.last - chunk <= JOIN_MANY;
+      if (!found) s_many[atomicAdd(&s_n, 1)] = it;
+    }
+  }
+  const int nq = 32 / lanes, q = lane / lanes, gl = lane % lanes;
+  const long long c0 = (long long)blockIdx.y * lanes, cstep = (long long)gridDim.y * lanes;
+  unsigned todo = __ballot_sync(0xffffffffu, found);
+  while (todo) {
+    const int src = __ffs(todo) - 1;
+    todo &= todo - 1;
+    const JoinItem f{__shfl_sync(0xffffffffu, it.chunk, src), __shfl_sync(0xffffffffu, it.last, src),
+                     __shfl_sync(0xffffffffu, it.row, src)};
+    for (long long b = c0; b < C; b += cstep) {
+      const long long col = b + gl;
+      float sum = 0.f;
+      if (col < C) sum = add_parts(a.partial + col, C, f.chunk + 1 + q, f.last + 1, nq);
+      for (int d = 16; d >= lanes; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (q == 0 && col < C) gtable[(long long)f.row * C + col] = from_f32<T>(a.partial[(2 * f.chunk + 1) * C + col] + sum);
     }
   }
   __syncthreads();
-  const int nq = 32 / lanes, q = lane / lanes, n = s_n;
+  const int n = s_n;
   for (int m = 0; m < n; ++m) {
     const JoinItem f = s_many[m];
     for (long long b = c0; b < C; b += cstep) {
@@ -285,7 +382,7 @@ __global__ void __launch_bounds__(GT) k_rows_join(GradArgs a, int lanes, T* __re
   }
 }
 
-size_t grad_space(long long N, long long C) { return align256((size_t)chunks_of(N) * 2 * (size_t)C * sizeof(float)); }
+size_t grad_space(long long N, long long C) { return align256((size_t)chunks_of(N, C) * 2 * (size_t)C * sizeof(float)); }
 
 template <class T>
 static int grad_unit(const void* table, long long table_stride, long long C, const void* gout, long long gout_stride,
@@ -303,14 +400,14 @@ bool grad_takes_weights(const void* table, long long table_stride, int type, lon
   return grad_shape(C, elem_bytes(type), grad_unit(type, table, table_stride, C, gout, gout_stride, gtable)).parts == 1;
 }
 
-int rows_grad(const RowUses& u, const uint2* sorted, const uint8_t* used, const void* table, long long table_stride, int type,
+int rows_grad(const RowUses& u, const uint2* sorted, uint8_t* used, const void* table, long long table_stride, int type,
               long long C, const void* gout, long long gout_stride, void* gtable, float* gweight, float* partial,
               cudaStream_t st) {
   const void* t = gweight ? table : nullptr;
   const int vb = grad_unit(type, t, table_stride, C, gout, gout_stride, gtable);
   GradShape g = grad_shape(C, elem_bytes(type), vb);
   // few chunks of wide rows: one unit a lane, more column parts
-  if (!gweight && g.per_lane > 1 && chunks_of(u.N) * g.lanes < 148 * 512) {
+  if (!gweight && g.per_lane > 1 && chunks_of(u.N, C) * g.lanes < 148 * 512) {
     g.per_lane = 1;
     g.parts = (int)((g.units + g.lanes - 1) / g.lanes);
     if (g.parts > 65535) g = grad_shape(C, elem_bytes(type), vb);
@@ -322,16 +419,15 @@ int rows_grad(const RowUses& u, const uint2* sorted, const uint8_t* used, const 
   a.C = C;
   a.table_stride = table_stride;
   a.gout_stride = gout_stride;
-  a.chunks = chunks_of(u.N);
-  a.L = chunk_len(u.N);
+  a.chunks = chunks_of(u.N, C);
+  a.L = chunk_len(u.N, C);
   a.lanes = g.lanes;
   a.units = (int)g.units;
+  a.unit = vb;
   a.gweight = gweight;
   a.partial = partial;
   const int per_block = GT / g.lanes;
-  a.group_blocks = (a.chunks + per_block - 1) / per_block;
-  const long long zero_blocks = used ? (u.R + per_block - 1) / per_block : 0;
-  const dim3 grid((unsigned)(a.group_blocks + zero_blocks), (unsigned)g.parts);
+  const dim3 grid((unsigned)((a.chunks + per_block - 1) / per_block), (unsigned)g.parts);
   return with_unit(type, vb, [&](auto e, auto b) {
     using T = decltype(e);
     constexpr int VB = decltype(b)::value;
@@ -353,12 +449,14 @@ int rows_grad(const RowUses& u, const uint2* sorted, const uint8_t* used, const 
       else
         k_rows_grad<T, VB, 4, false><<<grid, GT, 0, st>>>(a, tb, go, gt);
     }
-    if (a.chunks > 2) {      // a split row covers a chunk whole
+    if (a.chunks > 2 || used) {      // (a split row covers a chunk whole)
       int lanes = 1;
       while (lanes < 32 && lanes < C) lanes *= 2;
-      const long long cols = (C + lanes - 1) / lanes;
-      const dim3 jg((unsigned)((a.chunks * lanes + GT - 1) / GT), (unsigned)(cols < 32 ? cols : 32));
-      k_rows_join<T><<<jg, GT, 0, st>>>(a, lanes, gt);
+      const long long cols = (C + lanes - 1) / lanes, per = JOIN_TEST * JOIN_WARPS;
+      const unsigned jb = (unsigned)((a.chunks + per - 1) / per);
+      const long long rows = used ? (u.R * g.lanes + 4 * GT - 1) / (4 * GT) : 0;
+      const dim3 jg(jb + (unsigned)(rows < 148 * 8 ? rows : 148 * 8), (unsigned)(cols < 32 ? cols : 32));
+      k_rows_join<T><<<jg, GT, 0, st>>>(a, lanes, jb, gt);
     }
     return check_launch("row gradient");
   });

@@ -56,11 +56,9 @@ __device__ __forceinline__ unsigned same_digit(unsigned d, int bits, bool in) {
   return m;
 }
 
-// Digit counts of every pass, and the flags of the rows that are looked up.  One block per SM, so that few
-// blocks add their counts to the same words.
+// Digit counts of every pass.  One block per SM, so that few blocks add their counts to the same words.
 constexpr int DT = 1024;
-__global__ void __launch_bounds__(DT) k_sort_digits(RowUses u, Digits dg, unsigned* __restrict__ counts,
-                                                    uint8_t* __restrict__ used) {
+__global__ void __launch_bounds__(DT) k_sort_digits(RowUses u, Digits dg, unsigned* __restrict__ counts) {
   __shared__ unsigned h[MAX_PASSES * MAX_DIGITS];
   constexpr int UN = 4;
   const int D = 1 << dg.bits, all = dg.passes * D;
@@ -74,7 +72,6 @@ __global__ void __launch_bounds__(DT) k_sort_digits(RowUses u, Digits dg, unsign
 #pragma unroll
     for (int i = 0; i < UN; ++i) {
       if (n0 + i * step >= u.N) break;
-      if (k[i] < (unsigned)u.R) used[k[i]] = 1;
       for (int p = 0; p < dg.passes; ++p) atomicAdd(&h[p * D + ((k[i] >> dg.shift(p)) & (D - 1))], 1u);
     }
   }
@@ -360,7 +357,7 @@ int sort_uses(const RowUses& u, const SortSpace& s, void* clear, size_t clear_by
   unsigned* states = reinterpret_cast<unsigned*>(s.zeroed + align256((size_t)(MAX_PASSES + (size_t)dg.passes * D) * sizeof(unsigned)));
   long long blocks = (u.N + DT - 1) / DT;
   if (blocks > 148) blocks = 148;
-  k_sort_digits<<<(unsigned)blocks, DT, 0, st>>>(u, dg, counts, s.used);
+  k_sort_digits<<<(unsigned)blocks, DT, 0, st>>>(u, dg, counts);
   for (int p = 0; p < dg.passes; ++p) {
     // the last pass writes `sorted`, the ones before alternate so that none reads what it writes
     const bool to_sorted = (dg.passes - 1 - p) % 2 == 0;

@@ -355,7 +355,7 @@ def rows2d(t, width):
     between rows, an expanded one included); a copy where no such view exists."""
     if t.dim() != 2:
         t = t.reshape(-1, width) if width else t.reshape(t.shape[0], 0)
-    return t if width <= 1 or t.stride(1) == 1 else t.contiguous()
+    return t if (width <= 1 or t.stride(1) == 1) and t.stride(0) < 1 << 30 else t.contiguous()
 
 
 def _addr(t):
