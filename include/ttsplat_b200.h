@@ -54,8 +54,7 @@ const char* tts_last_error(void);
 
 /* Device status word written by kernels instead of trapping (bounded waits that gave up):
  * 1 = a bulk-copy wait of the forward, 2 = a relocation grid barrier, 4 = a peer barrier;
- * 8 = a cached binning table that spreads a gaussian over more than its stencil;
- * 16 = a wait of the row gradient's sort.
+ * 8 = a cached binning table that spreads a gaussian over more than its stencil.
  * Synchronous read + clear.  A non-zero word means a step skipped work: the Python train step
  * reads it at check_status / check_replicas and at the end of fit / train_mcmc, and raises. */
 int tts_read_status(int* status_host);

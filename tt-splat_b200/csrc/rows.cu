@@ -158,8 +158,8 @@ extern "C" int tts_gather_rows_bwd(const void* table, long long R, long long C, 
     char* w = reinterpret_cast<char*>(align256(reinterpret_cast<size_t>(workspace)));
     SortSpace s;
     const size_t at = sort_space(N, R, w, &s);
-    if (int rc = sort_uses(u, s, gtable, (size_t)R * C * elem(type), st)) return rc;
-    if (int rc = rows_grad(u, s.sorted, s.used, table, table_stride, type, C, gout, gout_stride, gtable,
+    if (int rc = sort_uses(u, s, gtable, (size_t)R * C * elem(type), fused ? gweight : nullptr, st)) return rc;
+    if (int rc = rows_grad(u, s, table, table_stride, type, C, gout, gout_stride, gtable,
                            fused ? gweight : nullptr, reinterpret_cast<float*>(w + at), st))
       return rc;
   }

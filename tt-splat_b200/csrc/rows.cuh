@@ -73,26 +73,28 @@ inline int with_unit(int type, int vb, F f) {
 inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // ---- the uses in row order ---------------------------------------------------------------------
-// Entries (row, use) sorted by row, equal rows in the order of their uses; unused and out-of-range slots
-// have the key R, behind every row.
+// Entries (row, use) sorted by row, equal rows in the order of their uses; unused and out-of-range slots are
+// left out.
 constexpr long long SORT_SMALL = 8192;      // uses up to which one block sorts them in shared memory
 
 struct SortSpace {
+  unsigned* n;         // entries in `sorted`
   uint2* sorted;       // [N] the result
-  uint2* other;        // [N] the pass before the last (large sorts)
-  char* zeroed;        // cleared before a large sort: digit counts, tickets, tile states, row flags
-  size_t zeroed_bytes;
-  uint8_t* used;       // [R] flags for the rows that are looked up, cleared (large sorts)
+  uint2* other;        // [N] the pass before the last (large sorts, as the rest)
+  unsigned* counts;    // digit counts of each tile
+  unsigned* totals;    // digit counts
+  uint8_t* used;       // [R] flags for the rows that are looked up, cleared
 };
 
 size_t sort_space(long long N, long long R, void* base, SortSpace* s);
-// Launches the sort.  Up to SORT_SMALL uses it clears the `clear_bytes` at `clear` as well (the whole
-// gradient); beyond, it clears the `used` flags instead, for the caller to find the rows without a use.
-int sort_uses(const RowUses& u, const SortSpace& s, void* clear, size_t clear_bytes, cudaStream_t st);
+// Launches the sort, which also clears the weights' gradients (or NULL) of slots that look nothing up.  Up to
+// SORT_SMALL uses it clears the `clear_bytes` at `clear` (the whole gradient); beyond, it clears the `used`
+// flags instead, for the caller to find the rows without a use.
+int sort_uses(const RowUses& u, const SortSpace& s, void* clear, size_t clear_bytes, float* gweight, cudaStream_t st);
 
 // ---- the sums over the sorted uses ---------------------------------------------------------------
 size_t grad_space(long long N, long long C);
-int rows_grad(const RowUses& u, const uint2* sorted, uint8_t* used, const void* table, long long table_stride, int type,
+int rows_grad(const RowUses& u, const SortSpace& s, const void* table, long long table_stride, int type,
               long long C, const void* gout, long long gout_stride, void* gtable, float* gweight, float* partial,
               cudaStream_t st);
 // Whether rows_grad can write the weights' gradient on its way (a row fits a warp's registers).

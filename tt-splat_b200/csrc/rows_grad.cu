@@ -45,6 +45,7 @@ static GradShape grad_shape(long long C, int elem, int vb) {
 struct GradArgs {
   RowUses u;
   const uint2* s;
+  const unsigned* n;
   uint8_t* used;
   long long C, table_stride, gout_stride, chunks;
   int L, lanes, units, unit;
@@ -106,21 +107,22 @@ __global__ void __launch_bounds__(GT, GW && PL * VB <= 8 ? 3 : 1) k_rows_grad(Gr
   constexpr int SPAN = BLOCK_USES + 2 * L_MAX + 2;
   __shared__ unsigned s_key[SPAN], s_use[SPAN];
   __shared__ float s_f[SPAN];
-  const long long N = a.u.N;
+  const long long N = *a.n;
   const unsigned R = (unsigned)a.u.R;
   // the block's uses, and as many beside them as a chunk looks at
   const int groups = GT / a.lanes, first = a.L + 1, behind = first + groups * a.L;
   const long long at = (long long)blockIdx.x * groups * a.L - first;
   for (int k = threadIdx.x; k < behind + first; k += GT) {
     const long long i = at + k;
-    uint2 p = make_uint2(R, 0xffffffffu);
-    if (i >= 0 && i < N) p = __ldg(a.s + i);
-    // (a row or use past the end only after a wait of the sort that ran out)
-    const bool in = p.x < R && p.y < N;
-    s_key[k] = in ? p.x : R;
+    uint2 p = make_uint2(R, 0);
+    float f = 0.f;
+    if (i >= 0 && i < N) {
+      p = __ldg(a.s + i);
+      f = factor_of(a.u, p.y);
+    }
+    s_key[k] = p.x;
     s_use[k] = p.y;
-    s_f[k] = in ? factor_of(a.u, p.y) : 0.f;
-    if (GW && !in && p.y < N && k >= first && k < behind) a.gweight[p.y] = 0.f;
+    s_f[k] = f;
   }
   __syncthreads();
   if (a.used && blockIdx.y == 0)
@@ -128,10 +130,9 @@ __global__ void __launch_bounds__(GT, GW && PL * VB <= 8 ? 3 : 1) k_rows_grad(Gr
       if (s_key[k] < R && s_key[k] != s_key[k - 1]) a.used[s_key[k]] = 1;
   const int group = threadIdx.x / a.lanes, gl = threadIdx.x % a.lanes;
   const long long chunk = (long long)blockIdx.x * groups + group;
-  if (chunk >= a.chunks) return;
+  if (chunk * a.L >= N) return;
   const ChunkEnds c(chunk, N, a.L, R, [&](long long i) { return s_key[i - at]; });
-  // the chunk's uses, without those of a first row that it skips, with those of a last row that it follows,
-  // and without unused slots, which lie at the end
+  // the chunk's uses, without those of a first row that it skips, with those of a last row that it follows
   auto first_at_least = [&](int lo, int hi, unsigned v) {
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
@@ -144,10 +145,7 @@ __global__ void __launch_bounds__(GT, GW && PL * VB <= 8 ? 3 : 1) k_rows_grad(Gr
   };
   int j = (int)(c.i0 - at), end = (int)(c.i1 - at);
   if (c.skip) j = first_at_least(j, end, c.first + 1);
-  if (c.follow)
-    end = first_at_least(end, end + a.L, c.last + 1);
-  else if (c.last >= R)
-    end = first_at_least(j, end, R);
+  if (c.follow) end = first_at_least(end, end + a.L, c.last + 1);
   const int u0 = blockIdx.y * a.lanes * PL + gl;
   bool col[PL];
 #pragma unroll
@@ -298,11 +296,11 @@ __device__ __forceinline__ void zero_rows(const GradArgs& a, void* gtable, long 
 constexpr int JOIN_TEST = 8;        // chunks of a warp
 
 template <class T>
-__global__ void __launch_bounds__(GT) k_rows_join(GradArgs a, int lanes, unsigned join_blocks, T* __restrict__ gtable) {
+__global__ void __launch_bounds__(GT, 5) k_rows_join(GradArgs a, int lanes, unsigned join_blocks, T* __restrict__ gtable) {
   __shared__ JoinItem s_many[JOIN_TEST * JOIN_WARPS];
   __shared__ int s_n;
   __shared__ float s_sum[JOIN_WARPS][32];
-  const long long N = a.u.N, C = a.C, L = a.L;
+  const long long N = *a.n, C = a.C, L = a.L;
   const unsigned R = (unsigned)a.u.R;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   if (blockIdx.x >= join_blocks) {
@@ -320,7 +318,7 @@ __global__ void __launch_bounds__(GT) k_rows_join(GradArgs a, int lanes, unsigne
   const long long chunk = ((long long)blockIdx.x * JOIN_WARPS + wid) * JOIN_TEST + lane;
   JoinItem it{0, 0, 0};
   bool found = false;
-  if (lane < JOIN_TEST && chunk < a.chunks) {
+  if (lane < JOIN_TEST && chunk * L < N) {
     const ChunkEnds c(chunk, N, L, R, [&](long long i) { return i >= 0 && i < N ? __ldg(&a.s[i].x) : R; });
     if (c.split && !(c.open && c.last == c.first)) {
       // the row's last use
@@ -400,7 +398,7 @@ bool grad_takes_weights(const void* table, long long table_stride, int type, lon
   return grad_shape(C, elem_bytes(type), grad_unit(type, table, table_stride, C, gout, gout_stride, gtable)).parts == 1;
 }
 
-int rows_grad(const RowUses& u, const uint2* sorted, uint8_t* used, const void* table, long long table_stride, int type,
+int rows_grad(const RowUses& u, const SortSpace& s, const void* table, long long table_stride, int type,
               long long C, const void* gout, long long gout_stride, void* gtable, float* gweight, float* partial,
               cudaStream_t st) {
   const void* t = gweight ? table : nullptr;
@@ -414,8 +412,9 @@ int rows_grad(const RowUses& u, const uint2* sorted, uint8_t* used, const void* 
   }
   GradArgs a;
   a.u = u;
-  a.s = sorted;
-  a.used = used;
+  a.s = s.sorted;
+  a.n = s.n;
+  a.used = s.used;
   a.C = C;
   a.table_stride = table_stride;
   a.gout_stride = gout_stride;
@@ -449,12 +448,12 @@ int rows_grad(const RowUses& u, const uint2* sorted, uint8_t* used, const void* 
       else
         k_rows_grad<T, VB, 4, false><<<grid, GT, 0, st>>>(a, tb, go, gt);
     }
-    if (a.chunks > 2 || used) {      // (a split row covers a chunk whole)
+    if (a.chunks > 2 || a.used) {      // (a split row covers a chunk whole)
       int lanes = 1;
       while (lanes < 32 && lanes < C) lanes *= 2;
       const long long cols = (C + lanes - 1) / lanes, per = JOIN_TEST * JOIN_WARPS;
       const unsigned jb = (unsigned)((a.chunks + per - 1) / per);
-      const long long rows = used ? (u.R * g.lanes + 4 * GT - 1) / (4 * GT) : 0;
+      const long long rows = a.used ? (u.R * g.lanes + 4 * GT - 1) / (4 * GT) : 0;
       const dim3 jg(jb + (unsigned)(rows < 148 * 8 ? rows : 148 * 8), (unsigned)(cols < 32 ? cols : 32));
       k_rows_join<T><<<jg, GT, 0, st>>>(a, lanes, jb, gt);
     }

@@ -1,31 +1,28 @@
-// Stable sort of the uses of a table's rows by row: LSD radix sort of (row, use) pairs.
+// Stable sort of the uses of a table's rows by row: LSD radix sort of (row, use) pairs.  Unused and
+// out-of-range slots are left out on the way.
 //
-// A use's place in a pass is the count of smaller digits everywhere, of equal digits in the tiles before
-// its own, and of equal digits before it in the tile.  The first comes from one counting kernel over the
-// indices (all passes at once), the last from ballots inside a warp and the warps' counts in shared memory.
-// The middle one is passed from tile to tile in the same launch: a tile publishes its counts, then adds up
-// those of the tiles before it, from the nearest back, until it meets one that has its own sum already.
-// Tiles are numbered by a ticket, so every tile that is waited for has started; the wait has a limit all
-// the same.  Each pass therefore reads and writes the pairs once.
+// A use's place in a pass is the count of smaller digits everywhere, of equal digits in the tiles before its
+// own, and of equal digits before it in the tile.  A pass is three launches: the tiles' digit counts; their
+// running sums over the tiles, digit by digit; and the move, in which a tile ranks its uses (ballots inside a
+// warp, the warps' counts in shared memory), orders them in shared memory and writes every digit's run.  No
+// block waits for another.  For 2M uses of 1M rows the sort takes 70 us; with one launch per pass, in which a
+// tile adds up what the tiles before it publish, it took 85 us: at 1024 digits the polling costs more than the
+// counts.  Tiles of 2048 uses: 4096 and 8192 leave SMs idle (move 47 instead of 41 us at 2M uses, 9 instead of
+// 7 us at 100k).  The moves are bound by the ballots (13 cycles a bit and warp).
 //
-// Digits have up to 10 bits and the passes share the bits evenly: 2 passes up to 2^20 rows.
+// Digits have 6 to 10 bits and the passes share the bits evenly: 2 passes up to 2^20 rows.
+#include <type_traits>
+
 #include "rows.cuh"
 
 namespace tts {
 
-constexpr int ST = 512;                       // threads of a tile
+constexpr int ST = 256;                       // threads of a tile
 constexpr int SW = ST / 32;
-constexpr int SI = 16;                        // entries per thread
+constexpr int SI = 8;                         // uses per thread
 constexpr int TILE = ST * SI;
-constexpr int MAX_BITS = 10;
+constexpr int MIN_BITS = 6, MAX_BITS = 10;
 constexpr int MAX_DIGITS = 1 << MAX_BITS;
-constexpr int MAX_PASSES = 4;
-constexpr int BACK = 8;                       // earlier tiles that a wait looks at in one go
-constexpr int PER = MAX_DIGITS / ST;          // neighbouring digits of a thread, their states one word pair
-static_assert(PER == 2, "a thread's digits are one 8-byte word of states and one 4-byte word of counts");
-constexpr int STATUS_SORT_TIMEOUT = 16;
-// tile states: what is published, in the top two bits of a word whose rest is the count (N < 2^30)
-constexpr unsigned HAVE_COUNT = 1u << 30, HAVE_SUM = 2u << 30, VALUE = (1u << 30) - 1;
 
 struct Digits {
   int bits, passes;
@@ -33,13 +30,15 @@ struct Digits {
 };
 static Digits digits_for(long long R, int max_bits) {
   int b = 1;
-  while ((R >> b) > 0) ++b;                   // keys are 0 .. R
+  while (((R - 1) >> b) > 0) ++b;             // keys are 0 .. R - 1
   Digits d;
   d.passes = (b + max_bits - 1) / max_bits;
   d.bits = (b + d.passes - 1) / d.passes;
+  if (d.bits < MIN_BITS) d.bits = MIN_BITS;
   return d;
 }
 
+// The row of use n, R where there is none.
 __device__ __forceinline__ unsigned key_of(const RowUses& u, long long n) {
   const long long v = row_of(u, n);
   return (unsigned)(v < 0 ? u.R : v);
@@ -47,165 +46,192 @@ __device__ __forceinline__ unsigned key_of(const RowUses& u, long long n) {
 
 // Lanes of the warp with the same digit as this one (ballots over its bits); lanes that are not `in`
 // match nobody.
-__device__ __forceinline__ unsigned same_digit(unsigned d, int bits, bool in) {
+template <int BITS>
+__device__ __forceinline__ unsigned same_digit(unsigned d, bool in) {
   unsigned m = __ballot_sync(0xffffffffu, in);
-  for (int b = 0; b < bits; ++b) {
+#pragma unroll
+  for (int b = 0; b < BITS; ++b) {
     const unsigned set = __ballot_sync(0xffffffffu, (d >> b) & 1u);
     m &= ((d >> b) & 1u) ? set : ~set;
   }
   return m;
 }
 
-// Digit counts of every pass.  One block per SM, so that few blocks add their counts to the same words.
-constexpr int DT = 1024;
-__global__ void __launch_bounds__(DT) k_sort_digits(RowUses u, Digits dg, unsigned* __restrict__ counts) {
-  __shared__ unsigned h[MAX_PASSES * MAX_DIGITS];
-  constexpr int UN = 4;
-  const int D = 1 << dg.bits, all = dg.passes * D;
-  for (int i = threadIdx.x; i < all; i += DT) h[i] = 0;
-  __syncthreads();
-  const long long step = (long long)gridDim.x * DT;
-  for (long long n0 = (long long)blockIdx.x * DT + threadIdx.x; n0 < u.N; n0 += UN * step) {
-    unsigned k[UN];
+// What a pass reads: the indices themselves in the first (every use, R where there is no row), the pairs of
+// the pass before in the others (*n of them).
+struct PassIn {
+  RowUses u;
+  const uint2* src;
+  const unsigned* n;
+  int shift;
+  __device__ __forceinline__ long long count() const { return src ? (long long)*n : u.N; }
+  __device__ __forceinline__ uint2 get(long long i, long long N) const {
+    if (i >= N) return make_uint2((unsigned)u.R, 0);
+    return src ? src[i] : make_uint2(key_of(u, i), (unsigned)i);
+  }
+};
+
+// Exclusive sum over the block's threads of x (all of ST threads take part).
+__device__ __forceinline__ unsigned block_before(unsigned x, unsigned* s_scan) {
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  unsigned incl = x;
 #pragma unroll
-    for (int i = 0; i < UN; ++i) k[i] = n0 + i * step < u.N ? key_of(u, n0 + i * step) : 0u;
-#pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      if (n0 + i * step >= u.N) break;
-      for (int p = 0; p < dg.passes; ++p) atomicAdd(&h[p * D + ((k[i] >> dg.shift(p)) & (D - 1))], 1u);
-    }
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < all; i += DT)
-    if (h[i]) atomicAdd(counts + i, h[i]);
-}
-
-__device__ __forceinline__ uint2 load_state(const unsigned* p) {
-  uint2 v;
-  asm volatile("ld.relaxed.gpu.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ void store_state(unsigned* p, uint2 v) {
-  asm volatile("st.relaxed.gpu.global.v2.u32 [%0], {%1, %2};" ::"l"(p), "r"(v.x), "r"(v.y) : "memory");
-}
-// The published words of both digits, which arrive each by itself: ready when both are there.
-__device__ __forceinline__ bool ready(uint2 s) { return (s.x >> 30) != 0 && (s.y >> 30) != 0; }
-
-__global__ void __launch_bounds__(ST) k_sort_pass(RowUses u, const uint2* __restrict__ src, Digits dg, int pass,
-                                                  const unsigned* __restrict__ counts, unsigned* __restrict__ ticket,
-                                                  unsigned* __restrict__ states, uint2* __restrict__ dst) {
-  __shared__ __align__(16) unsigned short s_warp[SW][MAX_DIGITS];     // counts of each warp, then of the warps before it
-  __shared__ unsigned s_base[MAX_DIGITS];               // where the tile's first entry of a digit goes
-  __shared__ unsigned s_scan[SW];
-  __shared__ unsigned s_tile;
-  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  const int D = 1 << dg.bits, shift = dg.shift(pass);
-  if (tid == 0) s_tile = atomicAdd(ticket, 1u);
-  for (int i = tid; i < SW * MAX_DIGITS / 8; i += ST) reinterpret_cast<uint4*>(s_warp)[i] = make_uint4(0, 0, 0, 0);
+  if (lane == 31) s_scan[wid] = incl;
   __syncthreads();
-  const unsigned tile = s_tile;
-  const long long base = (long long)tile * TILE + wid * (32 * SI);
+  unsigned run = incl - x;
+#pragma unroll
+  for (int w = 0; w < SW; ++w)
+    if (w < wid) run += s_scan[w];
+  return run;
+}
+
+// counts[tile][digit].  The first pass also clears the rows' flags and the weights' gradients of uses without
+// a row.
+__global__ void __launch_bounds__(ST) k_sort_count(PassIn in, int digits, unsigned* __restrict__ counts,
+                                                   uint8_t* __restrict__ used, float* __restrict__ gweight) {
+  __shared__ unsigned h[MAX_DIGITS];
+  for (int i = threadIdx.x; i < digits; i += ST) h[i] = 0;
+  __syncthreads();
+  const long long base = (long long)blockIdx.x * TILE, N = in.count();
+  unsigned k[SI];
+#pragma unroll
+  for (int i = 0; i < SI; ++i) k[i] = in.get(base + i * ST + threadIdx.x, N).x;
+#pragma unroll
+  for (int i = 0; i < SI; ++i) {
+    if (k[i] < (unsigned)in.u.R)
+      atomicAdd(&h[(k[i] >> in.shift) & (digits - 1)], 1u);
+    else if (gweight && base + i * ST + threadIdx.x < N)
+      gweight[base + i * ST + threadIdx.x] = 0.f;
+  }
+  if (used) {
+    const long long step = (long long)gridDim.x * ST, words = in.u.R / 16;
+    const long long t = (long long)blockIdx.x * ST + threadIdx.x;
+    for (long long i = t; i < words; i += step) reinterpret_cast<uint4*>(used)[i] = make_uint4(0, 0, 0, 0);
+    if (t < in.u.R - words * 16) used[words * 16 + t] = 0;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < digits; i += ST) counts[(long long)blockIdx.x * digits + i] = h[i];
+}
+
+// Running sums of the counts over the tiles (exclusive, in place) and the digits' totals: a block takes 32
+// digits, a lane for each, its warps consecutive parts of the tiles.
+constexpr int SCAN_WARPS = 32;
+__global__ void __launch_bounds__(32 * SCAN_WARPS) k_sort_scan(unsigned* __restrict__ counts, long long tiles, int digits,
+                                                               unsigned* __restrict__ totals) {
+  __shared__ unsigned s_part[SCAN_WARPS][32];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int d = blockIdx.x * 32 + lane;
+  const long long t0 = tiles * wid / SCAN_WARPS, t1 = tiles * (wid + 1) / SCAN_WARPS;
+  unsigned sum = 0;
+#pragma unroll 8
+  for (long long t = t0; t < t1; ++t) sum += counts[t * digits + d];
+  s_part[wid][lane] = sum;
+  __syncthreads();
+  unsigned run = 0;
+#pragma unroll
+  for (int w = 0; w < SCAN_WARPS; ++w)
+    if (w < wid) run += s_part[w][lane];
+  if (wid == SCAN_WARPS - 1) totals[d] = run + sum;
+  for (long long t = t0; t < t1; t += 8) {
+    unsigned c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = t + i < t1 ? counts[(t + i) * digits + d] : 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (t + i < t1) counts[(t + i) * digits + d] = run;
+      run += c[i];
+    }
+  }
+}
+
+template <int BITS>
+__global__ void __launch_bounds__(ST, 4) k_sort_move(PassIn in, const unsigned* __restrict__ counts,
+                                                  const unsigned* __restrict__ totals, unsigned* __restrict__ n_used,
+                                                  uint2* __restrict__ dst) {
+  constexpr int D = 1 << BITS, PER = D > ST ? D / ST : 1;
+  // the warps' digit counts, then (every place known) the tile's uses in order
+  __shared__ __align__(16) union {
+    unsigned short warp[SW][D];
+    uint2 e[TILE];
+  } s;
+  __shared__ unsigned s_start[D];      // where a digit begins in the tile
+  __shared__ unsigned s_to[D];         // and its uses' places in dst, less that
+  __shared__ unsigned s_scan[SW];
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  const unsigned R = (unsigned)in.u.R;
+  for (int i = tid; i < SW * D / 8; i += ST) reinterpret_cast<uint4*>(s.warp)[i] = make_uint4(0, 0, 0, 0);
+  const long long N = in.count(), base = (long long)blockIdx.x * TILE + wid * (32 * SI);
   uint2 e[SI];
   unsigned short rank[SI];
 #pragma unroll
-  for (int i = 0; i < SI; ++i) {
-    const long long n = base + i * 32 + lane;
-    e[i] = make_uint2(0, 0);
-    if (n < u.N) e[i] = src ? src[n] : make_uint2(key_of(u, n), (unsigned)n);
-  }
+  for (int i = 0; i < SI; ++i) e[i] = in.get(base + i * 32 + lane, N);
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < SI; ++i) {
-    const bool in = base + i * 32 + lane < u.N;
-    const unsigned d = (e[i].x >> shift) & (D - 1);
-    const unsigned peers = same_digit(d, dg.bits, in);
-    const unsigned first = s_warp[wid][d];
-    rank[i] = (unsigned short)(first + __popc(peers & ((1u << lane) - 1)));
+    const bool here = e[i].x < R;
+    const unsigned d = here ? (e[i].x >> in.shift) & (D - 1) : 0u;
+    const unsigned peers = same_digit<BITS>(d, here);
+    rank[i] = (unsigned short)(s.warp[wid][d] + __popc(peers & ((1u << lane) - 1)));
     __syncwarp();
-    if (in && (peers >> lane) == 1u) s_warp[wid][d] = (unsigned short)(rank[i] + 1);
+    if (here && (peers >> lane) == 1u) s.warp[wid][d] = (unsigned short)(rank[i] + 1);
     __syncwarp();
   }
   __syncthreads();
-  // the tile's counts (two digits to a word), published before anything is waited for
-  const int d0 = tid * PER;
-  uint2 count = make_uint2(0, 0);
-  if (d0 < D) {
-    unsigned run = 0;
+  // per digit: the warps' counts become those of the warps before; then the digits' starts, in the tile and
+  // in the whole
+  unsigned here[PER], all[PER], h = 0, a = 0;
 #pragma unroll
-    for (int w = 0; w < SW; ++w) {
-      unsigned* p = reinterpret_cast<unsigned*>(&s_warp[w][d0]);
-      const unsigned c = *p;
-      *p = run;
-      run += c;
-    }
-    count = make_uint2(run & 0xffffu, run >> 16);
-    if (tile > 0) store_state(states + (long long)tile * D + d0, make_uint2(HAVE_COUNT | count.x, HAVE_COUNT | count.y));
-  }
-  uint2 before = make_uint2(0, 0);
-  if (tile == 0) {
-    // the first tile starts each digit behind the smaller ones
-    uint2 c = make_uint2(0, 0);
-    if (d0 < D) c = make_uint2(counts[d0], counts[d0 + 1]);
-    unsigned incl = c.x + c.y;
+  for (int q = 0; q < PER; ++q) {
+    const int d = tid * PER + q;
+    here[q] = all[q] = 0;
+    if (d < D) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned y = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += y;
-    }
-    if (lane == 31) s_scan[wid] = incl;
-    __syncthreads();
-    before.x = incl - c.x - c.y;
-    for (int w = 0; w < wid; ++w) before.x += s_scan[w];
-    before.y = before.x + c.x;
-  } else if (d0 < D) {
-    long long t = (long long)tile - 1;
-    int tries = 0;
-    bool done = false;
-    while (!done && tries < (1 << 20)) {
-      // a few tiles at once, the nearest first; stop at one that has not published yet
-      uint2 s[BACK];
-#pragma unroll
-      for (int j = 0; j < BACK; ++j) s[j] = t - j >= 0 ? load_state(states + (t - j) * D + d0) : make_uint2(0, 0);
-      bool go = true;
-      int seen = 0;
-#pragma unroll
-      for (int j = 0; j < BACK; ++j) {
-        go = go && !done && ready(s[j]);
-        if (go) {
-          // a sum counts where both words hold one; a tile that is just turning its counts into sums is read
-          // again in the next round
-          const bool sx = (s[j].x & HAVE_SUM) != 0, sy = (s[j].y & HAVE_SUM) != 0;
-          if (sx != sy) {
-            go = false;
-          } else {
-            before.x += s[j].x & VALUE;
-            before.y += s[j].y & VALUE;
-            ++seen;
-            done = sx;
-          }
-        }
+      for (int w = 0; w < SW; ++w) {
+        const unsigned c = s.warp[w][d];
+        s.warp[w][d] = (unsigned short)here[q];
+        here[q] += c;
       }
-      t -= seen;
-      if (seen == 0) ++tries;
+      all[q] = totals[d];
     }
-    if (!done) {
-      atomicOr(&g_status, STATUS_SORT_TIMEOUT);
-      before = make_uint2(VALUE, VALUE);
-    }
+    h += here[q];
+    a += all[q];
   }
-  if (d0 < D) {
-    store_state(states + (long long)tile * D + d0,
-                make_uint2(HAVE_SUM | ((before.x + count.x) & VALUE), HAVE_SUM | ((before.y + count.y) & VALUE)));
-    s_base[d0] = before.x;
-    s_base[d0 + 1] = before.y;
+  unsigned start = block_before(h, s_scan), to = block_before(a, s_scan);
+  if (n_used && blockIdx.x == 0 && tid == ST - 1) *n_used = to + a;
+#pragma unroll
+  for (int q = 0; q < PER; ++q) {
+    const int d = tid * PER + q;
+    if (d < D) {
+      s_start[d] = start;
+      s_to[d] = to + counts[(long long)blockIdx.x * D + d] - start;
+    }
+    start += here[q];
+    to += all[q];
+  }
+  __syncthreads();
+  unsigned at[SI];
+#pragma unroll
+  for (int i = 0; i < SI; ++i) {
+    const unsigned d = (e[i].x >> in.shift) & (D - 1);
+    at[i] = e[i].x < R ? s_start[d] + s.warp[wid][d] + rank[i] : 0xffffffffu;
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < SI; ++i)
-    if (base + i * 32 + lane < u.N) {
-      const unsigned d = (e[i].x >> shift) & (D - 1);
-      const long long at = (long long)s_base[d] + s_warp[wid][d] + rank[i];
-      if (at < u.N) dst[at] = e[i];           // never past the end, after a wait that ran out either
-    }
+    if (at[i] != 0xffffffffu) s.e[at[i]] = e[i];
+  // the last digit's end
+  if (tid == ST - 1) s_scan[0] = start;
+  __syncthreads();
+  const int n = (int)s_scan[0];
+  for (int i = tid; i < n; i += ST) {
+    const uint2 x = s.e[i];
+    dst[s_to[(x.x >> in.shift) & (D - 1)] + i] = x;
+  }
 }
 
 // ---- one block: up to SORT_SMALL uses in shared memory --------------------------------------------
@@ -217,13 +243,14 @@ constexpr int SS_BITS = 8;
 constexpr int SS_DIGITS = 1 << SS_BITS;
 constexpr size_t SS_SMEM = SORT_SMALL * sizeof(uint2) + SS_WARPS * SS_DIGITS * sizeof(unsigned short) + 2 * SS_DIGITS * sizeof(unsigned);
 
-__device__ void sort_small(const RowUses& u, Digits dg, uint2* sorted) {
+__device__ void sort_small(const RowUses& u, Digits dg, uint2* sorted, unsigned* n_used, float* gweight) {
   extern __shared__ __align__(16) char smem[];
   uint2* s_e = reinterpret_cast<uint2*>(smem);
   unsigned short(*s_warp)[SS_DIGITS] = reinterpret_cast<unsigned short(*)[SS_DIGITS]>(smem + SORT_SMALL * sizeof(uint2));
   unsigned* s_base = reinterpret_cast<unsigned*>(&s_warp[SS_WARPS][0]);
   unsigned* s_scan = s_base + SS_DIGITS;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  const unsigned R = (unsigned)u.R;
   const int N = (int)u.N, D = 1 << dg.bits;
   // the warps share the entries evenly, in order
   const int steps = (N + SS_THREADS - 1) / SS_THREADS;
@@ -232,8 +259,11 @@ __device__ void sort_small(const RowUses& u, Digits dg, uint2* sorted) {
 #pragma unroll
   for (int i = 0; i < SS_ITEMS; ++i) {
     const int n = base + i * 32;
-    e[i] = make_uint2(0, 0);
-    if (i < steps && n < N) e[i] = make_uint2(key_of(u, n), (unsigned)n);
+    e[i] = make_uint2(R, 0);
+    if (i < steps && n < N) {
+      e[i] = make_uint2(key_of(u, n), (unsigned)n);
+      if (gweight && e[i].x == R) gweight[n] = 0.f;
+    }
   }
   for (int p = 0; p < dg.passes; ++p) {
     const int shift = dg.shift(p);
@@ -243,9 +273,9 @@ __device__ void sort_small(const RowUses& u, Digits dg, uint2* sorted) {
 #pragma unroll
     for (int i = 0; i < SS_ITEMS; ++i)
       if (i < steps) {
-        const bool in = base + i * 32 < N;
+        const bool in = e[i].x < R;
         const unsigned d = (e[i].x >> shift) & (D - 1);
-        const unsigned peers = same_digit(d, dg.bits, in);
+        const unsigned peers = same_digit<SS_BITS>(d, in);
         rank[i] = (unsigned short)(s_warp[wid][d] + __popc(peers & ((1u << lane) - 1)));
         __syncwarp();
         if (in && (peers >> lane) == 1u) s_warp[wid][d] = (unsigned short)(rank[i] + 1);
@@ -273,11 +303,14 @@ __device__ void sort_small(const RowUses& u, Digits dg, uint2* sorted) {
       unsigned run = incl - count;
       for (int w = 0; w < wid; ++w) run += s_scan[w];
       s_base[tid] = run;
+      if (tid == D - 1) s_scan[SS_WARPS] = run + count;
     }
     __syncthreads();
+    const int n_left = (int)s_scan[SS_WARPS];
+    if (tid == 0 && p == 0) *n_used = n_left;
 #pragma unroll
     for (int i = 0; i < SS_ITEMS; ++i)
-      if (i < steps && base + i * 32 < N) {
+      if (e[i].x < R) {
         const unsigned d = (e[i].x >> shift) & (D - 1);
         const unsigned at = s_base[d] + s_warp[wid][d] + rank[i];
         if (p + 1 < dg.passes)
@@ -289,14 +322,15 @@ __device__ void sort_small(const RowUses& u, Digits dg, uint2* sorted) {
     if (p + 1 < dg.passes)
 #pragma unroll
       for (int i = 0; i < SS_ITEMS; ++i)
-        if (i < steps && base + i * 32 < N) e[i] = s_e[base + i * 32];
+        e[i] = i < steps && base + i * 32 < n_left ? s_e[base + i * 32] : make_uint2(R, 0);
   }
 }
 
 __global__ void __launch_bounds__(SS_THREADS) k_sort_small(RowUses u, Digits dg, uint2* __restrict__ sorted,
-                                                           char* __restrict__ clear, size_t bytes) {
+                                                           unsigned* __restrict__ n_used, char* __restrict__ clear,
+                                                           size_t bytes, float* __restrict__ gweight) {
   if (blockIdx.x == 0) {
-    sort_small(u, dg, sorted);
+    sort_small(u, dg, sorted, n_used, gweight);
     return;
   }
   // whole 16-byte words first, then the bytes around them
@@ -316,28 +350,30 @@ static long long tiles_of(long long N) { return (N + TILE - 1) / TILE; }
 size_t sort_space(long long N, long long R, void* base, SortSpace* s) {
   char* p = static_cast<char*>(base);
   SortSpace t;
+  t.n = reinterpret_cast<unsigned*>(p);
+  p += 256;
   t.sorted = reinterpret_cast<uint2*>(p);
   p += align256((size_t)N * sizeof(uint2));
   t.other = nullptr;
-  t.zeroed = nullptr;
-  t.zeroed_bytes = 0;
+  t.counts = nullptr;
+  t.totals = nullptr;
   t.used = nullptr;
   if (N > SORT_SMALL) {
     const Digits dg = digits_for(R, MAX_BITS);
     t.other = reinterpret_cast<uint2*>(p);
     p += align256((size_t)N * sizeof(uint2));
-    t.zeroed = p;
-    p += align256((size_t)(MAX_PASSES + (size_t)dg.passes * (1 << dg.bits)) * sizeof(unsigned));
-    p += align256((size_t)dg.passes * tiles_of(N) * (1 << dg.bits) * sizeof(unsigned));
+    t.counts = reinterpret_cast<unsigned*>(p);
+    p += align256((size_t)tiles_of(N) * (1 << dg.bits) * sizeof(unsigned));
+    t.totals = reinterpret_cast<unsigned*>(p);
+    p += align256((size_t)MAX_DIGITS * sizeof(unsigned));
     t.used = reinterpret_cast<uint8_t*>(p);
     p += align256((size_t)R);
-    t.zeroed_bytes = (size_t)(p - t.zeroed);
   }
   if (s) *s = t;
   return (size_t)(p - static_cast<char*>(base));
 }
 
-int sort_uses(const RowUses& u, const SortSpace& s, void* clear, size_t clear_bytes, cudaStream_t st) {
+int sort_uses(const RowUses& u, const SortSpace& s, void* clear, size_t clear_bytes, float* gweight, cudaStream_t st) {
   if (u.N <= SORT_SMALL) {
     const Digits dg = digits_for(u.R, SS_BITS);
     static std::atomic<unsigned long long> done{0};
@@ -345,25 +381,30 @@ int sort_uses(const RowUses& u, const SortSpace& s, void* clear, size_t clear_by
     const size_t per = (size_t)SS_THREADS * 16 * 8;
     size_t blocks = (clear_bytes + per - 1) / per;
     if (blocks > 148 * 2 - 1) blocks = 148 * 2 - 1;
-    k_sort_small<<<(unsigned)blocks + 1, SS_THREADS, SS_SMEM, st>>>(u, dg, s.sorted, static_cast<char*>(clear), clear_bytes);
+    k_sort_small<<<(unsigned)blocks + 1, SS_THREADS, SS_SMEM, st>>>(u, dg, s.sorted, s.n, static_cast<char*>(clear), clear_bytes,
+                                                                    gweight);
     return check_launch("sort of the uses");
   }
   const Digits dg = digits_for(u.R, MAX_BITS);
-  const long long tiles = tiles_of(u.N);
+  const unsigned tiles = (unsigned)tiles_of(u.N);
   const int D = 1 << dg.bits;
-  if (cudaMemsetAsync(s.zeroed, 0, s.zeroed_bytes, st) != cudaSuccess) return check_launch("memset of the sort's state");
-  unsigned* tickets = reinterpret_cast<unsigned*>(s.zeroed);
-  unsigned* counts = tickets + MAX_PASSES;
-  unsigned* states = reinterpret_cast<unsigned*>(s.zeroed + align256((size_t)(MAX_PASSES + (size_t)dg.passes * D) * sizeof(unsigned)));
-  long long blocks = (u.N + DT - 1) / DT;
-  if (blocks > 148) blocks = 148;
-  k_sort_digits<<<(unsigned)blocks, DT, 0, st>>>(u, dg, counts);
   for (int p = 0; p < dg.passes; ++p) {
     // the last pass writes `sorted`, the ones before alternate so that none reads what it writes
     const bool to_sorted = (dg.passes - 1 - p) % 2 == 0;
-    const uint2* src = p == 0 ? nullptr : (to_sorted ? s.other : s.sorted);
-    k_sort_pass<<<(unsigned)tiles, ST, 0, st>>>(u, src, dg, p, counts + p * D, tickets + p, states + (size_t)p * tiles * D,
-                                                to_sorted ? s.sorted : s.other);
+    const PassIn in{u, p == 0 ? nullptr : (to_sorted ? s.other : s.sorted), s.n, dg.shift(p)};
+    uint2* dst = to_sorted ? s.sorted : s.other;
+    k_sort_count<<<tiles, ST, 0, st>>>(in, D, s.counts, p == 0 ? s.used : nullptr, p == 0 ? gweight : nullptr);
+    k_sort_scan<<<D / 32, 32 * SCAN_WARPS, 0, st>>>(s.counts, tiles, D, s.totals);
+    const auto move = [&](auto bits) {
+      k_sort_move<decltype(bits)::value><<<tiles, ST, 0, st>>>(in, s.counts, s.totals, p == 0 ? s.n : nullptr, dst);
+    };
+    switch (dg.bits) {
+      case 6: move(std::integral_constant<int, 6>()); break;
+      case 7: move(std::integral_constant<int, 7>()); break;
+      case 8: move(std::integral_constant<int, 8>()); break;
+      case 9: move(std::integral_constant<int, 9>()); break;
+      default: move(std::integral_constant<int, 10>()); break;
+    }
   }
   return check_launch("sort of the uses");
 }

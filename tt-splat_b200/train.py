@@ -37,7 +37,6 @@ STATUS_BITS = {
     4: "a peer-exchange wait timed out (a rank's gradient or update never arrived; the waiting "
        "blocks skipped their part of the update)",
     8: "a cached binning table spreads a gaussian over more tiles than its stencil box",
-    16: "a wait of the row gradient's sort timed out (gradients of looked-up rows are wrong)",
 }
 
 
