@@ -10,58 +10,60 @@
 
 namespace tts {
 
+// A block copies whole rows (or a part of one long row): the rows' addresses and factors go through shared
+// memory once, then the block's output is one run of units, spread evenly over its threads whatever the row
+// width, 4 loads of a thread in flight.  Unit e of the run lies in row e / units: the quotient by
+// multiplication, (e * magic) >> 32 with magic = ceil(2^32 / units), exact for e and units up to 2^16.  (A
+// group of lanes for each row, without shared memory or division, took 61 instead of XX us for 320000 rows of
+// 45 fp32: the indices of its rows are waited for by every lane.)
 constexpr int GATHER_THREADS = 256;
 constexpr int GATHER_UNITS = 2048;      // units of a block: 8 a thread
 
-// A block copies whole rows (or a part of one long row): the rows' places and factors go through shared
-// memory once, then the block's output is one run of units, 8 a thread, 4 loads in flight.  Unit e of the run
-// lies in row e / units: the quotient by multiplication, (e * magic) >> 32 with magic = ceil(2^32 / units),
-// exact for e, units <= 2^16.
 template <class T, int VB>
-__global__ void __launch_bounds__(GATHER_THREADS) k_gather_rows(RowUses u, const T* __restrict__ table, long long stride,
-                                                                long long units, int rows, unsigned long long magic,
-                                                                T* __restrict__ out) {
+__global__ void __launch_bounds__(GATHER_THREADS, 8) k_gather_rows(RowUses u, const T* __restrict__ table, long long stride,
+                                                                   long long units, int rows, unsigned magic,
+                                                                   T* __restrict__ out) {
   using U = Unit<T, VB>;
   using W = typename U::W;
-  __shared__ long long s_row[GATHER_THREADS];
+  __shared__ const W* s_row[GATHER_THREADS];
   __shared__ float s_f[GATHER_THREADS];
-  const long long n0 = (long long)blockIdx.x * rows;
+  const long long n0 = (long long)blockIdx.x * rows, part = (long long)blockIdx.y * GATHER_UNITS;
   const int n = (int)(u.N - n0 < rows ? u.N - n0 : rows);
   if (threadIdx.x < n) {
     const long long v = row_of(u, n0 + threadIdx.x);
-    s_row[threadIdx.x] = v >= u.R ? -2 : v;
-    s_f[threadIdx.x] = v >= 0 ? factor_of(u, n0 + threadIdx.x) : 0.f;
+    const float f = factor_of(u, n0 + threadIdx.x);
+    const bool in = v >= 0 && v < u.R;
+    s_row[threadIdx.x] = in ? reinterpret_cast<const W*>(table + v * stride) + part : nullptr;
+    s_f[threadIdx.x] = in ? f : (v < 0 ? 0.f : __int_as_float(0x7fc00000));
   }
   __syncthreads();
-  const long long part = (long long)blockIdx.y * GATHER_UNITS;      // of a row longer than a block's share
-  const int width = (int)(units - part < GATHER_UNITS ? units - part : GATHER_UNITS);
-  const int total = rows == 1 ? width : n * (int)units;
+  const unsigned w = rows == 1 ? (unsigned)(units - part < GATHER_UNITS ? units - part : GATHER_UNITS) : (unsigned)units;
+  const unsigned total = n * w;
   W* dst = reinterpret_cast<W*>(out) + n0 * units + part;
   constexpr int UN = 4;
-  for (int e0 = threadIdx.x; e0 < total; e0 += UN * GATHER_THREADS) {
+  for (unsigned e0 = threadIdx.x; e0 < total; e0 += UN * GATHER_THREADS) {
     U x[UN];
     float f[UN];
 #pragma unroll
     for (int i = 0; i < UN; ++i) {
-      const int e = e0 + i * GATHER_THREADS;
-      f[i] = 0.f;
+      const unsigned e = e0 + i * GATHER_THREADS;
       if (e < total) {
-        const int r = rows == 1 ? 0 : (int)((e * magic) >> 32);
-        const long long v = s_row[r];
-        f[i] = v == -2 ? __int_as_float(0x7fc00000) : s_f[r];
-        if (v >= 0)
-          x[i].w = __ldg(reinterpret_cast<const W*>(table + v * stride) + part + (rows == 1 ? e : e - r * (int)units));
-        else
-#pragma unroll
-          for (int k = 0; k < U::E; ++k) x[i].t[k] = from_f32<T>(0.f);
+        const unsigned r = rows == 1 ? 0u : (magic ? __umulhi(e, magic) : e);      // (magic 0: one unit a row)
+        const W* src = s_row[r];
+        f[i] = s_f[r];
+        memset(&x[i].w, 0, sizeof(W));
+        if (src) x[i].w = __ldg(src + (e - r * w));
       }
     }
 #pragma unroll
     for (int i = 0; i < UN; ++i) {
-      const int e = e0 + i * GATHER_THREADS;
+      const unsigned e = e0 + i * GATHER_THREADS;
       if (e < total) {
+        float v[U::E];
+        x[i].get(v);
 #pragma unroll
-        for (int k = 0; k < U::E; ++k) x[i].t[k] = from_f32<T>(f[i] * to_f32(x[i].t[k]));
+        for (int k = 0; k < U::E; ++k) v[k] *= f[i];
+        x[i].set(v);
         dst[e] = x[i].w;
       }
     }
@@ -85,11 +87,11 @@ __global__ void __launch_bounds__(256) k_weight_grad(RowUses u, const T* __restr
     const W* b = reinterpret_cast<const W*>(table + v * stride);
 #pragma unroll 4
     for (long long i = lane; i < units; i += 32) {
-      U x, y;
-      x.w = __ldg(a + i);
-      y.w = __ldg(b + i);
+      float x[U::E], y[U::E];
+      U(__ldg(a + i)).get(x);
+      U(__ldg(b + i)).get(y);
 #pragma unroll
-      for (int k = 0; k < U::E; ++k) acc = fmaf(to_f32(x.t[k]), to_f32(y.t[k]), acc);
+      for (int k = 0; k < U::E; ++k) acc = fmaf(x[k], y[k], acc);
     }
   }
 #pragma unroll
@@ -122,7 +124,7 @@ extern "C" int tts_gather_rows(const void* table, long long R, long long C, long
   const long long units = C * (long long)elem(type) / vb;
   long long rows = GATHER_UNITS / units;
   rows = rows < 1 ? 1 : (rows > GATHER_THREADS ? GATHER_THREADS : rows);
-  const unsigned long long magic = ((1ull << 32) + units - 1) / units;
+  const unsigned magic = units == 1 ? 0u : (unsigned)(((1ull << 32) + units - 1) / units);
   const dim3 grid((unsigned)((N + rows - 1) / rows), (unsigned)((units + GATHER_UNITS - 1) / GATHER_UNITS));
   return with_unit(type, vb, [&](auto t, auto b) {
     using T = decltype(t);

@@ -20,36 +20,15 @@ struct RowUses {
 
 // The row that use n looks up: -1 for an unused slot, R for one out of range.
 __device__ __forceinline__ long long row_of(const RowUses& u, long long n) {
-  if (u.valid && !__ldg(u.valid + n)) return -1;
   const long long v = load_index(u.idx, u.idx64, n);
-  return v < 0 ? -1 : (v < u.R ? v : u.R);
+  const bool ok = !u.valid || __ldg(u.valid + n);      // both on their way before either is looked at
+  return !ok || v < 0 ? -1 : (v < u.R ? v : u.R);
 }
 __device__ __forceinline__ float factor_of(const RowUses& u, long long n) {
   return u.weight ? u.scale * __ldg(u.weight + n) : u.scale;
 }
 
-// Memory units of VB bytes (16, 4 or 2) holding VB / sizeof(T) elements: rows are read and written in the
-// largest unit that divides their size, their distance and their address.
-template <int VB>
-struct UnitWord;
-template <>
-struct UnitWord<16> { using type = uint4; };
-template <>
-struct UnitWord<4> { using type = unsigned; };
-template <>
-struct UnitWord<2> { using type = unsigned short; };
-
-template <class T, int VB>
-struct Unit {
-  static constexpr int E = VB / (int)sizeof(T);
-  using W = typename UnitWord<VB>::type;
-  union {
-    W w;
-    T t[E];
-  };
-  __device__ __forceinline__ Unit() {}
-};
-
+// Rows are read and written in the largest unit that divides their size, their distance and their address.
 template <class T>
 inline int unit_bytes(std::initializer_list<const void*> ptrs, std::initializer_list<long long> sizes) {
   unsigned long long bits = 0;

@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(GT, GW && PL * VB <= 8 ? 3 : 1) k_rows_grad(Gr
   const unsigned gstep = (unsigned)(a.gout_stride * sizeof(T)), tstep = (unsigned)(a.table_stride * sizeof(T));
   constexpr unsigned NOTHING = 0xffffffffu;
   unsigned cur = NOTHING;
-  float acc[PL * E], row[GW ? PL * E : 1];
+  float acc[PL][E], row[GW ? PL : 1][E];
   auto flush = [&](bool split) {
     const bool open = c.open && cur == c.first;
     if (open || split) {
@@ -165,15 +165,14 @@ __global__ void __launch_bounds__(GT, GW && PL * VB <= 8 ? 3 : 1) k_rows_grad(Gr
       for (int k = 0; k < PL; ++k)
         if (col[k])
 #pragma unroll
-          for (int e = 0; e < E; ++e) p[k * a.lanes * E + e] = acc[k * E + e];
+          for (int e = 0; e < E; ++e) p[k * a.lanes * E + e] = acc[k][e];
     } else {
       W* g = reinterpret_cast<W*>(gtable + (long long)cur * a.C) + u0;
 #pragma unroll
       for (int k = 0; k < PL; ++k)
         if (col[k]) {
           U x;
-#pragma unroll
-          for (int e = 0; e < E; ++e) x.t[e] = from_f32<T>(acc[k * E + e]);
+          x.set(acc[k]);
           g[k * a.lanes] = x.w;
         }
     }
@@ -207,23 +206,25 @@ __global__ void __launch_bounds__(GT, GW && PL * VB <= 8 ? 3 : 1) k_rows_grad(Gr
           if (cur != NOTHING) flush(false);
           cur = key[q];
 #pragma unroll
-          for (int k = 0; k < PL * E; ++k) acc[k] = 0.f;
+          for (int k = 0; k < PL; ++k)
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[k][e] = 0.f;
           if constexpr (GW)
 #pragma unroll
-            for (int k = 0; k < PL; ++k)
-#pragma unroll
-              for (int e = 0; e < E; ++e) row[k * E + e] = to_f32(t[q][k].t[e]);
+            for (int k = 0; k < PL; ++k) t[q][k].get(row[k]);
         }
         const float f = s_f[j + q];
 #pragma unroll
-        for (int k = 0; k < PL; ++k)
+        for (int k = 0; k < PL; ++k) {
+          float x[E];
+          g[q][k].get(x);
 #pragma unroll
           for (int e = 0; e < E; ++e) {
-            const float x = to_f32(g[q][k].t[e]);
-            acc[k * E + e] = fmaf(f, x, acc[k * E + e]);
+            acc[k][e] = fmaf(f, x[e], acc[k][e]);
             if constexpr (GW)
-              if (col[k]) dot[q] = fmaf(x, row[k * E + e], dot[q]);
+              if (col[k]) dot[q] = fmaf(x[e], row[k][e], dot[q]);
           }
+        }
       }
     }
     if constexpr (GW) {
