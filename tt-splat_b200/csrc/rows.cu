@@ -70,6 +70,86 @@ __global__ void __launch_bounds__(GATHER_THREADS, 8) k_gather_rows(RowUses u, co
   }
 }
 
+// Many rows that are no whole number of 16-byte units (320000 rows of 45 fp32: 19.5 us, 24 by the kernel above,
+// which takes few rows and long ones): a thread reads the units of 16 consecutive output bytes,
+// which may lie in two rows or more, and stores them at once.  A block's rows are a multiple of 16 / SB, so
+// its output starts on a 16-byte boundary.
+template <class T, int SB>
+__global__ void __launch_bounds__(GATHER_THREADS) k_gather_packed(RowUses u, const T* __restrict__ table, long long stride,
+                                                                  unsigned units, int rows, unsigned magic,
+                                                                  T* __restrict__ out) {
+  using U = Unit<T, SB>;
+  using W = typename U::W;
+  constexpr int NU = 16 / SB, UN = 2;
+  __shared__ const W* s_row[GATHER_THREADS];
+  __shared__ float s_f[GATHER_THREADS];
+  const long long n0 = (long long)blockIdx.x * rows;
+  const int n = (int)(u.N - n0 < rows ? u.N - n0 : rows);
+  if (threadIdx.x < n) {
+    const long long v = row_of(u, n0 + threadIdx.x);
+    const float f = factor_of(u, n0 + threadIdx.x);
+    const bool in = v >= 0 && v < u.R;
+    s_row[threadIdx.x] = in ? reinterpret_cast<const W*>(table + v * stride) : nullptr;
+    s_f[threadIdx.x] = in ? f : (v < 0 ? 0.f : __int_as_float(0x7fc00000));
+  }
+  __syncthreads();
+  const unsigned total = n * units, whole = total / NU;
+  char* dst = reinterpret_cast<char*>(out) + n0 * units * SB;
+  for (unsigned q0 = threadIdx.x; q0 < whole; q0 += UN * GATHER_THREADS) {
+    U x[UN][NU];
+    float f[UN][NU];
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      const unsigned q = q0 + i * GATHER_THREADS;
+      if (q < whole) {
+        unsigned r = magic ? __umulhi(q * NU, magic) : q * NU, c = q * NU - r * units;
+        const W* src = s_row[r];
+        float g = s_f[r];
+#pragma unroll
+        for (int k = 0; k < NU; ++k) {
+          f[i][k] = g;
+          x[i][k].w = src ? __ldg(src + c) : W(0);
+          if (++c == units && k + 1 < NU) {
+            c = 0;
+            src = s_row[++r];
+            g = s_f[r];
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      const unsigned q = q0 + i * GATHER_THREADS;
+      if (q < whole) {
+        W y[NU];
+#pragma unroll
+        for (int k = 0; k < NU; ++k) {
+          float v[U::E];
+          x[i][k].get(v);
+#pragma unroll
+          for (int e = 0; e < U::E; ++e) v[e] *= f[i][k];
+          x[i][k].set(v);
+          y[k] = x[i][k].w;
+        }
+        uint4 z;
+        memcpy(&z, y, 16);
+        *reinterpret_cast<uint4*>(dst + (long long)q * 16) = z;
+      }
+    }
+  }
+  if (threadIdx.x < total - whole * NU) {
+    const unsigned e = whole * NU + threadIdx.x, r = magic ? __umulhi(e, magic) : e;
+    U x;
+    x.w = s_row[r] ? __ldg(s_row[r] + (e - r * units)) : W(0);
+    float v[U::E];
+    x.get(v);
+#pragma unroll
+    for (int k = 0; k < U::E; ++k) v[k] *= s_f[r];
+    x.set(v);
+    reinterpret_cast<W*>(dst)[e] = x.w;
+  }
+}
+
 // Weights' gradients of rows too wide for the sums' registers, or wanted alone: a warp for each use.
 template <class T, int VB>
 __global__ void __launch_bounds__(256) k_weight_grad(RowUses u, const T* __restrict__ table, long long stride, long long units,
@@ -124,6 +204,20 @@ extern "C" int tts_gather_rows(const void* table, long long R, long long C, long
   const long long units = C * (long long)elem(type) / vb;
   long long rows = GATHER_UNITS / units;
   rows = rows < 1 ? 1 : (rows > GATHER_THREADS ? GATHER_THREADS : rows);
+  const int step = 16 / vb;
+  if (vb < 16 && rows >= step && aligned16(out) && N * units >= 148ll * 4 * GATHER_UNITS) {
+    rows -= rows % step;
+    const unsigned magic = units == 1 ? 0u : (unsigned)(((1ull << 32) + units - 1) / units);
+    const unsigned blocks = (unsigned)((N + rows - 1) / rows);
+    return with_unit(type, vb, [&](auto t, auto b) {
+      using T = decltype(t);
+      constexpr int VB = decltype(b)::value;
+      if constexpr (VB < 16)
+        k_gather_packed<T, VB><<<blocks, GATHER_THREADS, 0, as_stream(stream)>>>(
+            u, static_cast<const T*>(table), table_stride, (unsigned)units, (int)rows, magic, static_cast<T*>(out));
+      return check_launch("gather_rows");
+    });
+  }
   const unsigned magic = units == 1 ? 0u : (unsigned)(((1ull << 32) + units - 1) / units);
   const dim3 grid((unsigned)((N + rows - 1) / rows), (unsigned)((units + GATHER_UNITS - 1) / GATHER_UNITS));
   return with_unit(type, vb, [&](auto t, auto b) {
