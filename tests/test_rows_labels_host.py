@@ -23,6 +23,8 @@ def test_gather_rows_refusals(pkg):
         binned.gather_rows(table, idx, valid=torch.ones(4, dtype=torch.bool))
     with pytest.raises(TypeError, match="weight"):
         binned.gather_rows(table, idx, weight=torch.ones(5, dtype=torch.float64))
+    with pytest.raises(TypeError, match="scale"):
+        binned.gather_rows(table, idx, scale=torch.ones(()))
     with pytest.raises(ValueError, match="weight"):
         binned.gather_rows(table, idx, weight=torch.ones(5, 1))
 

@@ -145,7 +145,7 @@ _NO_CONTEXT = contextlib.nullcontext()
 def on_device(t):
     """Context selecting a CUDA tensor's device (a no-op where that is the current one already, and for
     anything else: the ops then raise)."""
-    if isinstance(t, torch.Tensor) and t.is_cuda and t.device.index != torch.cuda.current_device():
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() != torch.cuda.current_device():
         return torch.cuda.device(t.device)
     return _NO_CONTEXT
 

@@ -126,6 +126,8 @@ def gather_rows(table, idx, valid=None, weight=None, scale=1.0):
     a leaf's gradient to the stream of the graph that is still alive, and the capture fails."""
     if table.dim() < 1:
         raise ValueError("table must have at least one dimension")
+    if isinstance(scale, torch.Tensor):
+        raise TypeError("scale must be a number (a factor that is learned goes into weight or the table)")
     ops.row_type(table, "table")
     ops.index_type(idx, "idx")
     shape, row_shape = idx.shape, tuple(table.shape[1:])

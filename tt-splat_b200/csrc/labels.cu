@@ -59,12 +59,15 @@ struct Soft {
     S += e;
     A = fmaf(e, d, A);
   }
-  __device__ __forceinline__ void merge(Soft o) {
-    const float m2 = max_nan(m, o.m);
+  // Over lanes that differ in the bits below `width` (a power of two).
+  __device__ __forceinline__ void reduce(int width) {
+    float m2 = m;
+    for (int d = width / 2; d > 0; d >>= 1) m2 = max_nan(m2, __shfl_xor_sync(0xffffffffu, m2, d));
     rebase(m2);
-    o.rebase(m2);
-    S += o.S;
-    A += o.A;
+    for (int d = width / 2; d > 0; d >>= 1) {
+      S += __shfl_xor_sync(0xffffffffu, S, d);
+      A += __shfl_xor_sync(0xffffffffu, A, d);
+    }
   }
   __device__ __forceinline__ bool bad() const { return !(m < CUDART_INF_F); }
 };
@@ -82,11 +85,10 @@ struct ScoreArgs {
 
 // A row's results but the alternatives; x is the row (global or shared memory).
 template <class T>
-__device__ __forceinline__ float2 write_scores(const ScoreArgs& a, long long r, const Soft& s, const T* x) {
+__device__ __forceinline__ float2 write_scores(const ScoreArgs& a, long long r, const Soft& s, const T* x, long long t) {
   const bool bad = s.bad(), empty = !bad && s.S == 0.f;
   const float nan = CUDART_NAN_F;
   const float m = bad ? nan : (empty ? 0.f : s.m), logS = bad ? nan : (empty ? -CUDART_INF_F : logf(s.S));
-  const long long t = load_index(a.labels, a.labels64, r);
   float lp = 0.f;
   if (t >= a.C)
     lp = nan;
@@ -104,36 +106,9 @@ __device__ __forceinline__ void write_top(const ScoreArgs& a, long long r, int k
   a.top_logp[r * a.top + k] = st.y != st.y ? CUDART_NAN_F : (id < 0 ? -CUDART_INF_F : (v - st.x) - st.y);
 }
 
-// ---- vectors of 16 bytes -----------------------------------------------------------------------
+// ---- many labels: rows in units of 16 bytes --------------------------------------------------------
 template <class T>
-struct Vec16 {
-  static constexpr int N = 16 / sizeof(T);
-  uint4 w;
-  __device__ __forceinline__ float get(int i) const {
-    if constexpr (sizeof(T) == 4) {
-      return __uint_as_float(i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w);
-    } else {
-      const unsigned p = i < 2 ? w.x : i < 4 ? w.y : i < 6 ? w.z : w.w;
-      const unsigned short h = (unsigned short)((i & 1) ? p >> 16 : p & 0xffffu);
-      T t;
-      memcpy(&t, &h, 2);
-      return to_f32(t);
-    }
-  }
-  __device__ __forceinline__ void set(int i, float f) {
-    const T t = from_f32<T>(f);
-    unsigned& p = sizeof(T) == 4 ? (i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w)
-                                 : (i < 2 ? w.x : i < 4 ? w.y : i < 6 ? w.z : w.w);
-    if constexpr (sizeof(T) == 4) {
-      p = __float_as_uint(f);
-    } else {
-      unsigned short h;
-      memcpy(&h, &t, 2);
-      p = (i & 1) ? (p & 0xffffu) | ((unsigned)h << 16) : (p & 0xffff0000u) | h;
-    }
-  }
-};
-
+using Vec16 = Unit<T, 16>;
 // A row of C elements as `head` single ones up to the first 16-byte boundary, nv vectors and a tail.
 template <class T>
 struct RowSplit {
@@ -143,8 +118,8 @@ struct RowSplit {
     const int off = (int)(reinterpret_cast<uintptr_t>(x) & 15u);
     const long long h = off ? (16 - off) / (int)sizeof(T) : 0;
     head = (int)(h < C ? h : C);
-    nv = (C - head) / Vec16<T>::N;
-    tail = (int)(C - head - nv * Vec16<T>::N);
+    nv = (C - head) / Vec16<T>::E;
+    tail = (int)(C - head - nv * Vec16<T>::E);
   }
 };
 
@@ -172,7 +147,7 @@ __device__ __forceinline__ bool before(float v, long long id, float w, long long
 template <class T>
 __device__ void block_top(const T* x, const RowSplit<T>& rs, long long lo, long long hi, bool ends, float tmax, int top,
                           BlockTop* out) {
-  constexpr int N = Vec16<T>::N;
+  constexpr int N = Vec16<T>::E;
   __shared__ float s_g[32];
   __shared__ float s_T;
   __shared__ int s_nq, s_nc;
@@ -213,9 +188,10 @@ __device__ void block_top(const T* x, const RowSplit<T>& rs, long long lo, long 
     const int q = (int)(p / rounds);
     const long long v = lo + s_q[q] + (p - (long long)q * rounds) * SB_THREADS;
     if (v >= hi) continue;
-    const Vec16<T> w{__ldg(xv + v)};
+    float w[N];
+    Vec16<T>(__ldg(xv + v)).get(w);
 #pragma unroll
-    for (int e = 0; e < N; ++e) consider(w.get(e), rs.head + v * N + e);
+    for (int e = 0; e < N; ++e) consider(w[e], rs.head + v * N + e);
   }
   const long long t0 = rs.head + rs.nv * N;
   if (ends && tid < rs.head) consider(to_f32(x[tid]), tid);
@@ -248,9 +224,10 @@ __device__ void block_top(const T* x, const RowSplit<T>& rs, long long lo, long 
     };
     if (ends && tid < rs.head) look(to_f32(x[tid]), tid);
     for (long long v = lo + tid; v < hi; v += SB_THREADS) {
-      const Vec16<T> w{__ldg(xv + v)};
+      float w[N];
+      Vec16<T>(__ldg(xv + v)).get(w);
 #pragma unroll
-      for (int e = 0; e < N; ++e) look(w.get(e), rs.head + v * N + e);
+      for (int e = 0; e < N; ++e) look(w[e], rs.head + v * N + e);
     }
     if (ends && tid < rs.tail) look(to_f32(x[t0 + tid]), t0 + tid);
 #pragma unroll
@@ -278,12 +255,14 @@ __device__ void block_top(const T* x, const RowSplit<T>& rs, long long lo, long 
 // one merge; the blocks of a cluster take a part of the row each and the first one merges theirs through
 // distributed shared memory.
 template <class T>
-__global__ void __launch_bounds__(SB_THREADS) k_scores_block(const T* __restrict__ logits, long long stride, int cs,
-                                                             ScoreArgs a) {
-  constexpr int N = Vec16<T>::N, UNROLL = 4;
-  __shared__ Soft s_soft[SB_THREADS / 32];
+__global__ void __launch_bounds__(SB_THREADS, 4) k_scores_block(const T* __restrict__ logits, long long stride, int cs,
+                                                                ScoreArgs a) {
+  constexpr int N = Vec16<T>::E, UNROLL = 4;
+  constexpr int WARPS = SB_THREADS / 32;
+  __shared__ Soft s_soft[WARPS > SB_CLUSTER ? WARPS : SB_CLUSTER];
   __shared__ Soft s_all;
   __shared__ BlockTop s_top;
+  __shared__ BlockTop s_tops[SB_CLUSTER];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const long long r = blockIdx.x / cs;
   const int rank = blockIdx.x % cs;
@@ -291,6 +270,7 @@ __global__ void __launch_bounds__(SB_THREADS) k_scores_block(const T* __restrict
   const RowSplit<T> rs(x, a.C);
   const long long lo = rs.nv * rank / cs, hi = rs.nv * (rank + 1) / cs;
   const uint4* xv = reinterpret_cast<const uint4*>(x + rs.head);
+  const long long label = load_index(a.labels, a.labels64, r);
   Soft s;
   s.init();
   if (rank == 0) {
@@ -312,78 +292,79 @@ __global__ void __launch_bounds__(SB_THREADS) k_scores_block(const T* __restrict
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
       if (v0 + u * SB_THREADS < hi) {
+        float f[N];
+        w[u].get(f);
 #pragma unroll
-        for (int e = 0; e < N; ++e) m = max_nan(m, w[u].get(e));
+        for (int e = 0; e < N; ++e) m = max_nan(m, f[e]);
       }
     if (!(m == s.m)) s.rebase(m);
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
       if (v0 + u * SB_THREADS < hi) {
+        float f[N];
+        w[u].get(f);
 #pragma unroll
-        for (int e = 0; e < N; ++e) s.add(w[u].get(e));
+        for (int e = 0; e < N; ++e) s.add(f[e]);
       }
   }
   const float tmax = s.m;
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    Soft o;
-    o.m = __shfl_xor_sync(0xffffffffu, s.m, d);
-    o.S = __shfl_xor_sync(0xffffffffu, s.S, d);
-    o.A = __shfl_xor_sync(0xffffffffu, s.A, d);
-    s.merge(o);
-  }
+  s.reduce(32);
   if (lane == 0) s_soft[wid] = s;
+  if (tid == 0) s_top.n = 0;
   __syncthreads();
-  s = s_soft[0];
-#pragma unroll
-  for (int w = 1; w < SB_THREADS / 32; ++w) s.merge(s_soft[w]);
-  if (tid == 0) {
-    s_all = s;
-    s_top.n = 0;
-  }
-  __syncthreads();
+  s = s_soft[lane % WARPS];
+  s.reduce(WARPS);
+  if (tid == 0) s_all = s;
   if (a.top > 0 && !s.bad()) block_top<T>(x, rs, lo, hi, rank == 0, tmax, a.top, &s_top);
   if (cs == 1) {
-    float2 st;
     if (tid == 0) {
-      s_all = s;
-      st = write_scores(a, r, s, x);
-      s_soft[0].m = st.x, s_soft[0].S = st.y;
+      const float2 st = write_scores(a, r, s, x, label);
+      s_all.m = st.x, s_all.S = st.y;
     }
     if (a.top > 0) {
       __syncthreads();
       if (tid < a.top)
-        write_top(a, r, tid, s_top.v[tid], tid < s_top.n ? s_top.id[tid] : -1, make_float2(s_soft[0].m, s_soft[0].S));
+        write_top(a, r, tid, s_top.v[tid], tid < s_top.n ? s_top.id[tid] : -1, make_float2(s_all.m, s_all.S));
     }
     return;
   }
   cg::cluster_group cluster = cg::this_cluster();
   cluster.sync();
-  if (rank == 0 && wid == 0) {
-    Soft all = s;
-    for (int b = 1; b < cs; ++b) all.merge(*cluster.map_shared_rank(&s_all, b));
-    float2 st;
-    if (lane == 0) st = write_scores(a, r, all, x);
-    st.x = __shfl_sync(0xffffffffu, st.x, 0);
-    st.y = __shfl_sync(0xffffffffu, st.y, 0);
-    const BlockTop* mine = lane < cs ? cluster.map_shared_rank(&s_top, lane) : &s_top;
-    const int n = lane < cs && !all.bad() ? mine->n : 0;
-    int at = 0;
-    for (int k = 0; k < a.top; ++k) {
-      float bv = at < n ? mine->v[at] : -CUDART_INF_F;
-      long long bi = at < n ? mine->id[at] : -1;
-      const long long own = bi;
-#pragma unroll
-      for (int d = SB_CLUSTER / 2; d > 0; d >>= 1) {
-        const float ov = __shfl_xor_sync(0xffffffffu, bv, d);
-        const long long oi = __shfl_xor_sync(0xffffffffu, bi, d);
-        if (oi >= 0 && (bi < 0 || before(ov, oi, bv, bi))) bv = ov, bi = oi;
+  if (rank == 0) {
+    // every block's part here, then the best of all their bests by counting how many come before each
+    if (wid == 0) {
+      Soft o;
+      o.init();
+      if (lane < cs) o = *cluster.map_shared_rank(&s_all, lane);
+      o.reduce(32);
+      if (lane == 0) {
+        const float2 st = write_scores(a, r, o, x, label);
+        s_soft[0].m = st.x, s_soft[0].S = st.y;
       }
-      bv = __shfl_sync(0xffffffffu, bv, 0);
-      bi = __shfl_sync(0xffffffffu, bi, 0);
-      if (bi >= 0 && own == bi) ++at;
-      if (lane == 0) write_top(a, r, k, bv, bi, st);
     }
+    const int b = tid / TOP_MAX, k = tid % TOP_MAX;
+    if (a.top > 0 && b < cs) {
+      const BlockTop* t = cluster.map_shared_rank(&s_top, b);
+      const int n = t->n;
+      s_tops[b].v[k] = k < n ? t->v[k] : -CUDART_INF_F;
+      s_tops[b].id[k] = k < n ? t->id[k] : -1;
+      if (k == 0) s_tops[b].n = n;
+    }
+    __syncthreads();
+    const float2 st = make_float2(s_soft[0].m, s_soft[0].S);
+    int all = 0;
+    if (a.top > 0 && st.y == st.y)
+      for (int q = 0; q < cs; ++q) all += s_tops[q].n;
+    if (a.top > 0 && b < cs && k < s_tops[b].n && st.y == st.y) {
+      const float v = s_tops[b].v[k];
+      const long long id = s_tops[b].id[k];
+      int place = k;
+      for (int q = 0; q < cs; ++q)
+        if (q != b)
+          for (int i = 0; i < s_tops[q].n; ++i) place += before(s_tops[q].v[i], s_tops[q].id[i], v, id);
+      if (place < a.top) write_top(a, r, place, v, id, st);
+    }
+    if (tid < a.top && tid >= all) write_top(a, r, tid, -CUDART_INF_F, -1, st);
   }
   cluster.sync();
 }
@@ -394,24 +375,43 @@ __global__ void __launch_bounds__(SB_THREADS) k_scores_block(const T* __restrict
 // then owns a row and nothing is shuffled.  Threads walk their rows in 4-byte words (two 16-bit logits) where
 // rows are whole words; with an even number of words to a row each thread starts one word further, so that
 // the warp's accesses fall into different banks.
+template <bool TURN>
 struct TileWalk {
   int n, at;        // units of a row; the next one
-  __device__ __forceinline__ TileWalk(int n_) : n(n_), at((n_ & 1) ? 0 : (int)threadIdx.x % n_) {}
-  __device__ __forceinline__ int next() {
+  __device__ __forceinline__ TileWalk(int n_) : n(n_), at(TURN ? (int)threadIdx.x % n_ : 0) {}
+  __device__ __forceinline__ int next(int i) {
+    if (!TURN) return i;
     const int j = at;
     at = at + 1 == n ? 0 : at + 1;
     return j;
   }
 };
 
-template <class T, int VB>
-struct TileUnit {
-  static constexpr int E = VB / (int)sizeof(T);
-  union {
-    typename std::conditional<VB == 4, unsigned, unsigned short>::type w;
-    T t[E];
-  };
-  __device__ __forceinline__ TileUnit() {}
+// The best few labels of a row in registers, best first.
+template <int K>
+struct Best {
+  float v[K];
+  int id[K];
+  __device__ __forceinline__ void init() {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = -CUDART_INF_F, id[k] = -1;
+  }
+  // (a masked label never comes before the -inf of an empty place)
+  __device__ __forceinline__ void add(float x, int j) {
+    if (!(x > v[K - 1] || (x == v[K - 1] && j < id[K - 1]))) return;
+#pragma unroll
+    for (int k = K - 1; k >= 0; --k) {
+      const bool here = x > v[k] || (x == v[k] && j < id[k]);
+      const bool above = k > 0 && (x > v[k > 0 ? k - 1 : 0] || (x == v[k > 0 ? k - 1 : 0] && j < id[k > 0 ? k - 1 : 0]));
+      if (above) {
+        v[k] = v[k > 0 ? k - 1 : 0];
+        id[k] = id[k > 0 ? k - 1 : 0];
+      } else if (here) {
+        v[k] = x;
+        id[k] = j;
+      }
+    }
+  }
 };
 
 // Copies rows [r0, r0 + n) into s (16-byte pieces by the bulk copy, the few bytes behind them by threads);
@@ -431,36 +431,52 @@ __device__ __forceinline__ bool load_tile(const T* logits, long long first, int 
   return whole == 0 || mbar_wait_bounded(bar, 0);
 }
 
-template <class T, int VB>
+constexpr int TILE_BEST = 4;      // alternatives kept in registers
+
+template <class T, int VB, bool TURN, bool FEW>
 __global__ void __launch_bounds__(128) k_scores_tile(const T* __restrict__ logits, long long P, ScoreArgs a) {
-  using U = TileUnit<T, VB>;
+  using U = Unit<T, VB>;
   extern __shared__ __align__(16) char smem[];
   __shared__ __align__(8) uint64_t bar;
   const int C = (int)a.C, units = C / U::E;
   const long long r0 = (long long)blockIdx.x * blockDim.x;
   const int rows = (int)(P - r0 < blockDim.x ? P - r0 : blockDim.x);
   T* s = reinterpret_cast<T*>(smem);
+  const long long r = r0 + threadIdx.x;
+  const long long label = threadIdx.x < rows ? load_index(a.labels, a.labels64, r) : -1;
   if (!load_tile(logits, r0 * C, rows * C, s, &bar)) return;
   if (threadIdx.x >= rows) return;
   T* x = s + threadIdx.x * C;
-  U* xu = reinterpret_cast<U*>(x);
+  typename U::W* xu = reinterpret_cast<typename U::W*>(x);
   Soft f;
   f.init();
-  TileWalk w(units);
+  Best<TILE_BEST> best;
+  if (FEW) best.init();
+  TileWalk<TURN> w(units);
 #pragma unroll 4
   for (int i = 0; i < units; ++i) {
-    const U u = xu[w.next()];
+    const int j = w.next(i);
+    float v[U::E];
+    U(xu[j]).get(v);
 #pragma unroll
-    for (int e = 0; e < U::E; ++e) f.m = max_nan(f.m, to_f32(u.t[e]));
+    for (int e = 0; e < U::E; ++e) {
+      f.m = max_nan(f.m, v[e]);
+      if (FEW) best.add(v[e], j * U::E + e);
+    }
   }
 #pragma unroll 4
   for (int i = 0; i < units; ++i) {
-    const U u = xu[w.next()];
+    float v[U::E];
+    U(xu[w.next(i)]).get(v);
 #pragma unroll
-    for (int e = 0; e < U::E; ++e) f.add(to_f32(u.t[e]));
+    for (int e = 0; e < U::E; ++e) f.add(v[e]);
   }
-  const long long r = r0 + threadIdx.x;
-  const float2 st = write_scores(a, r, f, x);
+  const float2 st = write_scores(a, r, f, x, label);
+  if constexpr (FEW) {
+#pragma unroll
+    for (int k = 0; k < TILE_BEST; ++k)
+      if (k < a.top) write_top(a, r, k, best.v[k], f.bad() ? -1 : best.id[k], st);
+  } else {
   // the best label left, taken out of the tile after each round
   for (int k = 0; k < a.top; ++k) {
     float bv = -CUDART_INF_F;
@@ -468,17 +484,18 @@ __global__ void __launch_bounds__(128) k_scores_tile(const T* __restrict__ logit
     if (!f.bad())
 #pragma unroll 4
       for (int i = 0; i < units; ++i) {
-        const int j = w.next();
-        const U u = xu[j];
+        const int j = w.next(i);
+        float v[U::E];
+        U(xu[j]).get(v);
 #pragma unroll
         for (int e = 0; e < U::E; ++e) {
-          const float v = to_f32(u.t[e]);
           const int id = j * U::E + e;
-          if (v > bv || (v == bv && id < bi)) bv = v, bi = id;
+          if (v[e] > bv || (TURN && v[e] == bv && id < bi)) bv = v[e], bi = id;
         }
       }
     if (bi >= 0) x[bi] = from_f32<T>(-CUDART_INF_F);
     write_top(a, r, k, bv, bi, st);
+  }
   }
 }
 
@@ -503,7 +520,7 @@ __global__ void __launch_bounds__(256) k_scores_warp(const T* __restrict__ logit
     s.A += __shfl_xor_sync(0xffffffffu, s.A, d);
   }
   float2 st;
-  if (lane == 0) st = write_scores(a, r, s, x);
+  if (lane == 0) st = write_scores(a, r, s, x, load_index(a.labels, a.labels64, r));
   st.x = __shfl_sync(0xffffffffu, st.x, 0);
   st.y = __shfl_sync(0xffffffffu, st.y, 0);
   // the k-th best is the best of those behind the (k-1)-th in the order (value down, id up)
@@ -589,7 +606,7 @@ constexpr int GB_UNROLL = 4;
 template <class T, bool SAME>
 __global__ void __launch_bounds__(GB_THREADS) k_scores_grad_block(const T* __restrict__ logits, long long stride, GradArgs a,
                                                                   T* __restrict__ glogits) {
-  constexpr int N = Vec16<T>::N;
+  constexpr int N = Vec16<T>::E;
   const long long r = blockIdx.x;
   const T* x = logits + r * stride;
   T* gx = glogits + r * a.C;
@@ -610,8 +627,10 @@ __global__ void __launch_bounds__(GB_THREADS) k_scores_grad_block(const T* __res
       if constexpr (SAME) {
         w[u].w = __ldcs(xv + v);
       } else {
+        float f[N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) w[u].set(e, to_f32(x[rs.head + v * N + e]));
+        for (int e = 0; e < N; ++e) f[e] = to_f32(x[rs.head + v * N + e]);
+        w[u].set(f);
       }
     }
   }
@@ -619,10 +638,12 @@ __global__ void __launch_bounds__(GB_THREADS) k_scores_grad_block(const T* __res
   for (int u = 0; u < GB_UNROLL; ++u) {
     const long long v = lo + u * GB_THREADS + threadIdx.x;
     if (v < hi) {
-      Vec16<T> o;
+      float f[N];
+      w[u].get(f);
 #pragma unroll
-      for (int e = 0; e < N; ++e) o.set(e, none ? 0.f : g(w[u].get(e)));
-      __stcs(gv + v, o.w);
+      for (int e = 0; e < N; ++e) f[e] = none ? 0.f : g(f[e]);
+      w[u].set(f);
+      __stcs(gv + v, w[u].w);
     }
   }
   if (blockIdx.y == 0 && threadIdx.x < rs.head)
@@ -657,41 +678,55 @@ __global__ void __launch_bounds__(256) k_scores_grad_warp(const T* __restrict__ 
   }
 }
 
-template <class T, int VB>
+template <class T, int VB, bool TURN>
 __global__ void __launch_bounds__(128) k_scores_grad_tile(const T* __restrict__ logits, long long P, GradArgs a,
                                                           T* __restrict__ glogits) {
-  using U = TileUnit<T, VB>;
+  using U = Unit<T, VB>;
   extern __shared__ __align__(16) char smem[];
   __shared__ __align__(8) uint64_t bar;
   const int C = (int)a.C, units = C / U::E;
   const long long r0 = (long long)blockIdx.x * blockDim.x;
   const int rows = (int)(P - r0 < blockDim.x ? P - r0 : blockDim.x);
   T* s = reinterpret_cast<T*>(smem);
+  const long long r = r0 + threadIdx.x;
+  const RowGrad g(a, threadIdx.x < rows ? r : r0);
   if (!load_tile(logits, r0 * C, rows * C, s, &bar)) return;
   if (threadIdx.x < rows) {
-    const long long r = r0 + threadIdx.x;
     T* x = s + threadIdx.x * C;
-    U* xu = reinterpret_cast<U*>(x);
-    const RowGrad g(a, r);
+    typename U::W* xu = reinterpret_cast<typename U::W*>(x);
     const bool none = g.zero || g.empty;
     // the labels with a term of their own, before their logits are overwritten
-    const int extra = 1 + (a.g_top ? a.top : 0);
-    float own[1 + TOP_MAX];
+    const int extra = a.g_top ? a.top : 0;
+    const float at_label = g.t >= 0 && g.t < C ? g.special(a, r, g.t, to_f32(x[g.t])) : 0.f;
+    float own[TOP_MAX];
     for (int k = 0; k < extra; ++k) {
-      const long long j = k == 0 ? g.t : a.top_ids[r * a.top + k - 1];
+      const long long j = a.top_ids[r * a.top + k];
       own[k] = j >= 0 && j < C ? g.special(a, r, j, to_f32(x[j])) : 0.f;
     }
-    TileWalk w(units);
-#pragma unroll 4
-    for (int i = 0; i < units; ++i) {
-      const int j = w.next();
-      U u = xu[j];
+    TileWalk<TURN> w(units);
+    if (none) {
+      U zero;
+      float v[U::E];
 #pragma unroll
-      for (int e = 0; e < U::E; ++e) u.t[e] = from_f32<T>(none ? 0.f : g(to_f32(u.t[e])));
-      xu[j] = u;
+      for (int e = 0; e < U::E; ++e) v[e] = 0.f;
+      zero.set(v);
+      for (int i = 0; i < units; ++i) xu[w.next(i)] = zero.w;
+    } else {
+#pragma unroll 4
+      for (int i = 0; i < units; ++i) {
+        const int j = w.next(i);
+        U u(xu[j]);
+        float v[U::E];
+        u.get(v);
+#pragma unroll
+        for (int e = 0; e < U::E; ++e) v[e] = g(v[e]);
+        u.set(v);
+        xu[j] = u.w;
+      }
     }
+    if (g.t >= 0 && g.t < C) x[g.t] = from_f32<T>(at_label);
     for (int k = 0; k < extra; ++k) {
-      const long long j = k == 0 ? g.t : a.top_ids[r * a.top + k - 1];
+      const long long j = a.top_ids[r * a.top + k];
       if (j >= 0 && j < C) x[j] = from_f32<T>(own[k]);
     }
   }
@@ -707,6 +742,16 @@ __global__ void __launch_bounds__(128) k_scores_grad_tile(const T* __restrict__ 
     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
   }
   for (int i = (int)(whole / sizeof(T)) + threadIdx.x; i < count; i += blockDim.x) glogits[r0 * C + i] = s[i];
+}
+
+// Calls f with the unit size and whether the walk turns, for rows of C elements of T.
+template <class T, class F>
+static int with_tile(long long C, F f) {
+  using B4 = std::integral_constant<int, 4>;
+  using BT = std::integral_constant<int, (int)sizeof(T)>;
+  if (C * sizeof(T) % 8 == 0) return f(B4(), std::true_type());
+  if (C * sizeof(T) % 4 == 0) return f(B4(), std::false_type());
+  return f(BT(), std::false_type());
 }
 
 // Rows of up to TILE_ROW_BYTES that lie one behind the other from a 16-byte boundary on take a thread each.
@@ -766,10 +811,15 @@ extern "C" int tts_label_log_probs(const void* logits, long long P, long long C,
       const int n = tile_threads(C, sizeof(T));
       const size_t bytes = (size_t)n * C * sizeof(T);
       const unsigned grid = (unsigned)((P + n - 1) / n);
-      if (C * sizeof(T) % 4 == 0)
-        k_scores_tile<T, 4><<<grid, n, bytes, as_stream(stream)>>>(x, P, a);
-      else
-        k_scores_tile<T, sizeof(T)><<<grid, n, bytes, as_stream(stream)>>>(x, P, a);
+      with_tile<T>(C, [&](auto vb, auto turn) {
+        constexpr int VB = decltype(vb)::value;
+        constexpr bool TURN = decltype(turn)::value;
+        if (top > 0 && top <= TILE_BEST)
+          k_scores_tile<T, VB, TURN, true><<<grid, n, bytes, as_stream(stream)>>>(x, P, a);
+        else
+          k_scores_tile<T, VB, TURN, false><<<grid, n, bytes, as_stream(stream)>>>(x, P, a);
+        return TTS_OK;
+      });
     } else if (C <= WARP_ROW_MAX) {
       k_scores_warp<T><<<(unsigned)((P + 7) / 8), 256, 0, as_stream(stream)>>>(x, P, row_stride, a);
     } else if (int rc = launch_scores_block<T>(x, P, row_stride, a, as_stream(stream))) {
@@ -798,17 +848,17 @@ extern "C" int tts_label_log_probs_bwd(const void* logits, long long P, long lon
       const int n = tile_threads(C, sizeof(T));
       const size_t bytes = (size_t)n * C * sizeof(T);
       const unsigned grid = (unsigned)((P + n - 1) / n);
-      if (C * sizeof(T) % 4 == 0)
-        k_scores_grad_tile<T, 4><<<grid, n, bytes, st>>>(x, P, a, gx);
-      else
-        k_scores_grad_tile<T, sizeof(T)><<<grid, n, bytes, st>>>(x, P, a, gx);
+      with_tile<T>(C, [&](auto vb, auto turn) {
+        k_scores_grad_tile<T, decltype(vb)::value, decltype(turn)::value><<<grid, n, bytes, st>>>(x, P, a, gx);
+        return TTS_OK;
+      });
     } else if (C <= WARP_ROW_MAX) {
       k_scores_grad_warp<T><<<(unsigned)((P + 7) / 8), 256, 0, st>>>(x, P, row_stride, a, gx);
     } else {
       // the logits' 16-byte vectors line up with the gradient's when both start on the same offset in every row
       const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(gx)) & 15u) == 0 &&
                         (row_stride - C) * (long long)sizeof(T) % 16 == 0;
-      const long long vecs = C / Vec16<T>::N, per = (long long)GB_THREADS * GB_UNROLL;
+      const long long vecs = C / Vec16<T>::E, per = (long long)GB_THREADS * GB_UNROLL;
       const dim3 grid((unsigned)P, (unsigned)((vecs + per - 1) / per));
       if (same)
         k_scores_grad_block<T, true><<<grid, GB_THREADS, 0, st>>>(x, row_stride, a, gx);

@@ -3,6 +3,8 @@
 Shapes follow ``include/ttsplat_b200.h``.  Every function validates that its tensors are CUDA
 and contiguous and raises otherwise (no CPU fallback).
 """
+import functools
+
 import numpy as np
 import torch
 
@@ -373,16 +375,18 @@ def _dev_rows(rows, *flat):
     if not rows.is_cuda:
         raise RuntimeError("tt-splat B200 ops need CUDA tensors (no CPU fallback)")
     cur = torch.cuda.current_device()
-    for t in (rows, *flat):
-        if t is not None:
-            if not t.is_cuda:
-                raise RuntimeError("tt-splat B200 ops need CUDA tensors (no CPU fallback)")
-            if t is not rows and not t.is_contiguous():
-                raise ValueError("tensors must be contiguous")
-            if t.device.index != cur:
-                raise ValueError(f"tensor on {t.device} but the current device is cuda:{cur}: "
-                                 "call under torch.cuda.device(...) of the tensors' device")
+    if rows.get_device() != cur:
+        raise ValueError(f"tensor on {rows.device} but the current device is cuda:{cur}: "
+                         "call under torch.cuda.device(...) of the tensors' device")
+    for t in flat:
+        if t is not None and (t.get_device() != cur or not t.is_contiguous()):
+            _dev(t)
     return cur
+
+
+@functools.lru_cache(maxsize=256)
+def _gather_rows_bwd_bytes(N, R, C):
+    return lib().tts_gather_rows_bwd_workspace_bytes(N, R, C)
 
 
 def gather_rows(table, idx, valid=None, weight=None, scale=1.0, row_shape=None):
@@ -391,9 +395,9 @@ def gather_rows(table, idx, valid=None, weight=None, scale=1.0, row_shape=None):
     (row_shape: the C elements of a row, (C,) when not given)."""
     dev = _dev_rows(table, idx, valid, weight)
     R, C = table.shape
-    out = torch.empty(idx.shape + ((C,) if row_shape is None else row_shape), dtype=table.dtype, device=table.device)
-    call("tts_gather_rows", _addr(table), R, C, table.stride(0), row_type(table, "table"), _addr(idx),
-         index_type(idx, "idx"), _addr(valid), _addr(weight), scale, idx.numel(), _addr(out), _stream(dev))
+    out = table.new_empty(idx.shape + ((C,) if row_shape is None else row_shape))
+    call("tts_gather_rows", table.data_ptr(), R, C, table.stride(0), row_type(table, "table"), idx.data_ptr(),
+         index_type(idx, "idx"), _addr(valid), _addr(weight), scale, idx.numel(), out.data_ptr(), _stream(dev))
     return out
 
 
@@ -409,7 +413,7 @@ def gather_rows_bwd(table, R, idx, valid, weight, scale, gout, want_table=True, 
     nbytes = 0
     if want_table:
         gtable = torch.empty((R, C) if row_shape is None else (R,) + row_shape, dtype=gout.dtype, device=gout.device)
-        nbytes = lib().tts_gather_rows_bwd_workspace_bytes(N, R, C)
+        nbytes = _gather_rows_bwd_bytes(N, R, C)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=gout.device)
     if want_weight:
         gweight = torch.empty(idx.shape, dtype=torch.float32, device=gout.device)
