@@ -387,29 +387,29 @@ struct TileWalk {
   }
 };
 
-// The best few labels of a row in registers, best first.
-template <int K>
+// The best K labels of a row in registers, best first.  A label passes down the places to the first that it
+// comes before and takes it.  Walks in the order of the ids (TURN false) need no look at the ids: an equal value
+// found later never comes before.
+template <int K, bool TURN>
 struct Best {
-  float v[K];
-  int id[K];
+  float v[K > 0 ? K : 1];
+  int id[K > 0 ? K : 1];
   __device__ __forceinline__ void init() {
 #pragma unroll
     for (int k = 0; k < K; ++k) v[k] = -CUDART_INF_F, id[k] = -1;
   }
   // (a masked label never comes before the -inf of an empty place)
   __device__ __forceinline__ void add(float x, int j) {
-    if (!(x > v[K - 1] || (x == v[K - 1] && j < id[K - 1]))) return;
+    bool first = false;      // once it has a place, all behind move down by one
 #pragma unroll
-    for (int k = K - 1; k >= 0; --k) {
-      const bool here = x > v[k] || (x == v[k] && j < id[k]);
-      const bool above = k > 0 && (x > v[k > 0 ? k - 1 : 0] || (x == v[k > 0 ? k - 1 : 0] && j < id[k > 0 ? k - 1 : 0]));
-      if (above) {
-        v[k] = v[k > 0 ? k - 1 : 0];
-        id[k] = id[k > 0 ? k - 1 : 0];
-      } else if (here) {
-        v[k] = x;
-        id[k] = j;
-      }
+    for (int k = 0; k < K; ++k) {
+      first = first || x > v[k] || (TURN && x == v[k] && j < id[k]);
+      const float w = v[k];
+      const int i = id[k];
+      v[k] = first ? x : w;
+      id[k] = first ? j : i;
+      x = first ? w : x;
+      j = first ? i : j;
     }
   }
 };
@@ -431,9 +431,9 @@ __device__ __forceinline__ bool load_tile(const T* logits, long long first, int 
   return whole == 0 || mbar_wait_bounded(bar, 0);
 }
 
-constexpr int TILE_BEST = 4;      // alternatives kept in registers
+constexpr int TILE_BEST = 4;      // alternatives kept in registers (K of them; K = 0: none or more than these)
 
-template <class T, int VB, bool TURN, bool FEW>
+template <class T, int VB, bool TURN, int K>
 __global__ void __launch_bounds__(128) k_scores_tile(const T* __restrict__ logits, long long P, ScoreArgs a) {
   using U = Unit<T, VB>;
   extern __shared__ __align__(16) char smem[];
@@ -450,8 +450,8 @@ __global__ void __launch_bounds__(128) k_scores_tile(const T* __restrict__ logit
   typename U::W* xu = reinterpret_cast<typename U::W*>(x);
   Soft f;
   f.init();
-  Best<TILE_BEST> best;
-  if (FEW) best.init();
+  Best<K, TURN> best;
+  best.init();
   TileWalk<TURN> w(units);
 #pragma unroll 4
   for (int i = 0; i < units; ++i) {
@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(128) k_scores_tile(const T* __restrict__ logit
 #pragma unroll
     for (int e = 0; e < U::E; ++e) {
       f.m = max_nan(f.m, v[e]);
-      if (FEW) best.add(v[e], j * U::E + e);
+      best.add(v[e], j * U::E + e);
     }
   }
 #pragma unroll 4
@@ -472,30 +472,29 @@ __global__ void __launch_bounds__(128) k_scores_tile(const T* __restrict__ logit
     for (int e = 0; e < U::E; ++e) f.add(v[e]);
   }
   const float2 st = write_scores(a, r, f, x, label);
-  if constexpr (FEW) {
+  if constexpr (K > 0) {
 #pragma unroll
-    for (int k = 0; k < TILE_BEST; ++k)
-      if (k < a.top) write_top(a, r, k, best.v[k], f.bad() ? -1 : best.id[k], st);
+    for (int k = 0; k < K; ++k) write_top(a, r, k, best.v[k], f.bad() ? -1 : best.id[k], st);
   } else {
-  // the best label left, taken out of the tile after each round
-  for (int k = 0; k < a.top; ++k) {
-    float bv = -CUDART_INF_F;
-    int bi = -1;
-    if (!f.bad())
+    // the best label left, taken out of the tile after each round
+    for (int k = 0; k < a.top; ++k) {
+      float bv = -CUDART_INF_F;
+      int bi = -1;
+      if (!f.bad())
 #pragma unroll 4
-      for (int i = 0; i < units; ++i) {
-        const int j = w.next(i);
-        float v[U::E];
-        U(xu[j]).get(v);
+        for (int i = 0; i < units; ++i) {
+          const int j = w.next(i);
+          float v[U::E];
+          U(xu[j]).get(v);
 #pragma unroll
-        for (int e = 0; e < U::E; ++e) {
-          const int id = j * U::E + e;
-          if (v[e] > bv || (TURN && v[e] == bv && id < bi)) bv = v[e], bi = id;
+          for (int e = 0; e < U::E; ++e) {
+            const int id = j * U::E + e;
+            if (v[e] > bv || (TURN && v[e] == bv && id < bi)) bv = v[e], bi = id;
+          }
         }
-      }
-    if (bi >= 0) x[bi] = from_f32<T>(-CUDART_INF_F);
-    write_top(a, r, k, bv, bi, st);
-  }
+      if (bi >= 0) x[bi] = from_f32<T>(-CUDART_INF_F);
+      write_top(a, r, k, bv, bi, st);
+    }
   }
 }
 
@@ -814,10 +813,16 @@ extern "C" int tts_label_log_probs(const void* logits, long long P, long long C,
       with_tile<T>(C, [&](auto vb, auto turn) {
         constexpr int VB = decltype(vb)::value;
         constexpr bool TURN = decltype(turn)::value;
-        if (top > 0 && top <= TILE_BEST)
-          k_scores_tile<T, VB, TURN, true><<<grid, n, bytes, as_stream(stream)>>>(x, P, a);
-        else
-          k_scores_tile<T, VB, TURN, false><<<grid, n, bytes, as_stream(stream)>>>(x, P, a);
+        const auto launch = [&](auto k) {
+          k_scores_tile<T, VB, TURN, decltype(k)::value><<<grid, n, bytes, as_stream(stream)>>>(x, P, a);
+        };
+        switch (top <= TILE_BEST ? top : 0) {
+          case 1: launch(std::integral_constant<int, 1>()); break;
+          case 2: launch(std::integral_constant<int, 2>()); break;
+          case 3: launch(std::integral_constant<int, 3>()); break;
+          case 4: launch(std::integral_constant<int, 4>()); break;
+          default: launch(std::integral_constant<int, 0>()); break;
+        }
         return TTS_OK;
       });
     } else if (C <= WARP_ROW_MAX) {
