@@ -281,12 +281,17 @@ __global__ void __launch_bounds__(SB_THREADS, 4) k_scores_block(const T* __restr
     s.add(h);
     s.add(t);
   }
+  Vec16<T> w[UNROLL], next[UNROLL];
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u)
+    if (lo + tid + u * SB_THREADS < hi) next[u].w = __ldg(xv + lo + tid + u * SB_THREADS);
   for (long long v0 = lo + tid; v0 < hi; v0 += UNROLL * SB_THREADS) {
-    Vec16<T> w[UNROLL];
+    // the next vectors are on their way while these are worked on
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const long long v = v0 + u * SB_THREADS;
-      if (v < hi) w[u].w = __ldg(xv + v);
+      w[u] = next[u];
+      const long long v = v0 + (UNROLL + u) * SB_THREADS;
+      if (v < hi) next[u].w = __ldg(xv + v);
     }
     float m = s.m;
 #pragma unroll
@@ -498,48 +503,107 @@ __global__ void __launch_bounds__(128) k_scores_tile(const T* __restrict__ logit
   }
 }
 
-// ---- one warp per row ----------------------------------------------------------------------------
-template <class T>
+// ---- one warp per row: rows of up to 1024 labels that no tile takes -------------------------------------
+// The row stays in registers, SLOTS logits a lane.  The k-th largest of the lanes' maxima is a bound that at
+// least k logits reach and few more; those are gathered, a lane for each, and placed by counting how many
+// come before.  More than 32 of them (equal values): one round over the registers for each alternative.
+constexpr long long WARP_ROW_MAX = 1024;
+
+// Unsigned numbers in the order of the floats (no NaN; -0 counts as 0).
+__device__ __forceinline__ unsigned order_key(float x) {
+  const unsigned b = __float_as_uint(x + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float order_value(unsigned k) {
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+
+template <class T, int SLOTS>
 __global__ void __launch_bounds__(256) k_scores_warp(const T* __restrict__ logits, long long P, long long stride,
                                                      ScoreArgs a) {
-  const int lane = threadIdx.x & 31;
+  __shared__ float s_v[8][32];
+  __shared__ int s_id[8][32];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const long long r = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   if (r >= P) return;
   const T* x = logits + r * stride;
   const int C = (int)a.C;
+  const long long label = load_index(a.labels, a.labels64, r);
+  float v[SLOTS];
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) v[i] = i * 32 + lane < C ? to_f32(x[i * 32 + lane]) : -CUDART_INF_F;
   Soft s;
   s.init();
-  for (int j = lane; j < C; j += 32) s.m = max_nan(s.m, to_f32(x[j]));
+  float most = -CUDART_INF_F;
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) most = max_nan(most, v[i]);
+  s.m = max_nan(s.m, most);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) s.m = max_nan(s.m, __shfl_xor_sync(0xffffffffu, s.m, d));
-  for (int j = lane; j < C; j += 32) s.add(to_f32(x[j]));
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i)
+    if (i * 32 < C) s.add(v[i]);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) {
     s.S += __shfl_xor_sync(0xffffffffu, s.S, d);
     s.A += __shfl_xor_sync(0xffffffffu, s.A, d);
   }
   float2 st;
-  if (lane == 0) st = write_scores(a, r, s, x, load_index(a.labels, a.labels64, r));
+  if (lane == 0) st = write_scores(a, r, s, x, label);
+  if (a.top == 0) return;
   st.x = __shfl_sync(0xffffffffu, st.x, 0);
   st.y = __shfl_sync(0xffffffffu, st.y, 0);
-  // the k-th best is the best of those behind the (k-1)-th in the order (value down, id up)
+  if (s.bad()) {
+    if (lane < a.top) write_top(a, r, lane, 0.f, -1, st);
+    return;
+  }
+  unsigned key = order_key(most), kth = 0;
+  for (int k = 0; k < a.top; ++k) {
+    kth = __reduce_max_sync(0xffffffffu, key);
+    if (lane == __ffs(__ballot_sync(0xffffffffu, key == kth)) - 1) key = 0;
+  }
+  const float bound = order_value(kth);
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) {
+    const bool c = v[i] >= bound && v[i] > -CUDART_INF_F;
+    const unsigned b = __ballot_sync(0xffffffffu, c);
+    if (b) {
+      const int at = n + __popc(b & ((1u << lane) - 1));
+      if (c && at < 32) {
+        s_v[wid][at] = v[i];
+        s_id[wid][at] = i * 32 + lane;
+      }
+      n += __popc(b);
+    }
+  }
+  __syncwarp();
+  if (n <= 32) {
+    if (lane < n) {
+      const float w = s_v[wid][lane];
+      const int id = s_id[wid][lane];
+      int place = 0;
+      for (int i = 0; i < n; ++i) place += before(s_v[wid][i], s_id[wid][i], w, id);
+      if (place < a.top) write_top(a, r, place, w, id, st);
+    }
+    if (lane >= n && lane < a.top) write_top(a, r, lane, 0.f, -1, st);
+    return;
+  }
   float pv = CUDART_INF_F;
   int pid = -1;
   for (int k = 0; k < a.top; ++k) {
     float bv = -CUDART_INF_F;
     int bi = C;
-    if (!s.bad())
-      for (int j = lane; j < C; j += 32) {
-        const float v = to_f32(x[j]);
-        if (before(pv, pid, v, j) && v > bv) bv = v, bi = j;
-      }
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i)
+      if (before(pv, pid, v[i], i * 32 + lane) && v[i] > bv) bv = v[i], bi = i * 32 + lane;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) {
       const float ov = __shfl_xor_sync(0xffffffffu, bv, d);
       const int oi = __shfl_xor_sync(0xffffffffu, bi, d);
       if (before(ov, oi, bv, bi)) bv = ov, bi = oi;
     }
-    if (lane == 0) write_top(a, r, k, bv, bi < C ? bi : -1, st);
+    if (lane == 0) write_top(a, r, k, bv, bi, st);
     pv = bv;
     pid = bi;
   }
@@ -564,19 +628,41 @@ struct RowGrad {
   long long t;
   bool zero;      // nothing comes in: zeros, whatever the row holds
   bool empty;     // masked labels only: zeros
-  __device__ __forceinline__ RowGrad(const GradArgs& a, long long r) {
+  // The gradients of the alternatives that there are, summed by one thread, or by a warp that asks together.
+  static __device__ __forceinline__ float tops(const GradArgs& a, long long r) {
+    float sum = 0.f;
+    if (a.g_top)
+      for (int k = 0; k < a.top; ++k) {
+        const float g = a.g_top[r * a.top + k];
+        if (a.top_ids[r * a.top + k] >= 0) sum += g;
+      }
+    return sum;
+  }
+  static __device__ __forceinline__ float warp_tops(const GradArgs& a, long long r) {
+    float sum = 0.f;
+    if (a.g_top) {
+      const int lane = threadIdx.x & 31;
+      if (lane < a.top) {
+        const float g = a.g_top[r * a.top + lane];
+        if (a.top_ids[r * a.top + lane] >= 0) sum = g;
+      }
+#pragma unroll
+      for (int d = TOP_MAX / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      sum = __shfl_sync(0xffffffffu, sum, 0);
+    }
+    return sum;
+  }
+  __device__ __forceinline__ RowGrad(const GradArgs& a, long long r, float of_tops) {
     const float2 st = a.stats[r];
+    const float H = a.entropy[r];
     gh = a.g_entropy ? a.g_entropy[r] : 0.f;
     t = load_index(a.labels, a.labels64, r);
     gl = 0.f;
     if (a.g_logp && t >= 0) gl = t < a.C ? a.g_logp[r] : CUDART_NAN_F;
-    float total = gl;
-    if (a.g_top)
-      for (int k = 0; k < a.top; ++k)
-        if (a.top_ids[r * a.top + k] >= 0) total += a.g_top[r * a.top + k];
+    const float total = gl + of_tops;
     m = st.x;
     c = -st.y * LOG2E;
-    alpha = st.y != st.y ? CUDART_NAN_F : -total - gh * (a.entropy[r] - st.y);
+    alpha = st.y != st.y ? CUDART_NAN_F : -total - gh * (H - st.y);
     zero = total == 0.f && gh == 0.f;
     empty = st.y == -CUDART_INF_F;
     if (empty) gl = 0.f;
@@ -609,7 +695,7 @@ __global__ void __launch_bounds__(GB_THREADS) k_scores_grad_block(const T* __res
   const long long r = blockIdx.x;
   const T* x = logits + r * stride;
   T* gx = glogits + r * a.C;
-  const RowGrad g(a, r);
+  const RowGrad g(a, r, RowGrad::warp_tops(a, r));
   const bool none = g.zero || g.empty;
   const RowSplit<T> rs(gx, a.C);
   const long long per = (long long)GB_THREADS * GB_UNROLL;
@@ -666,7 +752,7 @@ __global__ void __launch_bounds__(256) k_scores_grad_warp(const T* __restrict__ 
   if (r >= P) return;
   const T* x = logits + r * stride;
   T* gx = glogits + r * a.C;
-  const RowGrad g(a, r);
+  const RowGrad g(a, r, RowGrad::warp_tops(a, r));
   const bool none = g.zero || g.empty;
   const int C = (int)a.C;
   for (int j = lane; j < C; j += 32) gx[j] = from_f32<T>(none ? 0.f : g(to_f32(x[j])));
@@ -688,7 +774,8 @@ __global__ void __launch_bounds__(128) k_scores_grad_tile(const T* __restrict__ 
   const int rows = (int)(P - r0 < blockDim.x ? P - r0 : blockDim.x);
   T* s = reinterpret_cast<T*>(smem);
   const long long r = r0 + threadIdx.x;
-  const RowGrad g(a, threadIdx.x < rows ? r : r0);
+  const long long mine = threadIdx.x < rows ? r : r0;
+  const RowGrad g(a, mine, RowGrad::tops(a, mine));
   if (!load_tile(logits, r0 * C, rows * C, s, &bar)) return;
   if (threadIdx.x < rows) {
     T* x = s + threadIdx.x * C;
@@ -760,8 +847,6 @@ static bool tile_rows(long long C, size_t elem, long long stride, const void* x,
 }
 static int tile_threads(long long C, size_t elem) { return C * (long long)elem <= 128 ? 128 : 64; }
 
-constexpr long long WARP_ROW_MAX = 1024;      // labels up to which a warp takes a row
-
 static int check_labels(long long P, long long C, int type, int top) {
   TTS_REQUIRE(type >= TTS_ROW_F32 && type <= TTS_ROW_F16, "unknown row type");
   TTS_REQUIRE(P >= 0 && P < (1ll << 31), "the number of rows must be below 2^31");
@@ -826,7 +911,13 @@ extern "C" int tts_label_log_probs(const void* logits, long long P, long long C,
         return TTS_OK;
       });
     } else if (C <= WARP_ROW_MAX) {
-      k_scores_warp<T><<<(unsigned)((P + 7) / 8), 256, 0, as_stream(stream)>>>(x, P, row_stride, a);
+      const unsigned grid = (unsigned)((P + 7) / 8);
+      if (C <= 256)
+        k_scores_warp<T, 8><<<grid, 256, 0, as_stream(stream)>>>(x, P, row_stride, a);
+      else if (C <= 512)
+        k_scores_warp<T, 16><<<grid, 256, 0, as_stream(stream)>>>(x, P, row_stride, a);
+      else
+        k_scores_warp<T, 32><<<grid, 256, 0, as_stream(stream)>>>(x, P, row_stride, a);
     } else if (int rc = launch_scores_block<T>(x, P, row_stride, a, as_stream(stream))) {
       return rc;
     }
