@@ -73,10 +73,14 @@ class _LabelLogProbs(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g_logp, g_entropy, g_top, _):
         logits, labels, stats, entropy, top_ids = ctx.saved_tensors
-        f = lambda g: None if g is None else g.contiguous()  # noqa: E731
+        if g_logp is not None:
+            g_logp = g_logp.contiguous()
+        if g_entropy is not None:
+            g_entropy = g_entropy.contiguous()
+        if g_top is not None:
+            g_top = g_top.contiguous()
         with on_device(logits):
-            return ops.label_log_probs_bwd(logits, labels, stats, entropy, top_ids, f(g_logp), f(g_entropy),
-                                           f(g_top)), None, None
+            return ops.label_log_probs_bwd(logits, labels, stats, entropy, top_ids, g_logp, g_entropy, g_top), None, None
 
 
 def label_log_probs(logits, labels, top=0):

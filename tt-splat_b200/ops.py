@@ -401,10 +401,10 @@ def gather_rows(table, idx, valid=None, weight=None, scale=1.0, row_shape=None):
     return out
 
 
-def gather_rows_bwd(table, R, idx, valid, weight, scale, gout, want_table=True, want_weight=False, row_shape=None):
-    """Gradients of gather_rows from gout [N, C] (unit stride along the rows): gtable [R, *row_shape] in
-    gout's type and gweight of idx's shape (each None when not wanted); ``table`` is read for the weight
-    gradient only and may be None without it."""
+def gather_rows_bwd(table, R, idx, valid, weight, scale, gout, want_table=True, want_weight=False):
+    """Gradients of gather_rows from gout [N, C] (unit stride along the rows): gtable [R, C] in gout's type
+    and gweight of idx's shape (each None when not wanted); ``table`` is read for the weight gradient only
+    and may be None without it."""
     dev = _dev_rows(gout, idx, valid, weight)
     if table is not None:
         _dev_rows(table)
@@ -412,11 +412,11 @@ def gather_rows_bwd(table, R, idx, valid, weight, scale, gout, want_table=True, 
     gtable = gweight = ws = None
     nbytes = 0
     if want_table:
-        gtable = torch.empty((R, C) if row_shape is None else (R,) + row_shape, dtype=gout.dtype, device=gout.device)
+        gtable = gout.new_empty((R, C))
         nbytes = _gather_rows_bwd_bytes(N, R, C)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=gout.device)
+        ws = gout.new_empty(nbytes, dtype=torch.uint8)
     if want_weight:
-        gweight = torch.empty(idx.shape, dtype=torch.float32, device=gout.device)
+        gweight = idx.new_empty(idx.shape, dtype=torch.float32)
     call("tts_gather_rows_bwd", _addr(table), R, C, 0 if table is None else table.stride(0), row_type(gout, "gout"),
          _addr(idx), index_type(idx, "idx"), _addr(valid), _addr(weight), scale, N, _addr(gout), gout.stride(0),
          _addr(gtable), _addr(gweight), _addr(ws), nbytes, _stream(dev))
@@ -429,14 +429,14 @@ def label_log_probs(logits, labels, top=0, want_stats=True):
     is None when not wanted."""
     dev = _dev_rows(logits, labels)
     P, C = logits.shape
-    on = dict(dtype=torch.float32, device=logits.device)
-    logp, entropy = torch.empty(labels.shape, **on), torch.empty(labels.shape, **on)
-    top_logp = torch.empty(labels.shape + (top,), **on)
-    top_ids = torch.empty(labels.shape + (top,), dtype=torch.int64, device=logits.device)
-    stats = torch.empty((P, 2), **on) if want_stats else None
-    call("tts_label_log_probs", _addr(logits), P, C, logits.stride(0), row_type(logits, "logits"), _addr(labels),
-         index_type(labels, "labels"), top, _addr(logp), _addr(entropy), _addr(top_logp), _addr(top_ids), _addr(stats),
-         _stream(dev))
+    shape, f32 = labels.shape, torch.float32
+    logp, entropy = labels.new_empty(shape, dtype=f32), labels.new_empty(shape, dtype=f32)
+    top_logp = labels.new_empty(shape + (top,), dtype=f32)
+    top_ids = labels.new_empty(shape + (top,), dtype=torch.int64)
+    stats = labels.new_empty((P, 2), dtype=f32) if want_stats else None
+    call("tts_label_log_probs", logits.data_ptr(), P, C, logits.stride(0), row_type(logits, "logits"), labels.data_ptr(),
+         index_type(labels, "labels"), top, logp.data_ptr(), entropy.data_ptr(), top_logp.data_ptr(), top_ids.data_ptr(),
+         _addr(stats), _stream(dev))
     return logp, entropy, top_logp, top_ids, stats
 
 
@@ -444,10 +444,10 @@ def label_log_probs_bwd(logits, labels, stats, entropy, top_ids, g_logp=None, g_
     """Gradient of label_log_probs in the logits, [P, C] contiguous; absent gradients count as zero."""
     dev = _dev_rows(logits, labels, stats, entropy, top_ids, g_logp, g_entropy, g_top)
     P, C = logits.shape
-    gx = torch.empty((P, C), dtype=logits.dtype, device=logits.device)
-    call("tts_label_log_probs_bwd", _addr(logits), P, C, logits.stride(0), row_type(logits, "logits"), _addr(labels),
-         index_type(labels, "labels"), top_ids.shape[-1], _addr(stats), _addr(entropy), _addr(top_ids), _addr(g_logp),
-         _addr(g_entropy), _addr(g_top), _addr(gx), _stream(dev))
+    gx = logits.new_empty((P, C))
+    call("tts_label_log_probs_bwd", logits.data_ptr(), P, C, logits.stride(0), row_type(logits, "logits"),
+         labels.data_ptr(), index_type(labels, "labels"), top_ids.shape[-1], stats.data_ptr(), entropy.data_ptr(),
+         top_ids.data_ptr(), _addr(g_logp), _addr(g_entropy), _addr(g_top), gx.data_ptr(), _stream(dev))
     return gx
 
 
