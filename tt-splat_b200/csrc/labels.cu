@@ -685,12 +685,14 @@ struct RowGrad {
 
 constexpr int GB_THREADS = 256;
 constexpr int GB_UNROLL = 4;
+constexpr long long GB_STEP = (long long)GB_THREADS * GB_UNROLL;
 
-// Blocks of one row each (blockIdx.x: row, blockIdx.y: part of its vectors); the labels whose gradient has
-// a term of its own are stored last, behind a barrier.
+// Blocks of one row each (blockIdx.x: row, blockIdx.y: a part of `steps` steps of its vectors, the next step's
+// on their way while this one's are worked on); the labels whose gradient has a term of its own are stored
+// last, behind a barrier.
 template <class T, bool SAME>
-__global__ void __launch_bounds__(GB_THREADS) k_scores_grad_block(const T* __restrict__ logits, long long stride, GradArgs a,
-                                                                  T* __restrict__ glogits) {
+__global__ void __launch_bounds__(GB_THREADS) k_scores_grad_block(const T* __restrict__ logits, long long stride, int steps,
+                                                                  GradArgs a, T* __restrict__ glogits) {
   constexpr int N = Vec16<T>::E;
   const long long r = blockIdx.x;
   const T* x = logits + r * stride;
@@ -698,37 +700,45 @@ __global__ void __launch_bounds__(GB_THREADS) k_scores_grad_block(const T* __res
   const RowGrad g(a, r, RowGrad::warp_tops(a, r));
   const bool none = g.zero || g.empty;
   const RowSplit<T> rs(gx, a.C);
-  const long long per = (long long)GB_THREADS * GB_UNROLL;
-  const long long lo = blockIdx.y * per, hi = lo + per < rs.nv ? lo + per : rs.nv;
+  const long long lo = blockIdx.y * steps * GB_STEP, hi = lo + steps * GB_STEP < rs.nv ? lo + steps * GB_STEP : rs.nv;
   const long long j0 = blockIdx.y == 0 ? 0 : rs.head + lo * N;
   const long long j1 = blockIdx.y == gridDim.y - 1 ? a.C : rs.head + hi * N;
   const uint4* xv = reinterpret_cast<const uint4*>(x + rs.head);
   uint4* gv = reinterpret_cast<uint4*>(gx + rs.head);
-  Vec16<T> w[GB_UNROLL];
+  Vec16<T> next[GB_UNROLL];
+  auto fetch = [&](long long v0) {
 #pragma unroll
-  for (int u = 0; u < GB_UNROLL; ++u) {
-    const long long v = lo + u * GB_THREADS + threadIdx.x;
-    if (v < hi && !none) {
-      if constexpr (SAME) {
-        w[u].w = __ldcs(xv + v);
-      } else {
-        float f[N];
+    for (int u = 0; u < GB_UNROLL; ++u) {
+      const long long v = v0 + u * GB_THREADS;
+      if (v < hi && !none) {
+        if constexpr (SAME) {
+          next[u].w = __ldcs(xv + v);
+        } else {
+          float f[N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) f[e] = to_f32(x[rs.head + v * N + e]);
-        w[u].set(f);
+          for (int e = 0; e < N; ++e) f[e] = to_f32(x[rs.head + v * N + e]);
+          next[u].set(f);
+        }
       }
     }
-  }
+  };
+  fetch(lo + threadIdx.x);
+  for (long long v0 = lo + threadIdx.x; v0 < hi; v0 += GB_STEP) {
+    Vec16<T> w[GB_UNROLL];
 #pragma unroll
-  for (int u = 0; u < GB_UNROLL; ++u) {
-    const long long v = lo + u * GB_THREADS + threadIdx.x;
-    if (v < hi) {
-      float f[N];
-      w[u].get(f);
+    for (int u = 0; u < GB_UNROLL; ++u) w[u] = next[u];
+    fetch(v0 + GB_STEP);
 #pragma unroll
-      for (int e = 0; e < N; ++e) f[e] = none ? 0.f : g(f[e]);
-      w[u].set(f);
-      __stcs(gv + v, w[u].w);
+    for (int u = 0; u < GB_UNROLL; ++u) {
+      const long long v = v0 + u * GB_THREADS;
+      if (v < hi) {
+        float f[N];
+        w[u].get(f);
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = none ? 0.f : g(f[e]);
+        w[u].set(f);
+        __stcs(gv + v, w[u].w);
+      }
     }
   }
   if (blockIdx.y == 0 && threadIdx.x < rs.head)
@@ -954,12 +964,15 @@ extern "C" int tts_label_log_probs_bwd(const void* logits, long long P, long lon
       // the logits' 16-byte vectors line up with the gradient's when both start on the same offset in every row
       const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(gx)) & 15u) == 0 &&
                         (row_stride - C) * (long long)sizeof(T) % 16 == 0;
-      const long long vecs = C / Vec16<T>::E, per = (long long)GB_THREADS * GB_UNROLL;
-      const dim3 grid((unsigned)P, (unsigned)((vecs + per - 1) / per));
+      // a few steps to a block where that leaves blocks enough for the SMs
+      const long long parts = (C / Vec16<T>::E + GB_STEP - 1) / GB_STEP;
+      int steps = 1;
+      while (steps < 8 && steps < parts && P * parts / (steps * 2) >= 148 * 16) steps *= 2;
+      const dim3 grid((unsigned)P, (unsigned)((parts + steps - 1) / steps));
       if (same)
-        k_scores_grad_block<T, true><<<grid, GB_THREADS, 0, st>>>(x, row_stride, a, gx);
+        k_scores_grad_block<T, true><<<grid, GB_THREADS, 0, st>>>(x, row_stride, steps, a, gx);
       else
-        k_scores_grad_block<T, false><<<grid, GB_THREADS, 0, st>>>(x, row_stride, a, gx);
+        k_scores_grad_block<T, false><<<grid, GB_THREADS, 0, st>>>(x, row_stride, steps, a, gx);
     }
     return check_launch("label_log_probs_bwd");
   });
