@@ -99,7 +99,7 @@ __device__ __forceinline__ float sum8(float (&v)[8], int gl, int lanes, unsigned
 }
 
 template <class T, int VB, int PL, bool GW>
-__global__ void __launch_bounds__(GT, GW && PL * VB <= 8 ? 3 : 1) k_rows_grad(GradArgs a, const T* __restrict__ table, const T* __restrict__ gout,
+__global__ void __launch_bounds__(GT, PL * VB <= (GW ? 8 : 16) ? 3 : 1) k_rows_grad(GradArgs a, const T* __restrict__ table, const T* __restrict__ gout,
                                                   T* __restrict__ gtable) {
   using U = Unit<T, VB>;
   using W = typename U::W;

@@ -118,25 +118,34 @@ __global__ void __launch_bounds__(ST) k_sort_count(PassIn in, int digits, unsign
   for (int i = threadIdx.x; i < digits; i += ST) counts[(long long)blockIdx.x * digits + i] = h[i];
 }
 
-// Running sums of the counts over the tiles (exclusive, in place) and the digits' totals: a block takes 32
-// digits, a lane for each, its warps consecutive parts of the tiles.
+// Running sums of the counts over the tiles (exclusive, in place) and the digits' totals.  A block takes 8
+// digits (32 bytes of a tile's counts) and its 128 groups of 8 lanes consecutive parts of the tiles, so that
+// a thread has few loads to wait for.
+constexpr int SCAN_DIGITS = 8;
 constexpr int SCAN_WARPS = 32;
+constexpr int SCAN_PARTS = SCAN_WARPS * 32 / SCAN_DIGITS;
 __global__ void __launch_bounds__(32 * SCAN_WARPS) k_sort_scan(unsigned* __restrict__ counts, long long tiles, int digits,
                                                                unsigned* __restrict__ totals) {
-  __shared__ unsigned s_part[SCAN_WARPS][32];
+  __shared__ unsigned s_warp[SCAN_WARPS][SCAN_DIGITS];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const int d = blockIdx.x * 32 + lane;
-  const long long t0 = tiles * wid / SCAN_WARPS, t1 = tiles * (wid + 1) / SCAN_WARPS;
+  const int dl = lane % SCAN_DIGITS, d = blockIdx.x * SCAN_DIGITS + dl, part = threadIdx.x / SCAN_DIGITS;
+  const long long t0 = tiles * part / SCAN_PARTS, t1 = tiles * (part + 1) / SCAN_PARTS;
   unsigned sum = 0;
 #pragma unroll 8
   for (long long t = t0; t < t1; ++t) sum += counts[t * digits + d];
-  s_part[wid][lane] = sum;
+  unsigned incl = sum;
+#pragma unroll
+  for (int o = SCAN_DIGITS; o < 32; o <<= 1) {
+    const unsigned y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane >= 32 - SCAN_DIGITS) s_warp[wid][dl] = incl;
   __syncthreads();
-  unsigned run = 0;
+  unsigned run = incl - sum;
 #pragma unroll
   for (int w = 0; w < SCAN_WARPS; ++w)
-    if (w < wid) run += s_part[w][lane];
-  if (wid == SCAN_WARPS - 1) totals[d] = run + sum;
+    if (w < wid) run += s_warp[w][dl];
+  if (part == SCAN_PARTS - 1) totals[d] = run + sum;
   for (long long t = t0; t < t1; t += 8) {
     unsigned c[8];
 #pragma unroll
@@ -394,7 +403,7 @@ int sort_uses(const RowUses& u, const SortSpace& s, void* clear, size_t clear_by
     const PassIn in{u, p == 0 ? nullptr : (to_sorted ? s.other : s.sorted), s.n, dg.shift(p)};
     uint2* dst = to_sorted ? s.sorted : s.other;
     k_sort_count<<<tiles, ST, 0, st>>>(in, D, s.counts, p == 0 ? s.used : nullptr, p == 0 ? gweight : nullptr);
-    k_sort_scan<<<D / 32, 32 * SCAN_WARPS, 0, st>>>(s.counts, tiles, D, s.totals);
+    k_sort_scan<<<D / SCAN_DIGITS, 32 * SCAN_WARPS, 0, st>>>(s.counts, tiles, D, s.totals);
     const auto move = [&](auto bits) {
       k_sort_move<decltype(bits)::value><<<tiles, ST, 0, st>>>(in, s.counts, s.totals, p == 0 ? s.n : nullptr, dst);
     };
