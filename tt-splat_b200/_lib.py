@@ -7,12 +7,14 @@ work and can be captured in CUDA graphs.
 """
 import contextlib
 import ctypes as C
+import importlib.util
 import os
 
 import torch
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libttsplat_b200.so")
+TORCH_OPS_PATH = os.path.join(HERE, "_torch_ops.so")
 
 P = C.c_void_p
 I = C.c_int
@@ -110,6 +112,24 @@ def lib():
             fn.argtypes = args
         _lib = h
     return _lib
+
+
+_torch_ops = None
+
+
+def torch_ops():
+    """Load (once) and return the torch functions of ``csrc/torch_ops.cpp``; raises when they have not
+    been built."""
+    global _torch_ops
+    if _torch_ops is None:
+        if not os.path.exists(TORCH_OPS_PATH):
+            raise RuntimeError(f"{TORCH_OPS_PATH} is missing: build it with __graft_entry__.build() "
+                               "(there is no CPU fallback)")
+        spec = importlib.util.spec_from_file_location("_torch_ops", TORCH_OPS_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        _torch_ops = mod
+    return _torch_ops
 
 
 class TTSError(RuntimeError):

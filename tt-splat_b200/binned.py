@@ -11,9 +11,8 @@
   the per-tile WSR forward and backward on operands in the reference's layout.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
-from ._lib import on_device
+from ._lib import on_device, torch_ops
 from . import ops
 from .camera import as_camera, pack_cameras
 from .model import flat_of
@@ -86,30 +85,6 @@ def theta_u_gathered(conic_t, mu_t, origins, k):
         return _ThetaGathered.apply(conic_t, mu_t, origins, float(k))
 
 
-class _GatherRows(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, table, weight, idx, valid, scale, row_shape):
-        ctx.save_for_backward(table if ctx.needs_input_grad[1] else None, weight, idx, valid)
-        ctx.scale, ctx.R, ctx.row_shape = scale, table.shape[0], row_shape
-        return ops.gather_rows(table, idx, valid, weight, scale, row_shape)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gout):
-        table, weight, idx, valid = ctx.saved_tensors
-        width = 1
-        for n in ctx.row_shape:
-            width *= n
-        if width:
-            gout = ops.rows2d(gout, width)
-        else:
-            gout = gout.reshape(idx.numel(), 0)
-        with on_device(gout):
-            gt, gw = ops.gather_rows_bwd(table, ctx.R, idx, valid, weight, ctx.scale, gout,
-                                         want_table=ctx.needs_input_grad[0], want_weight=ctx.needs_input_grad[1])
-        return gt, gw, None, None, None, None
-
-
 def gather_rows(table, idx, valid=None, weight=None, scale=1.0):
     """Rows of ``table`` [R, ...] by ``idx`` [...] -> [*idx.shape, *table.shape[1:]]: slot n gets
     scale * weight[n] * table[idx[n]], rounded once to the table's type.
@@ -124,34 +99,9 @@ def gather_rows(table, idx, valid=None, weight=None, scale=1.0):
     nothing looks up.  To capture a training step in a CUDA graph, take its gradients with
     ``torch.autograd.grad`` and drop the outputs of eager calls on the same leaves first: torch ties
     a leaf's gradient to the stream of the graph that is still alive, and the capture fails."""
-    if table.dim() < 1:
-        raise ValueError("table must have at least one dimension")
     if isinstance(scale, torch.Tensor):
         raise TypeError("scale must be a number (a factor that is learned goes into weight or the table)")
-    ops.row_type(table, "table")
-    ops.index_type(idx, "idx")
-    shape, row_shape = idx.shape, tuple(table.shape[1:])
-    idx = idx.contiguous()
-    if valid is not None:
-        if valid.dtype not in (torch.bool, torch.uint8):
-            raise TypeError(f"valid must be bool or uint8, got {valid.dtype}")
-        if valid.shape != shape:
-            raise ValueError(f"valid must have the shape of idx {tuple(shape)}, got {tuple(valid.shape)}")
-        valid = valid.contiguous()
-    if weight is not None:
-        if weight.dtype != torch.float32:
-            raise TypeError(f"weight must be float32, got {weight.dtype}")
-        if weight.shape != shape:
-            raise ValueError(f"weight must have the shape of idx {tuple(shape)}, got {tuple(weight.shape)}")
-        weight = weight.contiguous()
-    width = 1
-    for n in row_shape:
-        width *= n
-    with on_device(table):
-        rows = ops.rows2d(table, width)
-        if torch.is_grad_enabled() and (rows.requires_grad or (weight is not None and weight.requires_grad)):
-            return _GatherRows.apply(rows, weight, idx, valid, float(scale), row_shape)
-        return ops.gather_rows(rows, idx, valid, weight, float(scale), row_shape)
+    return torch_ops().gather_rows(table, idx, valid, weight, scale)
 
 
 class _Operands(torch.autograd.Function):

@@ -2,7 +2,9 @@
 
 Each ``csrc/*.cu`` compiles to an object with relocatable device code (the device status word
 is shared across translation units), then nvcc links them into one shared library next to this
-file.  Objects are rebuilt only when a source or header is newer.  Usage:
+file.  ``csrc/torch_ops.cpp`` (torch functions over the C entry points) compiles with g++ against the
+installed torch into ``_torch_ops.so``, which links to that library.  Objects are rebuilt only when a
+source or header is newer.  Usage:
 
     python tt-splat_b200/build.py            # or __graft_entry__.build()
 """
@@ -16,6 +18,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libttsplat_b200.so")
+TORCH_OPS = os.path.join(HERE, "_torch_ops.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -38,6 +41,38 @@ def _headers_mtime():
     paths = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
     paths += [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE)]
     return max((os.path.getmtime(p) for p in paths), default=0.0)
+
+
+def _torch_ops_command():
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    gxx = os.environ.get("CXX") or shutil.which("g++")
+    if not gxx:
+        raise RuntimeError("g++ not found: the torch functions cannot be built")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
+    inc = cpp_extension.include_paths() + [cuda, sysconfig.get_paths()["include"]]
+    lib = cpp_extension.library_paths()
+    return [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_torch_ops",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in inc),
+            # the C++ library before torch's, which carry parts of another one
+            os.path.join(CSRC, "torch_ops.cpp"), "-o", TORCH_OPS, "-Wl,--no-as-needed", "-l:libstdc++.so.6",
+            *(f"-L{p}" for p in lib), f"-L{HERE}", "-lttsplat_b200", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+
+
+def build_torch_ops(verbose=True):
+    """``_torch_ops.so``; needs the CUDA library to link to."""
+    src = os.path.join(CSRC, "torch_ops.cpp")
+    newest = max(os.path.getmtime(src), _headers_mtime())
+    if not os.path.exists(TORCH_OPS) or os.path.getmtime(TORCH_OPS) < newest:
+        if verbose:
+            print("torch_ops.cpp -o _torch_ops.so", flush=True)
+        res = subprocess.run(_torch_ops_command(), capture_output=True, text=True)
+        if res.returncode != 0:
+            sys.stderr.write(res.stdout + res.stderr)
+            raise RuntimeError("g++ failed on torch_ops.cpp")
+    return TORCH_OPS
 
 
 def build_library(verbose=True, extra_flags=()):
@@ -67,6 +102,7 @@ def build_library(verbose=True, extra_flags=()):
         if res.returncode != 0:
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError("nvcc link failed")
+    build_torch_ops(verbose)
     return LIB
 
 

@@ -7,9 +7,8 @@ pass; the autograd backward scales the stored gradient.  Images are [H,W,3] (or 
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from ._lib import on_device
+from ._lib import on_device, torch_ops
 from . import ops
 
 
@@ -60,29 +59,6 @@ class LabelLogProbs(NamedTuple):
     top_ids: torch.Tensor     # [..., top] their ids (int64)
 
 
-class _LabelLogProbs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, top):
-        logp, entropy, top_logp, top_ids, stats = ops.label_log_probs(logits, labels, top)
-        ctx.save_for_backward(logits, labels, stats, entropy, top_ids)
-        ctx.mark_non_differentiable(top_ids)
-        ctx.set_materialize_grads(False)
-        return logp, entropy, top_logp, top_ids
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_logp, g_entropy, g_top, _):
-        logits, labels, stats, entropy, top_ids = ctx.saved_tensors
-        if g_logp is not None:
-            g_logp = g_logp.contiguous()
-        if g_entropy is not None:
-            g_entropy = g_entropy.contiguous()
-        if g_top is not None:
-            g_top = g_top.contiguous()
-        with on_device(logits):
-            return ops.label_log_probs_bwd(logits, labels, stats, entropy, top_ids, g_logp, g_entropy, g_top), None, None
-
-
 def label_log_probs(logits, labels, top=0):
     """Log probabilities of ``labels`` [...] under the softmax of ``logits`` [..., C], with the
     entropy of each row and its ``top`` (0 to 16) best labels -> ``LabelLogProbs`` in fp32.
@@ -97,19 +73,4 @@ def label_log_probs(logits, labels, top=0):
     gets zeros whatever it holds.  To capture a training step in a CUDA graph, take its gradients
     with ``torch.autograd.grad`` and drop the outputs of eager calls on the same leaves first: torch
     ties a leaf's gradient to the stream of the graph that is still alive, and the capture fails."""
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError(f"logits must be [..., C] with at least one label, got {tuple(logits.shape)}")
-    ops.row_type(logits, "logits")
-    ops.index_type(labels, "labels")
-    shape = logits.shape[:-1]
-    if labels.shape != shape:
-        raise ValueError(f"labels must have the shape {tuple(shape)}, got {tuple(labels.shape)}")
-    if not 0 <= int(top) <= 16:
-        raise ValueError(f"top must be 0 to 16, got {top}")
-    top = int(top)
-    labels = labels.contiguous()
-    with on_device(logits):
-        x = ops.rows2d(logits, logits.shape[-1])
-        if torch.is_grad_enabled() and x.requires_grad:
-            return LabelLogProbs(*_LabelLogProbs.apply(x, labels, top))
-        return LabelLogProbs(*ops.label_log_probs(x, labels, top, want_stats=False)[:4])
+    return LabelLogProbs(*torch_ops().label_log_probs(logits, labels, top))

@@ -3,8 +3,6 @@
 Shapes follow ``include/ttsplat_b200.h``.  Every function validates that its tensors are CUDA
 and contiguous and raises otherwise (no CPU fallback).
 """
-import functools
-
 import numpy as np
 import torch
 
@@ -333,122 +331,6 @@ def unit_from_u8(src, out=None):
         out = torch.empty(src.shape, dtype=torch.float32, device=src.device)
     call("tts_unit_from_u8", ptr(src), src.numel(), ptr(out), stream())
     return out
-
-
-_ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_INDEX_TYPES = {torch.int32: 0, torch.int64: 1}
-
-
-def row_type(t, what):
-    """Type code (TTS_ROW_*) of a tensor of rows."""
-    if t.dtype not in _ROW_TYPES:
-        raise TypeError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
-    return _ROW_TYPES[t.dtype]
-
-
-def index_type(t, what):
-    if t.dtype not in _INDEX_TYPES:
-        raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
-    return _INDEX_TYPES[t.dtype]
-
-
-def rows2d(t, width):
-    """[n, width] view of a tensor's rows with unit stride along them (the kernels take any distance
-    between rows, an expanded one included); a copy where no such view exists."""
-    if t.dim() != 2:
-        t = t.reshape(-1, width) if width else t.reshape(t.shape[0], 0)
-    return t if (width <= 1 or t.stride(1) == 1) and t.stride(0) < 1 << 30 else t.contiguous()
-
-
-def _addr(t):
-    """Device address of a tensor that has passed _dev or _dev_rows, or was allocated here."""
-    return None if t is None else t.data_ptr()
-
-
-def _stream(index):
-    """Current stream of the current device ``index``."""
-    return torch._C._cuda_getCurrentRawStream(index)
-
-
-def _dev_rows(rows, *flat):
-    """As _dev, with a first tensor of rows that need not be contiguous; returns the device index."""
-    if not rows.is_cuda:
-        raise RuntimeError("tt-splat B200 ops need CUDA tensors (no CPU fallback)")
-    cur = torch.cuda.current_device()
-    if rows.get_device() != cur:
-        raise ValueError(f"tensor on {rows.device} but the current device is cuda:{cur}: "
-                         "call under torch.cuda.device(...) of the tensors' device")
-    for t in flat:
-        if t is not None and (t.get_device() != cur or not t.is_contiguous()):
-            _dev(t)
-    return cur
-
-
-@functools.lru_cache(maxsize=256)
-def _gather_rows_bwd_bytes(N, R, C):
-    return lib().tts_gather_rows_bwd_workspace_bytes(N, R, C)
-
-
-def gather_rows(table, idx, valid=None, weight=None, scale=1.0, row_shape=None):
-    """out[n] = scale * weight[n] * table[idx[n]] for table [R, C] (unit stride along the rows) and
-    contiguous idx, valid (uint8 or bool) and weight (float32) of one shape -> [*idx.shape, *row_shape]
-    (row_shape: the C elements of a row, (C,) when not given)."""
-    dev = _dev_rows(table, idx, valid, weight)
-    R, C = table.shape
-    out = table.new_empty(idx.shape + ((C,) if row_shape is None else row_shape))
-    call("tts_gather_rows", table.data_ptr(), R, C, table.stride(0), row_type(table, "table"), idx.data_ptr(),
-         index_type(idx, "idx"), _addr(valid), _addr(weight), scale, idx.numel(), out.data_ptr(), _stream(dev))
-    return out
-
-
-def gather_rows_bwd(table, R, idx, valid, weight, scale, gout, want_table=True, want_weight=False):
-    """Gradients of gather_rows from gout [N, C] (unit stride along the rows): gtable [R, C] in gout's type
-    and gweight of idx's shape (each None when not wanted); ``table`` is read for the weight gradient only
-    and may be None without it."""
-    dev = _dev_rows(gout, idx, valid, weight)
-    if table is not None:
-        _dev_rows(table)
-    N, C = gout.shape
-    gtable = gweight = ws = None
-    nbytes = 0
-    if want_table:
-        gtable = gout.new_empty((R, C))
-        nbytes = _gather_rows_bwd_bytes(N, R, C)
-        ws = gout.new_empty(nbytes, dtype=torch.uint8)
-    if want_weight:
-        gweight = idx.new_empty(idx.shape, dtype=torch.float32)
-    call("tts_gather_rows_bwd", _addr(table), R, C, 0 if table is None else table.stride(0), row_type(gout, "gout"),
-         _addr(idx), index_type(idx, "idx"), _addr(valid), _addr(weight), scale, N, _addr(gout), gout.stride(0),
-         _addr(gtable), _addr(gweight), _addr(ws), nbytes, _stream(dev))
-    return gtable, gweight
-
-
-def label_log_probs(logits, labels, top=0, want_stats=True):
-    """-> (logp, entropy, top_logp [..., top], top_ids [..., top] int64, stats [P, 2]) of logits [P, C] (unit
-    stride along the rows) and contiguous labels [...] of P entries; stats, which only the backward needs,
-    is None when not wanted."""
-    dev = _dev_rows(logits, labels)
-    P, C = logits.shape
-    shape, f32 = labels.shape, torch.float32
-    logp, entropy = labels.new_empty(shape, dtype=f32), labels.new_empty(shape, dtype=f32)
-    top_logp = labels.new_empty(shape + (top,), dtype=f32)
-    top_ids = labels.new_empty(shape + (top,), dtype=torch.int64)
-    stats = labels.new_empty((P, 2), dtype=f32) if want_stats else None
-    call("tts_label_log_probs", logits.data_ptr(), P, C, logits.stride(0), row_type(logits, "logits"), labels.data_ptr(),
-         index_type(labels, "labels"), top, logp.data_ptr(), entropy.data_ptr(), top_logp.data_ptr(), top_ids.data_ptr(),
-         _addr(stats), _stream(dev))
-    return logp, entropy, top_logp, top_ids, stats
-
-
-def label_log_probs_bwd(logits, labels, stats, entropy, top_ids, g_logp=None, g_entropy=None, g_top=None):
-    """Gradient of label_log_probs in the logits, [P, C] contiguous; absent gradients count as zero."""
-    dev = _dev_rows(logits, labels, stats, entropy, top_ids, g_logp, g_entropy, g_top)
-    P, C = logits.shape
-    gx = logits.new_empty((P, C))
-    call("tts_label_log_probs_bwd", logits.data_ptr(), P, C, logits.stride(0), row_type(logits, "logits"),
-         labels.data_ptr(), index_type(labels, "labels"), top_ids.shape[-1], stats.data_ptr(), entropy.data_ptr(),
-         top_ids.data_ptr(), _addr(g_logp), _addr(g_entropy), _addr(g_top), gx.data_ptr(), _stream(dev))
-    return gx
 
 
 def read_status():
