@@ -177,12 +177,25 @@ __global__ void __launch_bounds__(GT, PL * VB <= (GW ? 8 : 16) ? 3 : 1) k_rows_g
         }
     }
   };
-  for (; j < end; j += UN) {
-    U g[UN][PL], t[GW ? UN : 1][GW ? PL : 1];
+  // (units past the row's end stay zero)
+  U g[UN][PL], t[GW ? UN : 1][GW ? PL : 1];
+  float zero[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) zero[e] = 0.f;
+#pragma unroll
+  for (int q = 0; q < UN; ++q)
+#pragma unroll
+    for (int k = 0; k < PL; ++k) {
+      g[q][k].set(zero);
+      if constexpr (GW) t[q][k].set(zero);
+    }
+  // UN uses at once, n of them (all in every step but the last)
+  auto step = [&](auto full, int n) {
+    constexpr bool ALL = decltype(full)::value;
     unsigned key[UN];
 #pragma unroll
     for (int q = 0; q < UN; ++q)
-      if (j + q < end) {
+      if (ALL || q < n) {
         key[q] = s_key[j + q];
         const W* src = reinterpret_cast<const W*>(gbase + (unsigned long long)s_use[j + q] * gstep);
 #pragma unroll
@@ -201,7 +214,7 @@ __global__ void __launch_bounds__(GT, PL * VB <= (GW ? 8 : 16) ? 3 : 1) k_rows_g
 #pragma unroll
     for (int q = 0; q < UN; ++q) {
       dot[q] = 0.f;
-      if (j + q < end) {
+      if (ALL || q < n) {
         if (key[q] != cur) {
           if (cur != NOTHING) flush(false);
           cur = key[q];
@@ -221,8 +234,7 @@ __global__ void __launch_bounds__(GT, PL * VB <= (GW ? 8 : 16) ? 3 : 1) k_rows_g
 #pragma unroll
           for (int e = 0; e < E; ++e) {
             acc[k][e] = fmaf(f, x[e], acc[k][e]);
-            if constexpr (GW)
-              if (col[k]) dot[q] = fmaf(x[e], row[k][e], dot[q]);
+            if constexpr (GW) dot[q] = fmaf(x[e], row[k][e], dot[q]);
           }
         }
       }
@@ -232,17 +244,19 @@ __global__ void __launch_bounds__(GT, PL * VB <= (GW ? 8 : 16) ? 3 : 1) k_rows_g
         if constexpr (UN == 8) {
           const float sum = sum8(dot, gl, a.lanes, mask);
           const int q = gl / (a.lanes / 8);
-          if (gl % (a.lanes / 8) == 0 && j + q < end) a.gweight[s_use[j + q]] = a.u.scale * sum;
+          if (gl % (a.lanes / 8) == 0 && (ALL || q < n)) a.gweight[s_use[j + q]] = a.u.scale * sum;
         }
       } else {
 #pragma unroll
         for (int q = 0; q < UN; ++q) {
           for (int d = a.lanes / 2; d > 0; d >>= 1) dot[q] += __shfl_xor_sync(mask, dot[q], d);
-          if (gl == 0 && j + q < end) a.gweight[s_use[j + q]] = a.u.scale * dot[q];
+          if (gl == 0 && (ALL || q < n)) a.gweight[s_use[j + q]] = a.u.scale * dot[q];
         }
       }
     }
-  }
+  };
+  for (; j + UN <= end; j += UN) step(std::true_type(), UN);
+  if (j < end) step(std::false_type(), end - j);
   if (cur != NOTHING) flush(c.split);
 }
 
@@ -256,6 +270,25 @@ struct JoinItem {
   long long chunk, last;
   unsigned row;
 };
+
+// The first sorted use behind row v, which use `from` still belongs to: the warp's lanes look at 32 places at a
+// time, `step` apart, first outwards and then inwards.
+__device__ __forceinline__ long long past_row(const uint2* __restrict__ s, long long N, unsigned v, long long from,
+                                              long long step) {
+  const int lane = threadIdx.x & 31;
+  long long lo = from;
+  while (true) {
+    const long long p = lo + step * (lane + 1) - 1;
+    const int k = __popc(__ballot_sync(0xffffffffu, p < N && __ldg(&s[p < N ? p : 0].x) == v));
+    lo += step * k;
+    if (k == 32)
+      step *= 32;
+    else if (step == 1)
+      return lo;
+    else
+      step = (step + 31) / 32;
+  }
+}
 
 // Column p of the parts of chunks from, from + step, ... below to.
 __device__ __forceinline__ float add_parts(const float* p, long long C, long long from, long long to, int step) {
@@ -321,28 +354,8 @@ __global__ void __launch_bounds__(GT, 5) k_rows_join(GradArgs a, int lanes, unsi
   bool found = false;
   if (lane < JOIN_TEST && chunk * L < N) {
     const ChunkEnds c(chunk, N, L, R, [&](long long i) { return i >= 0 && i < N ? __ldg(&a.s[i].x) : R; });
-    if (c.split && !(c.open && c.last == c.first)) {
-      // the row's last use
-      long long lo = c.i1 + L, hi = N;
-      for (long long w = L; lo < N; w *= 2) {      // behind a few chunks for most rows
-        const long long at = lo + w < N ? lo + w : N;
-        if (at == N || a.s[at].x > c.last) {
-          hi = at;
-          break;
-        }
-        lo = at + 1;
-      }
-      while (lo < hi) {
-        const long long mid = (lo + hi) >> 1;
-        if (a.s[mid].x <= c.last)
-          lo = mid + 1;
-        else
-          hi = mid;
-      }
-      it = JoinItem{chunk, (lo - 1) / L, c.last};
-      found = it.last - chunk <= JOIN_MANY;
-      if (!found) s_many[atomicAdd(&s_n, 1)] = it;
-    }
+    found = c.split && !(c.open && c.last == c.first);
+    it = JoinItem{chunk, c.i1 + L, c.last};      // (the last use: not before there)
   }
   const int nq = 32 / lanes, q = lane / lanes, gl = lane % lanes;
   const long long c0 = (long long)blockIdx.y * lanes, cstep = (long long)gridDim.y * lanes;
@@ -350,8 +363,13 @@ __global__ void __launch_bounds__(GT, 5) k_rows_join(GradArgs a, int lanes, unsi
   while (todo) {
     const int src = __ffs(todo) - 1;
     todo &= todo - 1;
-    const JoinItem f{__shfl_sync(0xffffffffu, it.chunk, src), __shfl_sync(0xffffffffu, it.last, src),
-                     __shfl_sync(0xffffffffu, it.row, src)};
+    JoinItem f{__shfl_sync(0xffffffffu, it.chunk, src), __shfl_sync(0xffffffffu, it.last, src),
+               __shfl_sync(0xffffffffu, it.row, src)};
+    f.last = (past_row(a.s, N, f.row, f.last, L) - 1) / L;
+    if (f.last - f.chunk > JOIN_MANY) {
+      if (lane == 0) s_many[atomicAdd(&s_n, 1)] = f;
+      continue;
+    }
     for (long long b = c0; b < C; b += cstep) {
       const long long col = b + gl;
       float sum = 0.f;
