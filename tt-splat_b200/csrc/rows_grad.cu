@@ -15,17 +15,16 @@ namespace tts {
 
 constexpr int GT = 256;
 
-// Uses of a chunk: few where there are few, so that they still spread over the SMs, and at most 8 for each lane
-// of the smallest group that rows of this width can have, which bounds a block's uses by BLOCK_USES.
+// Uses of a chunk: few where there are few, so that they still spread over the SMs (100k lookups of 45 fp16: sums
+// and joining 22 us at 16 uses, 31 at 64; 845k of 41 bf16 from 526 rows: 104 us at 32, 88 at 64), and at most 8
+// for each lane of a group, which bounds a block's uses by BLOCK_USES.
 constexpr int L_MAX = 64;
 constexpr int BLOCK_USES = 8 * GT;
-static int chunk_len(long long N, long long C) {
-  int lanes = 1;
-  while (lanes < 32 && lanes * 8 < C) lanes *= 2;
-  const int l = N <= (1 << 14) ? 8 : (N <= (1 << 17) ? 16 : (N <= (1 << 20) ? 32 : L_MAX));
+static int chunk_len(long long N, int lanes) {
+  const int l = N <= (1 << 14) ? 8 : (N <= (1 << 17) ? 16 : L_MAX);
   return l < 8 * lanes ? l : 8 * lanes;
 }
-static long long chunks_of(long long N, long long C) { return (N + chunk_len(N, C) - 1) / chunk_len(N, C); }
+static long long chunks_of(long long N, int lanes) { return (N + chunk_len(N, lanes) - 1) / chunk_len(N, lanes); }
 
 struct GradShape {
   long long units;        // of a row
@@ -399,7 +398,12 @@ __global__ void __launch_bounds__(GT, 5) k_rows_join(GradArgs a, int lanes, unsi
   }
 }
 
-size_t grad_space(long long N, long long C) { return align256((size_t)chunks_of(N, C) * 2 * (size_t)C * sizeof(float)); }
+size_t grad_space(long long N, long long C) {
+  // for the fewest lanes that a group can have, which are those of 16-byte units of two bytes' elements
+  int lanes = 1;
+  while (lanes < 32 && lanes * 8 < C) lanes *= 2;
+  return align256((size_t)chunks_of(N, lanes) * 2 * (size_t)C * sizeof(float));
+}
 
 template <class T>
 static int grad_unit(const void* table, long long table_stride, long long C, const void* gout, long long gout_stride,
@@ -423,11 +427,11 @@ int rows_grad(const RowUses& u, const SortSpace& s, const void* table, long long
   const void* t = gweight ? table : nullptr;
   const int vb = grad_unit(type, t, table_stride, C, gout, gout_stride, gtable);
   GradShape g = grad_shape(C, elem_bytes(type), vb);
-  // few chunks of wide rows: one unit a lane, more column parts
-  if (!gweight && g.per_lane > 1 && chunks_of(u.N, C) * g.lanes < 148 * 512) {
+  // wide rows: one unit a lane and column parts, unless the weights' sums need the row in one warp (134k lookups
+  // of 328 fp32: 52 us, 64 with 4 units a lane)
+  if (!gweight && g.per_lane > 1 && (g.units + g.lanes - 1) / g.lanes <= 65535) {
     g.per_lane = 1;
     g.parts = (int)((g.units + g.lanes - 1) / g.lanes);
-    if (g.parts > 65535) g = grad_shape(C, elem_bytes(type), vb);
   }
   GradArgs a;
   a.u = u;
@@ -437,8 +441,8 @@ int rows_grad(const RowUses& u, const SortSpace& s, const void* table, long long
   a.C = C;
   a.table_stride = table_stride;
   a.gout_stride = gout_stride;
-  a.chunks = chunks_of(u.N, C);
-  a.L = chunk_len(u.N, C);
+  a.chunks = chunks_of(u.N, g.lanes);
+  a.L = chunk_len(u.N, g.lanes);
   a.lanes = g.lanes;
   a.units = (int)g.units;
   a.unit = vb;
