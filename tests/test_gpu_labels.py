@@ -52,7 +52,7 @@ def _reference(x, t, top):
     tlp[:, :k] = torch.where(v[:, :k] > -math.inf, (v[:, :k] - m[:, None]) - logS[:, None], -math.inf)
     # error bounds of the header
     d = torch.where(p > 0, (x - m[:, None]).abs(), 0.0)
-    n = (C + 31) // 32 + 16
+    n = max((C + 31) // 32 + 16, C // 4 + 6 if C <= 256 else 0)
     D, D2 = (p * d).sum(1), (p * d * d).sum(1)
     eS = U * (2 * D + 4 + n)
     eL = eS + 4 * U * (1 + logS)
@@ -128,6 +128,37 @@ def test_label_counts(C, dt):
 def test_row_counts(P, C):
     x, t = _inputs(P, C, seed=P, index=torch.int32)
     _check(x, t, top=3)
+
+
+@pytest.mark.parametrize("C", [1, 2, 3, 4, 5, 16, 21, 33, 64, 100, 127, 128, 150, 200, 255, 256, 257])
+def test_many_rows_of_few_labels(C):
+    """As many rows as an image has: odd and even row sizes on both sides of what a thread's tile takes, a
+    last tile that is not full, ties and masks among them."""
+    for k, dt in enumerate(TYPES):
+        x, t = _inputs(38007, C, dt, seed=C, masked=0.2, index=torch.int32 if k else torch.int64)
+        x[::3] = (x[::3] * 0.5).round()
+        x[1::997] = -math.inf
+        x[2::997] = 1.0
+        _check(x, t, top=(3, 7, 0)[(C + k) % 3], grads=("logp", "entropy", "top") if (C + k) % 3 < 2 else ("logp",))
+        if C in (21, 64, 150):
+            for top in (1, 2, 4, 16):
+                _check(x, t, top=top, grads=("logp",))
+
+
+def test_many_rows_bad_values():
+    from tt_splat_b200 import metrics
+    x, t = _inputs(40000, 20, unlabelled=0.0)
+    x[7, 3], x[8, 0], x[9, 19] = math.nan, math.inf, math.nan
+    t[9], t[10] = -1, 20
+    leaf = x.requires_grad_(True)
+    for top in (2, 6):
+        s = metrics.label_log_probs(leaf, t, top=top)
+        (g,) = torch.autograd.grad(s.logp, leaf, torch.ones(40000, device=DEV))
+        bad = torch.zeros(40000, dtype=torch.bool, device=DEV)
+        bad[7], bad[8], bad[10] = True, True, True
+        assert torch.equal(s.logp.isnan(), bad) and s.logp[9] == 0
+        assert torch.equal(g.isnan().all(1), bad) and torch.equal(g.isnan().any(1), bad) and (g[9] == 0).all()
+        assert (s.top_ids[7:10] == -1).all() and s.top_logp[7:10].isnan().all() and (s.top_ids[10:] >= 0).all()
 
 
 @pytest.mark.parametrize("P,C", [(1, 131072), (2, 65537), (5, 32000), (148, 16384), (300, 50257), (700, 9001)])

@@ -72,6 +72,25 @@ struct Soft {
   __device__ __forceinline__ bool bad() const { return !(m < CUDART_INF_F); }
 };
 
+// A whole row's sums by one thread: four of each in turn, which keeps the additions' roundings of a long row
+// down by as much and the chains of dependent additions short.
+struct Soft4 {
+  float m, S[4], A[4];
+  __device__ __forceinline__ void init() {
+    m = F_LOWEST;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) S[i] = A[i] = 0.f;
+  }
+  __device__ __forceinline__ void add(float x, int i) {
+    const float d = fmaxf(x - m, D_MIN), e = exp2_fast(d * LOG2E);
+    S[i] += e;
+    A[i] = fmaf(e, d, A[i]);
+  }
+  __device__ __forceinline__ Soft total() const {
+    return Soft{m, (S[0] + S[1]) + (S[2] + S[3]), (A[0] + A[1]) + (A[2] + A[3])};
+  }
+};
+
 struct ScoreArgs {
   const void* labels;
   float* logp;
@@ -124,7 +143,9 @@ struct RowSplit {
 };
 
 // ---- one block (or a cluster of blocks) per row: many labels -------------------------------------
-constexpr int SB_THREADS = 256;
+// TH threads: 256, or 128 for rows of up to BLOCK_FEW labels, where the steps behind the pass cost more than
+// the pass and more rows at once hide them (6434 x 12487 bf16: 61 instead of 82 us).
+constexpr long long BLOCK_FEW = 16384;
 constexpr int SB_CAND = 256;      // candidates for the alternatives held in shared memory
 constexpr int SB_CLUSTER = 8;
 
@@ -139,26 +160,27 @@ __device__ __forceinline__ bool before(float v, long long id, float w, long long
   return v > w || (v == w && id < jd);
 }
 
-// The `top` best labels of the block's part of the row, best first.  Threads are 8 to a group; the k-th
+// The `top` best labels of the block's part of the row, best first.  Threads form 32 groups; the k-th
 // largest of the 32 groups' maxima is a bound that at least k elements reach and few more (about 1.4 k
 // for distinct random values), and only threads whose own maximum reaches it hold any: their elements
 // alone are read again.  More candidates than fit (long runs of equal values): one pass for each
 // alternative.
-template <class T>
+template <class T, int TH>
 __device__ void block_top(const T* x, const RowSplit<T>& rs, long long lo, long long hi, bool ends, float tmax, int top,
                           BlockTop* out) {
   constexpr int N = Vec16<T>::E;
   __shared__ float s_g[32];
   __shared__ float s_T;
   __shared__ int s_nq, s_nc;
-  __shared__ unsigned char s_q[SB_THREADS];
+  __shared__ unsigned char s_q[TH];
   __shared__ float s_v[SB_CAND];
   __shared__ long long s_id[SB_CAND];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   float g = tmax;
+  constexpr int GROUP = TH / 32;
 #pragma unroll
-  for (int d = 4; d > 0; d >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, d));
-  if ((lane & 7) == 0) s_g[wid * 4 + (lane >> 3)] = g;
+  for (int d = GROUP / 2; d > 0; d >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, d));
+  if (lane % GROUP == 0) s_g[tid / GROUP] = g;
   if (tid == 0) s_nq = s_nc = 0;
   __syncthreads();
   if (wid == 0) {
@@ -181,12 +203,12 @@ __device__ void block_top(const T* x, const RowSplit<T>& rs, long long lo, long 
       }
     }
   };
-  const int rounds = (int)((hi - lo + SB_THREADS - 1) / SB_THREADS);
+  const int rounds = (int)((hi - lo + TH - 1) / TH);
   const long long work = (long long)s_nq * rounds;
   const uint4* xv = reinterpret_cast<const uint4*>(x + rs.head);
-  for (long long p = tid; p < work; p += SB_THREADS) {
+  for (long long p = tid; p < work; p += TH) {
     const int q = (int)(p / rounds);
-    const long long v = lo + s_q[q] + (p - (long long)q * rounds) * SB_THREADS;
+    const long long v = lo + s_q[q] + (p - (long long)q * rounds) * TH;
     if (v >= hi) continue;
     float w[N];
     Vec16<T>(__ldg(xv + v)).get(w);
@@ -199,9 +221,9 @@ __device__ void block_top(const T* x, const RowSplit<T>& rs, long long lo, long 
   __syncthreads();
   const int nc = s_nc;
   if (nc <= SB_CAND) {
-    if (tid < nc) {
-      const float v = s_v[tid];
-      const long long id = s_id[tid];
+    for (int c = tid; c < nc; c += TH) {
+      const float v = s_v[c];
+      const long long id = s_id[c];
       int rank = 0;
       for (int i = 0; i < nc; ++i) rank += before(s_v[i], s_id[i], v, id);
       if (rank < top) {
@@ -223,7 +245,7 @@ __device__ void block_top(const T* x, const RowSplit<T>& rs, long long lo, long 
       if (before(pv, pid, v, id) && v > bv) bv = v, bi = id;
     };
     if (ends && tid < rs.head) look(to_f32(x[tid]), tid);
-    for (long long v = lo + tid; v < hi; v += SB_THREADS) {
+    for (long long v = lo + tid; v < hi; v += TH) {
       float w[N];
       Vec16<T>(__ldg(xv + v)).get(w);
 #pragma unroll
@@ -240,7 +262,7 @@ __device__ void block_top(const T* x, const RowSplit<T>& rs, long long lo, long 
     if (lane == 0) s_v[wid] = bv, s_id[wid] = bi;
     __syncthreads();
     bv = s_v[0], bi = s_id[0];
-    for (int w = 1; w < SB_THREADS / 32; ++w)
+    for (int w = 1; w < TH / 32; ++w)
       if (s_id[w] >= 0 && (bi < 0 || before(s_v[w], s_id[w], bv, bi))) bv = s_v[w], bi = s_id[w];
     if (bi < 0) break;
     if (tid == 0) out->v[k] = bv, out->id[k] = bi;
@@ -254,11 +276,11 @@ __device__ void block_top(const T* x, const RowSplit<T>& rs, long long lo, long 
 // One pass over the row with each thread's own running maximum and sums (UNROLL vectors in flight), then
 // one merge; the blocks of a cluster take a part of the row each and the first one merges theirs through
 // distributed shared memory.
-template <class T>
-__global__ void __launch_bounds__(SB_THREADS, 4) k_scores_block(const T* __restrict__ logits, long long stride, int cs,
+template <class T, int TH>
+__global__ void __launch_bounds__(TH, 1024 / TH) k_scores_block(const T* __restrict__ logits, long long stride, int cs,
                                                                 ScoreArgs a) {
   constexpr int N = Vec16<T>::E, UNROLL = 4;
-  constexpr int WARPS = SB_THREADS / 32;
+  constexpr int WARPS = TH / 32;
   __shared__ Soft s_soft[WARPS > SB_CLUSTER ? WARPS : SB_CLUSTER];
   __shared__ Soft s_all;
   __shared__ BlockTop s_top;
@@ -284,19 +306,19 @@ __global__ void __launch_bounds__(SB_THREADS, 4) k_scores_block(const T* __restr
   Vec16<T> w[UNROLL], next[UNROLL];
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u)
-    if (lo + tid + u * SB_THREADS < hi) next[u].w = __ldg(xv + lo + tid + u * SB_THREADS);
-  for (long long v0 = lo + tid; v0 < hi; v0 += UNROLL * SB_THREADS) {
+    if (lo + tid + u * TH < hi) next[u].w = __ldg(xv + lo + tid + u * TH);
+  for (long long v0 = lo + tid; v0 < hi; v0 += UNROLL * TH) {
     // the next vectors are on their way while these are worked on
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       w[u] = next[u];
-      const long long v = v0 + (UNROLL + u) * SB_THREADS;
+      const long long v = v0 + (UNROLL + u) * TH;
       if (v < hi) next[u].w = __ldg(xv + v);
     }
     float m = s.m;
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
-      if (v0 + u * SB_THREADS < hi) {
+      if (v0 + u * TH < hi) {
         float f[N];
         w[u].get(f);
 #pragma unroll
@@ -305,7 +327,7 @@ __global__ void __launch_bounds__(SB_THREADS, 4) k_scores_block(const T* __restr
     if (!(m == s.m)) s.rebase(m);
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
-      if (v0 + u * SB_THREADS < hi) {
+      if (v0 + u * TH < hi) {
         float f[N];
         w[u].get(f);
 #pragma unroll
@@ -320,7 +342,7 @@ __global__ void __launch_bounds__(SB_THREADS, 4) k_scores_block(const T* __restr
   s = s_soft[lane % WARPS];
   s.reduce(WARPS);
   if (tid == 0) s_all = s;
-  if (a.top > 0 && !s.bad()) block_top<T>(x, rs, lo, hi, rank == 0, tmax, a.top, &s_top);
+  if (a.top > 0 && !s.bad()) block_top<T, TH>(x, rs, lo, hi, rank == 0, tmax, a.top, &s_top);
   if (cs == 1) {
     if (tid == 0) {
       const float2 st = write_scores(a, r, s, x, label);
@@ -453,8 +475,8 @@ __global__ void __launch_bounds__(128) k_scores_tile(const T* __restrict__ logit
   if (threadIdx.x >= rows) return;
   T* x = s + threadIdx.x * C;
   typename U::W* xu = reinterpret_cast<typename U::W*>(x);
-  Soft f;
-  f.init();
+  Soft4 sums;
+  sums.init();
   Best<K, TURN> best;
   best.init();
   TileWalk<TURN> w(units);
@@ -465,17 +487,29 @@ __global__ void __launch_bounds__(128) k_scores_tile(const T* __restrict__ logit
     U(xu[j]).get(v);
 #pragma unroll
     for (int e = 0; e < U::E; ++e) {
-      f.m = max_nan(f.m, v[e]);
+      sums.m = max_nan(sums.m, v[e]);
       best.add(v[e], j * U::E + e);
     }
   }
-#pragma unroll 4
-  for (int i = 0; i < units; ++i) {
+  constexpr int PER = 4 / U::E;
+  int i = 0;
+#pragma unroll 2
+  for (; i + PER <= units; i += PER) {
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+      float v[U::E];
+      U(xu[w.next(i + q)]).get(v);
+#pragma unroll
+      for (int e = 0; e < U::E; ++e) sums.add(v[e], q * U::E + e);
+    }
+  }
+  for (; i < units; ++i) {
     float v[U::E];
     U(xu[w.next(i)]).get(v);
 #pragma unroll
-    for (int e = 0; e < U::E; ++e) f.add(v[e]);
+    for (int e = 0; e < U::E; ++e) sums.add(v[e], e);
   }
+  const Soft f = sums.total();
   const float2 st = write_scores(a, r, f, x, label);
   if constexpr (K > 0) {
 #pragma unroll
@@ -697,8 +731,6 @@ __global__ void __launch_bounds__(GB_THREADS) k_scores_grad_block(const T* __res
   const long long r = blockIdx.x;
   const T* x = logits + r * stride;
   T* gx = glogits + r * a.C;
-  const RowGrad g(a, r, RowGrad::warp_tops(a, r));
-  const bool none = g.zero || g.empty;
   const RowSplit<T> rs(gx, a.C);
   const long long lo = blockIdx.y * steps * GB_STEP, hi = lo + steps * GB_STEP < rs.nv ? lo + steps * GB_STEP : rs.nv;
   const long long j0 = blockIdx.y == 0 ? 0 : rs.head + lo * N;
@@ -710,7 +742,7 @@ __global__ void __launch_bounds__(GB_THREADS) k_scores_grad_block(const T* __res
 #pragma unroll
     for (int u = 0; u < GB_UNROLL; ++u) {
       const long long v = v0 + u * GB_THREADS;
-      if (v < hi && !none) {
+      if (v < hi) {
         if constexpr (SAME) {
           next[u].w = __ldcs(xv + v);
         } else {
@@ -722,12 +754,15 @@ __global__ void __launch_bounds__(GB_THREADS) k_scores_grad_block(const T* __res
       }
     }
   };
+  // the first step's vectors and the row's numbers are on their way together
   fetch(lo + threadIdx.x);
+  const RowGrad g(a, r, RowGrad::warp_tops(a, r));
+  const bool none = g.zero || g.empty;
   for (long long v0 = lo + threadIdx.x; v0 < hi; v0 += GB_STEP) {
     Vec16<T> w[GB_UNROLL];
 #pragma unroll
     for (int u = 0; u < GB_UNROLL; ++u) w[u] = next[u];
-    fetch(v0 + GB_STEP);
+    if (!none) fetch(v0 + GB_STEP);
 #pragma unroll
     for (int u = 0; u < GB_UNROLL; ++u) {
       const long long v = v0 + u * GB_THREADS;
@@ -850,10 +885,13 @@ static int with_tile(long long C, F f) {
   return f(BT(), std::false_type());
 }
 
-// Rows of up to TILE_ROW_BYTES that lie one behind the other from a 16-byte boundary on take a thread each.
+// Rows of up to TILE_ROW_BYTES that lie one behind the other from a 16-byte boundary on take a thread each, from
+// TILE_ROWS rows on: fewer leave SMs idle that a warp for each row keeps busy (13938 x 60 fp16 top 4: 12 us by
+// tiles, 10 by warps).
 constexpr long long TILE_ROW_BYTES = 512;
-static bool tile_rows(long long C, size_t elem, long long stride, const void* x, const void* gx) {
-  return C * (long long)elem <= TILE_ROW_BYTES && stride == C && aligned16(x) && aligned16(gx);
+constexpr long long TILE_ROWS = 148 * 256;
+static bool tile_rows(long long P, long long C, size_t elem, long long stride, const void* x, const void* gx) {
+  return P >= TILE_ROWS && C * (long long)elem <= TILE_ROW_BYTES && stride == C && aligned16(x) && aligned16(gx);
 }
 static int tile_threads(long long C, size_t elem) { return C * (long long)elem <= 128 ? 128 : 64; }
 
@@ -872,7 +910,8 @@ static int launch_scores_block(const T* x, long long P, long long stride, const 
   while (cs < SB_CLUSTER && P * cs * 2 <= 148 * 4 && a.C / (cs * 2) >= 2048) cs *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(P * cs));
-  cfg.blockDim = dim3(SB_THREADS);
+  const bool few = a.C <= BLOCK_FEW && cs == 1;
+  cfg.blockDim = dim3(few ? 128 : 256);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -880,8 +919,9 @@ static int launch_scores_block(const T* x, long long P, long long stride, const 
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cs > 1 ? 1 : 0;
-  if (cudaLaunchKernelEx(&cfg, k_scores_block<T>, x, stride, cs, a) != cudaSuccess)
-    return check_launch("label_log_probs (block per row)");
+  const cudaError_t rc = few ? cudaLaunchKernelEx(&cfg, k_scores_block<T, 128>, x, stride, cs, a)
+                             : cudaLaunchKernelEx(&cfg, k_scores_block<T, 256>, x, stride, cs, a);
+  if (rc != cudaSuccess) return check_launch("label_log_probs (block per row)");
   return TTS_OK;
 }
 
@@ -901,7 +941,7 @@ extern "C" int tts_label_log_probs(const void* logits, long long P, long long C,
   return with_row_type(type, [&](auto t) {
     using T = decltype(t);
     const T* x = static_cast<const T*>(logits);
-    if (tile_rows(C, sizeof(T), row_stride, x, nullptr)) {
+    if (tile_rows(P, C, sizeof(T), row_stride, x, nullptr)) {
       const int n = tile_threads(C, sizeof(T));
       const size_t bytes = (size_t)n * C * sizeof(T);
       const unsigned grid = (unsigned)((P + n - 1) / n);
@@ -950,7 +990,7 @@ extern "C" int tts_label_log_probs_bwd(const void* logits, long long P, long lon
     using T = decltype(t);
     const T* x = static_cast<const T*>(logits);
     T* gx = static_cast<T*>(glogits);
-    if (tile_rows(C, sizeof(T), row_stride, x, gx)) {
+    if (tile_rows(P, C, sizeof(T), row_stride, x, gx)) {
       const int n = tile_threads(C, sizeof(T));
       const size_t bytes = (size_t)n * C * sizeof(T);
       const unsigned grid = (unsigned)((P + n - 1) / n);
