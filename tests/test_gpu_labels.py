@@ -3,8 +3,9 @@ against float64, at the sizes and masks where they can go wrong.
 
 Tolerances, with u = 2^-24: d = x - m is off by u |d|; exp of it, computed as 2^(d log2 e), by |d| u for
 the product, 2^-22 = 4u for the power and u |d| for d, together (2|d| + 4) u relative, so the sum S by
-e_S = u (2 D + 4 + n) with D = sum p |d| and n = ceil(C / 32) + 16 additions on the longest path of a
-sum.  From there:
+e_S = u (2 D + 4 + n) with D = sum p |d| and n additions on the longest path of a sum: ceil(C / 32) + 16
+where a warp or a block shares a row; C / 4 + 6 where one thread takes a row of up to 256 labels in four
+sums (up to 3 labels more in one, and 3 additions of the sums).  From there:
 * log S: e_S + 4u (1 + log S);  log p_j: u |d_j| + that + u |log p_j|;
 * A / S with A = sum e d: u sum p |d| (2|d| + 5 + n) + e_S D, and H adds the error of log S and u H;
 * p_j: relative, the error of log p_j + (|log p_j| + 4) u;
