@@ -146,6 +146,41 @@ def test_many_rows_of_few_labels(C):
                 _check(x, t, top=top, grads=("logp",))
 
 
+@pytest.mark.parametrize("P,C", [(1801, 1025), (1776, 1500), (2000, 2048), (1900, 4095), (1777, 4096), (1800, 4097)])
+def test_many_rows_of_some_thousand_labels(P, C):
+    """Both sides of what a warp takes for itself, with ties, masks, bad and empty rows, and rows that start at
+    every offset from a 16-byte boundary, their gradients' offset another one too."""
+    from tt_splat_b200 import metrics
+    for k, dt in enumerate(TYPES):
+        x, t = _inputs(P, C, dt, seed=C + k, masked=0.3 * k)
+        x[::3] = (x[::3] * 0.5).round()
+        x[1::97] = -math.inf
+        x[2::97] = 1.0
+        x[4::97, C // 2:] = 9.0
+        x[5::97] = torch.finfo(dt).min
+        _check(x, t, top=(8, 16, 1)[k])
+        wide = torch.randn(P, C + 5, device=DEV).to(dt)
+        wide[:, 1:-4] = x
+        leaf = wide[:, 1:-4].detach().requires_grad_(True)
+        s, q = metrics.label_log_probs(leaf, t, top=3), metrics.label_log_probs(x, t, top=3)
+        tol = 2 * _reference(x, t, 0)["elp"].gather(1, t.clamp(min=0)[:, None])[:, 0]
+        assert torch.equal(s.top_ids, q.top_ids) and _close(s.logp.detach(), q.logp.double(), tol)
+        (g,) = torch.autograd.grad(s.logp, leaf, torch.ones(P, device=DEV))
+        y = x.detach().requires_grad_(True)
+        (h,) = torch.autograd.grad(metrics.label_log_probs(y, t).logp, y, torch.ones(P, device=DEV))
+        # each is within its bound of the exact one, at most (5 |log p| + n + 30) u of p on each side, and rounded
+        p = _reference(x, t, 0)["p"]
+        far = (p * (5 * 80 + C / 32 + 60) * 2 * U + 2 * torch.finfo(dt).eps / 2 * h.double().abs() + 2.0 ** -24)
+        assert ((g.double() - h.double()).abs() <= far).all()
+        z = x.clone()
+        z[7, C - 1], z[8, 0], z[9, 5] = math.nan, math.inf, math.nan
+        t[7], t[8], t[9], t[11] = 0, 0, -1, C
+        s = metrics.label_log_probs(z.requires_grad_(True), t, top=2)
+        (g,) = torch.autograd.grad(s.logp, z, torch.ones(P, device=DEV))
+        assert s.logp[7:9].isnan().all() and s.logp[9] == 0 and s.logp[11].isnan() and s.entropy[7:10].isnan().all()
+        assert (s.top_ids[7:10] == -1).all() and g[7:9].isnan().all() and (g[9] == 0).all() and g[11].isnan().all()
+
+
 def test_many_rows_bad_values():
     from tt_splat_b200 import metrics
     x, t = _inputs(40000, 20, unlabelled=0.0)

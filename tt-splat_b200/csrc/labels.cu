@@ -552,6 +552,36 @@ __device__ __forceinline__ float order_value(unsigned k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
+// The k-th largest of the lanes' numbers.
+__device__ __forceinline__ float kth_of_lanes(float mine, int k) {
+  unsigned key = order_key(mine), kth = 0;
+  for (int i = 0; i < k; ++i) {
+    kth = __reduce_max_sync(0xffffffffu, key);
+    if ((threadIdx.x & 31) == __ffs(__ballot_sync(0xffffffffu, key == kth)) - 1) key = 0;
+  }
+  return order_value(kth);
+}
+// Writes the row's alternatives from n <= 32 candidates that hold them, a lane for each.
+__device__ __forceinline__ void place_candidates(const ScoreArgs& a, long long r, int n, const float* v, const int* id,
+                                                 float2 st) {
+  const int lane = threadIdx.x & 31;
+  if (lane < n) {
+    int place = 0;
+    for (int i = 0; i < n; ++i) place += before(v[i], id[i], v[lane], id[lane]);
+    if (place < a.top) write_top(a, r, place, v[lane], id[lane], st);
+  }
+  if (lane >= n && lane < a.top) write_top(a, r, lane, 0.f, -1, st);
+}
+// The best of the lanes' labels, in all of them.
+__device__ __forceinline__ void best_of_lanes(float& v, int& id) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    const float ov = __shfl_xor_sync(0xffffffffu, v, d);
+    const int oi = __shfl_xor_sync(0xffffffffu, id, d);
+    if (before(ov, oi, v, id)) v = ov, id = oi;
+  }
+}
+
 template <class T, int SLOTS>
 __global__ void __launch_bounds__(256) k_scores_warp(const T* __restrict__ logits, long long P, long long stride,
                                                      ScoreArgs a) {
@@ -591,12 +621,7 @@ __global__ void __launch_bounds__(256) k_scores_warp(const T* __restrict__ logit
     if (lane < a.top) write_top(a, r, lane, 0.f, -1, st);
     return;
   }
-  unsigned key = order_key(most), kth = 0;
-  for (int k = 0; k < a.top; ++k) {
-    kth = __reduce_max_sync(0xffffffffu, key);
-    if (lane == __ffs(__ballot_sync(0xffffffffu, key == kth)) - 1) key = 0;
-  }
-  const float bound = order_value(kth);
+  const float bound = kth_of_lanes(most, a.top);
   int n = 0;
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i) {
@@ -613,14 +638,7 @@ __global__ void __launch_bounds__(256) k_scores_warp(const T* __restrict__ logit
   }
   __syncwarp();
   if (n <= 32) {
-    if (lane < n) {
-      const float w = s_v[wid][lane];
-      const int id = s_id[wid][lane];
-      int place = 0;
-      for (int i = 0; i < n; ++i) place += before(s_v[wid][i], s_id[wid][i], w, id);
-      if (place < a.top) write_top(a, r, place, w, id, st);
-    }
-    if (lane >= n && lane < a.top) write_top(a, r, lane, 0.f, -1, st);
+    place_candidates(a, r, n, s_v[wid], s_id[wid], st);
     return;
   }
   float pv = CUDART_INF_F;
@@ -631,13 +649,117 @@ __global__ void __launch_bounds__(256) k_scores_warp(const T* __restrict__ logit
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i)
       if (before(pv, pid, v[i], i * 32 + lane) && v[i] > bv) bv = v[i], bi = i * 32 + lane;
+    best_of_lanes(bv, bi);
+    if (lane == 0) write_top(a, r, k, bv, bi < C ? bi : -1, st);
+    pv = bv;
+    pid = bi;
+  }
+}
+
+// Longer rows of a warp stay in memory: one pass with each lane's own running sums, then the lanes whose maximum
+// reaches the bound read theirs again (from a cache, mostly) for the candidates.
+// Rows of up to 4096 labels where there are enough to keep the SMs busy; longer or fewer ones take a block each
+// (20000 x 1100 fp16 top 8: 34 us, 99 by blocks; 4000 x 8000 fp32: 47 and 35; 1200 x 2000 fp32: 9 and 8).
+constexpr long long WARP_LONG_MAX = 4096;
+constexpr long long WARP_LONG_ROWS = 148 * 12;
+
+template <class T>
+__global__ void __launch_bounds__(256, 4) k_scores_warp_long(const T* __restrict__ logits, long long P, long long stride,
+                                                             ScoreArgs a) {
+  constexpr int N = Vec16<T>::E, UNROLL = 4;
+  __shared__ float s_v[8][32];
+  __shared__ int s_id[8][32], s_n[8];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const long long r = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  if (r >= P) return;
+  const T* x = logits + r * stride;
+  const RowSplit<T> rs(x, a.C);
+  const int nv = (int)rs.nv, t0 = rs.head + nv * N;
+  const uint4* xv = reinterpret_cast<const uint4*>(x + rs.head);
+  const long long label = load_index(a.labels, a.labels64, r);
+  const float h = lane < rs.head ? to_f32(x[lane]) : -CUDART_INF_F;
+  const float t = lane < rs.tail ? to_f32(x[t0 + lane]) : -CUDART_INF_F;
+  Soft s;
+  s.init();
+  s.m = max_nan(s.m, max_nan(h, t));
+  s.add(h);
+  s.add(t);
+  for (int v0 = lane; v0 < nv; v0 += 32 * UNROLL) {
+    Vec16<T> w[UNROLL];
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-      const float ov = __shfl_xor_sync(0xffffffffu, bv, d);
-      const int oi = __shfl_xor_sync(0xffffffffu, bi, d);
-      if (before(ov, oi, bv, bi)) bv = ov, bi = oi;
+    for (int u = 0; u < UNROLL; ++u)
+      if (v0 + 32 * u < nv) w[u].w = __ldg(xv + v0 + 32 * u);
+    float m = s.m;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (v0 + 32 * u < nv) {
+        float f[N];
+        w[u].get(f);
+#pragma unroll
+        for (int e = 0; e < N; ++e) m = max_nan(m, f[e]);
+      }
+    if (!(m == s.m)) s.rebase(m);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (v0 + 32 * u < nv) {
+        float f[N];
+        w[u].get(f);
+#pragma unroll
+        for (int e = 0; e < N; ++e) s.add(f[e]);
+      }
+  }
+  const float most = s.m;
+  s.reduce(32);
+  float2 st;
+  if (lane == 0) st = write_scores(a, r, s, x, label);
+  if (a.top == 0) return;
+  st.x = __shfl_sync(0xffffffffu, st.x, 0);
+  st.y = __shfl_sync(0xffffffffu, st.y, 0);
+  if (s.bad()) {
+    if (lane < a.top) write_top(a, r, lane, 0.f, -1, st);
+    return;
+  }
+  const float bound = kth_of_lanes(most, a.top);
+  if (lane == 0) s_n[wid] = 0;
+  __syncwarp();
+  auto each = [&](auto look) {
+    if (lane < rs.head) look(h, lane);
+#pragma unroll 2
+    for (int v = lane; v < nv; v += 32) {
+      float f[N];
+      Vec16<T>(__ldg(xv + v)).get(f);
+#pragma unroll
+      for (int e = 0; e < N; ++e) look(f[e], rs.head + v * N + e);
     }
-    if (lane == 0) write_top(a, r, k, bv, bi, st);
+    if (lane < rs.tail) look(t, t0 + lane);
+  };
+  // (the bound is at least the lowest number: masked labels are below)
+  if (most >= bound)
+    each([&](float v, int id) {
+      if (v >= bound) {
+        const int at = atomicAdd(&s_n[wid], 1);
+        if (at < 32) {
+          s_v[wid][at] = v;
+          s_id[wid][at] = id;
+        }
+      }
+    });
+  __syncwarp();
+  const int n = s_n[wid];
+  if (n <= 32) {
+    place_candidates(a, r, n, s_v[wid], s_id[wid], st);
+    return;
+  }
+  float pv = CUDART_INF_F;
+  int pid = -1;
+  for (int k = 0; k < a.top; ++k) {
+    float bv = -CUDART_INF_F;
+    int bi = (int)a.C;
+    each([&](float v, int id) {
+      if (before(pv, pid, v, id) && v > bv) bv = v, bi = id;
+    });
+    best_of_lanes(bv, bi);
+    if (lane == 0) write_top(a, r, k, bv, bi < a.C ? bi : -1, st);
     pv = bv;
     pid = bi;
   }
@@ -789,18 +911,45 @@ __global__ void __launch_bounds__(GB_THREADS) k_scores_grad_block(const T* __res
   }
 }
 
-template <class T>
+// A warp for each row, in 16-byte units where the logits' line up with the gradient's.
+template <class T, bool SAME>
 __global__ void __launch_bounds__(256) k_scores_grad_warp(const T* __restrict__ logits, long long P, long long stride,
                                                           GradArgs a, T* __restrict__ glogits) {
+  constexpr int N = Vec16<T>::E, UNROLL = 4;
   const int lane = threadIdx.x & 31;
   const long long r = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   if (r >= P) return;
   const T* x = logits + r * stride;
   T* gx = glogits + r * a.C;
+  const int C = (int)a.C;
   const RowGrad g(a, r, RowGrad::warp_tops(a, r));
   const bool none = g.zero || g.empty;
-  const int C = (int)a.C;
-  for (int j = lane; j < C; j += 32) gx[j] = from_f32<T>(none ? 0.f : g(to_f32(x[j])));
+  if constexpr (SAME) {
+    const RowSplit<T> rs(gx, C);
+    const int nv = (int)rs.nv, t0 = rs.head + nv * N;
+    const uint4* xv = reinterpret_cast<const uint4*>(x + rs.head);
+    uint4* gv = reinterpret_cast<uint4*>(gx + rs.head);
+    for (int v0 = lane; v0 < nv; v0 += 32 * UNROLL) {
+      Vec16<T> w[UNROLL];
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u)
+        if (v0 + 32 * u < nv && !none) w[u].w = __ldg(xv + v0 + 32 * u);
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u)
+        if (v0 + 32 * u < nv) {
+          float f[N];
+          w[u].get(f);
+#pragma unroll
+          for (int e = 0; e < N; ++e) f[e] = none ? 0.f : g(f[e]);
+          w[u].set(f);
+          gv[v0 + 32 * u] = w[u].w;
+        }
+    }
+    if (lane < rs.head) gx[lane] = from_f32<T>(none ? 0.f : g(to_f32(x[lane])));
+    if (lane < rs.tail) gx[t0 + lane] = from_f32<T>(none ? 0.f : g(to_f32(x[t0 + lane])));
+  } else {
+    for (int j = lane; j < C; j += 32) gx[j] = from_f32<T>(none ? 0.f : g(to_f32(x[j])));
+  }
   __syncwarp();
   if (lane <= (a.g_top ? a.top : 0)) {
     const long long j = lane == 0 ? g.t : a.top_ids[r * a.top + lane - 1];
@@ -968,6 +1117,8 @@ extern "C" int tts_label_log_probs(const void* logits, long long P, long long C,
         k_scores_warp<T, 16><<<grid, 256, 0, as_stream(stream)>>>(x, P, row_stride, a);
       else
         k_scores_warp<T, 32><<<grid, 256, 0, as_stream(stream)>>>(x, P, row_stride, a);
+    } else if (C <= WARP_LONG_MAX && P >= WARP_LONG_ROWS) {
+      k_scores_warp_long<T><<<(unsigned)((P + 7) / 8), 256, 0, as_stream(stream)>>>(x, P, row_stride, a);
     } else if (int rc = launch_scores_block<T>(x, P, row_stride, a, as_stream(stream))) {
       return rc;
     }
@@ -998,12 +1149,18 @@ extern "C" int tts_label_log_probs_bwd(const void* logits, long long P, long lon
         k_scores_grad_tile<T, decltype(vb)::value, decltype(turn)::value><<<grid, n, bytes, st>>>(x, P, a, gx);
         return TTS_OK;
       });
-    } else if (C <= WARP_ROW_MAX) {
-      k_scores_grad_warp<T><<<(unsigned)((P + 7) / 8), 256, 0, st>>>(x, P, row_stride, a, gx);
     } else {
       // the logits' 16-byte vectors line up with the gradient's when both start on the same offset in every row
       const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(gx)) & 15u) == 0 &&
                         (row_stride - C) * (long long)sizeof(T) % 16 == 0;
+      if (C <= WARP_ROW_MAX || (C <= WARP_LONG_MAX && P >= WARP_LONG_ROWS)) {
+        const unsigned grid = (unsigned)((P + 7) / 8);
+        if (same)
+          k_scores_grad_warp<T, true><<<grid, 256, 0, st>>>(x, P, row_stride, a, gx);
+        else
+          k_scores_grad_warp<T, false><<<grid, 256, 0, st>>>(x, P, row_stride, a, gx);
+        return check_launch("label_log_probs_bwd");
+      }
       // a few steps to a block where that leaves blocks enough for the SMs
       const long long parts = (C / Vec16<T>::E + GB_STEP - 1) / GB_STEP;
       int steps = 1;
