@@ -137,6 +137,55 @@ def test_shapes_of_tables_and_indices():
     assert torch.equal(binned.gather_rows(t, i.transpose(0, 2)), t[i.transpose(0, 2)])
 
 
+@pytest.mark.parametrize("rows,index", [((30,), (4, 8)), ((30,), (30, 1)), ((30, 1), (5, 3)), ((30, 2, 3), (7,)), ((30, 15, 3), (2, 4, 8)),
+                                        ((30, 6), ()), ((30,), ()), ((30, 4), (20, 500))])
+def test_gradients_of_any_shape(rows, index):
+    """Against index_add in float64 of flattened rows, (n + 3) u sum|g| for a row of n uses."""
+    from tt_splat_b200 import binned
+    t = torch.randn(rows, device=DEV, requires_grad=True)
+    i = torch.randint(0, 30, index, device=DEV)
+    out = binned.gather_rows(t, i)
+    assert out.shape == (*index, *rows[1:]) and torch.equal(out, t.detach()[i])
+    gout = torch.randn(out.shape, device=DEV)
+    (g,) = torch.autograd.grad(out, t, gout)
+    n = i.numel()
+    add = lambda y: torch.zeros(30, t[0].numel(), dtype=torch.float64, device=DEV).index_add_(  # noqa: E731
+        0, i.reshape(-1), y.double().reshape(n, -1))
+    uses = torch.bincount(i.reshape(-1), minlength=30)[:, None]
+    assert g.shape == t.shape
+    assert ((g.double().reshape(30, -1) - add(gout)).abs() <= (uses + 3) * U * add(gout.abs())).all()
+
+
+@pytest.mark.parametrize("N", [500, 50000])
+@pytest.mark.parametrize("C", [5, 64, 3001])
+def test_one_gradient_alone(N, C):
+    """Only the table, or only the weights, ask for a gradient: as when both do, up to the order in which the
+    terms are added ((n + 3) u sum|f g| of a row's n uses and (C + 3) u sum|g t|, on each side)."""
+    from tt_splat_b200 import binned
+    x = _inputs(40, C, (N,), seed=C)
+    _, (gt, gw) = _check(x)
+    t = x["table"].detach().requires_grad_(True)
+    (g,) = torch.autograd.grad(binned.gather_rows(t, x["idx"], x["valid"], x["weight"]), t, x["gout"])
+    use = (x["idx"] >= 0) & x["valid"]
+    term = (x["weight"][use, None].double() * x["gout"][use].double()).abs()
+    mag = torch.zeros(40, C, dtype=torch.float64, device=DEV).index_add_(0, x["idx"][use], term)
+    uses = torch.bincount(x["idx"][use], minlength=40)[:, None]
+    assert ((g.double() - gt.double()).abs() <= 2 * (uses + 3) * U * mag).all()
+    w = x["weight"].detach().requires_grad_(True)
+    (g,) = torch.autograd.grad(binned.gather_rows(x["table"], x["idx"], x["valid"], w), w, x["gout"])
+    tab = x["table"].double()[x["idx"].clamp(min=0)]
+    assert ((g.double() - gw.double()).abs() <= 2 * (C + 3) * U * (tab * x["gout"].double()).abs().sum(1)).all()
+
+
+def test_many_unused():
+    """Nothing, or a single slot, of many looked up: every row is written all the same."""
+    x = _inputs(70001, 3, (20000,), unused=0.0)
+    x["valid"][:] = False
+    _check(x)
+    x["valid"][12345] = True
+    _check(x)
+
+
 @pytest.mark.parametrize("dt", TYPES)
 def test_strided_tables_and_gradients(dt):
     """Columns of a wider table, an offset that breaks 16-byte alignment, and gradients that arrive as a

@@ -61,7 +61,7 @@ T* ptr(const Tensor& t) {
 // [n, width] view of a tensor's rows with unit stride along them (the kernels take any distance between rows
 // below 2^30, an expanded row's included); a copy where no such view exists.
 Tensor rows2d(const Tensor& t, int64_t n, int64_t width) {
-  const Tensor r = t.dim() == 2 ? t : t.reshape({n, width});
+  const Tensor r = t.dim() == 2 && t.size(0) == n && t.size(1) == width ? t : t.reshape({n, width});
   return (width <= 1 || r.stride(1) == 1) && (n <= 1 || r.stride(0) < (1ll << 30)) ? r : r.contiguous();
 }
 int64_t row_stride(const Tensor& rows) { return rows.size(0) <= 1 ? rows.size(1) : rows.stride(0); }
