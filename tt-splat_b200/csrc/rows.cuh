@@ -55,6 +55,7 @@ inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 // Entries (row, use) sorted by row, equal rows in the order of their uses; unused and out-of-range slots are
 // left out.
 constexpr long long SORT_SMALL = 8192;      // uses up to which one block sorts them in shared memory
+constexpr long long FEW_USES = 4;            // rows for a use from which on the gradient is cleared as a whole
 
 struct SortSpace {
   unsigned* n;         // entries in `sorted`
@@ -62,13 +63,13 @@ struct SortSpace {
   uint2* other;        // [N] the pass before the last (large sorts, as the rest)
   unsigned* counts;    // digit counts of each tile
   unsigned* totals;    // digit counts
-  uint8_t* used;       // [R] flags for the rows that are looked up, cleared
+  uint8_t* used;       // [R] flags for the rows that are looked up, cleared; NULL with few uses for the rows
 };
 
 size_t sort_space(long long N, long long R, void* base, SortSpace* s);
 // Launches the sort, which also clears the weights' gradients (or NULL) of slots that look nothing up.  Up to
-// SORT_SMALL uses it clears the `clear_bytes` at `clear` (the whole gradient); beyond, it clears the `used`
-// flags instead, for the caller to find the rows without a use.
+// SORT_SMALL uses, and where most rows have none, it clears the `clear_bytes` at `clear` (the whole gradient);
+// else the `used` flags, for the caller to find the rows without a use.
 int sort_uses(const RowUses& u, const SortSpace& s, void* clear, size_t clear_bytes, float* gweight, cudaStream_t st);
 
 // ---- the sums over the sorted uses ---------------------------------------------------------------

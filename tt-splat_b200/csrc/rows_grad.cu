@@ -98,11 +98,11 @@ __device__ __forceinline__ float sum8(float (&v)[8], int gl, int lanes, unsigned
 }
 
 template <class T, int VB, int PL, bool GW>
-__global__ void __launch_bounds__(GT, PL * VB <= (GW ? 8 : 16) ? 3 : 1) k_rows_grad(GradArgs a, const T* __restrict__ table, const T* __restrict__ gout,
+__global__ void __launch_bounds__(GT, PL * VB <= (GW ? 8 : 16) ? 3 : (PL * VB <= 32 ? 2 : 1)) k_rows_grad(GradArgs a, const T* __restrict__ table, const T* __restrict__ gout,
                                                   T* __restrict__ gtable) {
   using U = Unit<T, VB>;
   using W = typename U::W;
-  constexpr int E = U::E, UN = PL * VB > 32 ? 4 : 8;
+  constexpr int E = U::E, UN = PL * VB > (GW ? 16 : 32) ? 4 : 8;
   constexpr int SPAN = BLOCK_USES + 2 * L_MAX + 2;
   __shared__ unsigned s_key[SPAN], s_use[SPAN];
   __shared__ float s_f[SPAN];
@@ -329,15 +329,17 @@ __device__ __forceinline__ void zero_rows(const GradArgs& a, void* gtable, long 
 constexpr int JOIN_TEST = 8;        // chunks of a warp
 
 template <class T>
-__global__ void __launch_bounds__(GT, 5) k_rows_join(GradArgs a, int lanes, unsigned join_blocks, T* __restrict__ gtable) {
+__global__ void __launch_bounds__(GT, 5) k_rows_join(GradArgs a, int lanes, unsigned test_blocks, unsigned parts,
+                                                     T* __restrict__ gtable) {
   __shared__ JoinItem s_many[JOIN_TEST * JOIN_WARPS];
   __shared__ int s_n;
   __shared__ float s_sum[JOIN_WARPS][32];
   const long long N = *a.n, C = a.C, L = a.L;
   const unsigned R = (unsigned)a.u.R;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  // test_blocks blocks for each of the column parts, then those for the unused rows
+  const unsigned join_blocks = test_blocks * parts, block = blockIdx.x % test_blocks, part = blockIdx.x / test_blocks;
   if (blockIdx.x >= join_blocks) {
-    if (blockIdx.y > 0) return;
     if (a.unit == 16)
       zero_rows<uint4>(a, gtable, blockIdx.x - join_blocks, gridDim.x - join_blocks);
     else if (a.unit == 4)
@@ -348,7 +350,7 @@ __global__ void __launch_bounds__(GT, 5) k_rows_join(GradArgs a, int lanes, unsi
   }
   if (threadIdx.x == 0) s_n = 0;
   __syncthreads();
-  const long long chunk = ((long long)blockIdx.x * JOIN_WARPS + wid) * JOIN_TEST + lane;
+  const long long chunk = ((long long)block * JOIN_WARPS + wid) * JOIN_TEST + lane;
   JoinItem it{0, 0, 0};
   bool found = false;
   if (lane < JOIN_TEST && chunk * L < N) {
@@ -357,7 +359,7 @@ __global__ void __launch_bounds__(GT, 5) k_rows_join(GradArgs a, int lanes, unsi
     it = JoinItem{chunk, c.i1 + L, c.last};      // (the last use: not before there)
   }
   const int nq = 32 / lanes, q = lane / lanes, gl = lane % lanes;
-  const long long c0 = (long long)blockIdx.y * lanes, cstep = (long long)gridDim.y * lanes;
+  const long long c0 = (long long)part * lanes, cstep = (long long)parts * lanes;
   unsigned todo = __ballot_sync(0xffffffffu, found);
   while (todo) {
     const int src = __ffs(todo) - 1;
@@ -475,10 +477,9 @@ int rows_grad(const RowUses& u, const SortSpace& s, const void* table, long long
       int lanes = 1;
       while (lanes < 32 && lanes < C) lanes *= 2;
       const long long cols = (C + lanes - 1) / lanes, per = JOIN_TEST * JOIN_WARPS;
-      const unsigned jb = (unsigned)((a.chunks + per - 1) / per);
-      const long long rows = a.used ? (u.R * g.lanes + 4 * GT - 1) / (4 * GT) : 0;
-      const dim3 jg(jb + (unsigned)(rows < 148 * 8 ? rows : 148 * 8), (unsigned)(cols < 32 ? cols : 32));
-      k_rows_join<T><<<jg, GT, 0, st>>>(a, lanes, jb, gt);
+      const unsigned tests = (unsigned)((a.chunks + per - 1) / per), jp = (unsigned)(cols < 32 ? cols : 32);
+      const long long zero = a.used ? (u.R * g.lanes + 4 * GT - 1) / (4 * GT) : 0;
+      k_rows_join<T><<<tests * jp + (unsigned)(zero < 148 * 8 ? zero : 148 * 8), GT, 0, st>>>(a, lanes, tests, jp, gt);
     }
     return check_launch("row gradient");
   });

@@ -375,8 +375,10 @@ size_t sort_space(long long N, long long R, void* base, SortSpace* s) {
     p += align256((size_t)tiles_of(N) * (1 << dg.bits) * sizeof(unsigned));
     t.totals = reinterpret_cast<unsigned*>(p);
     p += align256((size_t)MAX_DIGITS * sizeof(unsigned));
-    t.used = reinterpret_cast<uint8_t*>(p);
-    p += align256((size_t)R);
+    if (N > R / FEW_USES) {
+      t.used = reinterpret_cast<uint8_t*>(p);
+      p += align256((size_t)R);
+    }
   }
   if (s) *s = t;
   return (size_t)(p - static_cast<char*>(base));
@@ -394,6 +396,7 @@ int sort_uses(const RowUses& u, const SortSpace& s, void* clear, size_t clear_by
                                                                     gweight);
     return check_launch("sort of the uses");
   }
+  if (!s.used && cudaMemsetAsync(clear, 0, clear_bytes, st) != cudaSuccess) return check_launch("memset of the gradient");
   const Digits dg = digits_for(u.R, MAX_BITS);
   const unsigned tiles = (unsigned)tiles_of(u.N);
   const int D = 1 << dg.bits;
