@@ -303,22 +303,11 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_scores_block(const T* __restr
     s.add(h);
     s.add(t);
   }
-  Vec16<T> w[UNROLL], next[UNROLL];
-#pragma unroll
-  for (int u = 0; u < UNROLL; ++u)
-    if (lo + tid + u * TH < hi) next[u].w = __ldg(xv + lo + tid + u * TH);
-  for (long long v0 = lo + tid; v0 < hi; v0 += UNROLL * TH) {
-    // the next vectors are on their way while these are worked on
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      w[u] = next[u];
-      const long long v = v0 + (UNROLL + u) * TH;
-      if (v < hi) next[u].w = __ldg(xv + v);
-    }
+  auto take = [&](const Vec16<T>(&w)[UNROLL], int n) {
     float m = s.m;
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
-      if (v0 + u * TH < hi) {
+      if (u < n) {
         float f[N];
         w[u].get(f);
 #pragma unroll
@@ -327,12 +316,41 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_scores_block(const T* __restr
     if (!(m == s.m)) s.rebase(m);
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
-      if (v0 + u * TH < hi) {
+      if (u < n) {
         float f[N];
         w[u].get(f);
 #pragma unroll
         for (int e = 0; e < N; ++e) s.add(f[e]);
       }
+  };
+  constexpr int STEP = UNROLL * TH;
+  const uint4* at = xv + lo + tid;
+  int left = (int)(hi - lo) - tid;      // vectors from this thread's next one on, its own every TH-th of them
+  Vec16<T> w[UNROLL], next[UNROLL];
+  if (left > (UNROLL - 1) * TH) {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) next[u].w = __ldg(at + u * TH);
+    while (left > STEP + (UNROLL - 1) * TH) {
+      // the next vectors are on their way while these are worked on
+      at += STEP;
+      left -= STEP;
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        w[u] = next[u];
+        next[u].w = __ldg(at + u * TH);
+      }
+      take(w, UNROLL);
+    }
+    take(next, UNROLL);
+    at += STEP;
+    left -= STEP;
+  }
+  if (left > 0) {
+    const int n = (left + TH - 1) / TH;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (u < n) w[u].w = __ldg(at + u * TH);
+    take(w, n);
   }
   const float tmax = s.m;
   s.reduce(32);
