@@ -98,8 +98,8 @@ __device__ __forceinline__ float sum8(float (&v)[8], int gl, int lanes, unsigned
 }
 
 template <class T, int VB, int PL, bool GW>
-__global__ void __launch_bounds__(GT, PL * VB <= (GW ? 8 : 16) ? 3 : (PL * VB <= 32 ? 2 : 1)) k_rows_grad(GradArgs a, const T* __restrict__ table, const T* __restrict__ gout,
-                                                  T* __restrict__ gtable) {
+__global__ void __launch_bounds__(GT, PL * VB <= (GW ? 8 : 16) ? 3 : (PL * VB <= 32 ? 2 : 1))
+    k_rows_grad(GradArgs a, const T* __restrict__ table, const T* __restrict__ gout, T* __restrict__ gtable) {
   using U = Unit<T, VB>;
   using W = typename U::W;
   constexpr int E = U::E, UN = PL * VB > (GW ? 16 : 32) ? 4 : 8;
