@@ -272,6 +272,18 @@ def test_nan_infinite_and_bad_labels(C):
     assert (g[:5] == 0).all()
 
 
+@pytest.mark.parametrize("P,C", [(8, 5), (8, 150), (8, 3001), (40000, 21)])
+def test_bad_labels_left_out_of_the_loss(P, C):
+    """A label past the last whose log probability does not reach the loss leaves its row's gradient zero."""
+    from tt_splat_b200 import metrics
+    x, t = _inputs(P, C, seed=3, unlabelled=0.0)
+    t[2], t[5] = C, 2 ** 31 - 1
+    leaf = x.requires_grad_(True)
+    s = metrics.label_log_probs(leaf, t)
+    (g,) = torch.autograd.grad(torch.where(t < C, s.logp, 0.0).sum(), leaf)
+    assert (g[2] == 0).all() and (g[5] == 0).all() and torch.isfinite(g).all() and (g[:2] != 0).any(1).all()
+
+
 @pytest.mark.parametrize("grads", [("logp",), ("entropy",), ("top",), ("logp", "top")])
 @pytest.mark.parametrize("C", [11, 300, 12000])
 def test_each_gradient_alone(grads, C):

@@ -832,7 +832,10 @@ struct RowGrad {
     gh = a.g_entropy ? a.g_entropy[r] : 0.f;
     t = load_index(a.labels, a.labels64, r);
     gl = 0.f;
-    if (a.g_logp && t >= 0) gl = t < a.C ? a.g_logp[r] : CUDART_NAN_F;
+    if (a.g_logp && t >= 0) {
+      gl = a.g_logp[r];
+      if (t >= a.C && gl != 0.f) gl = CUDART_NAN_F;
+    }
     const float total = gl + of_tops;
     m = st.x;
     c = -st.y * LOG2E;
