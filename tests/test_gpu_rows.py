@@ -82,6 +82,12 @@ def test_widths(C, dt):
     _check(_inputs(37, C, (129,), dt, seed=C), scale=0.75)
 
 
+def test_the_widest_rows():
+    """A width with more column parts of one unit a lane than a grid has, and the widest there is."""
+    for C in (2 ** 21 + 1, 2 ** 22):
+        _check(_inputs(3, C, (5,), seed=1, weight=False))
+
+
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("N", [1, 2, 31, 32, 33, 255, 257, 4095, 4097, 8193, 40000])
 def test_lengths(N, dt):

@@ -41,7 +41,7 @@ static GradShape grad_shape(long long C, int elem, int vb) {
   return g;
 }
 
-struct GradArgs {
+struct RowsGradArgs {
   RowUses u;
   const uint2* s;
   const unsigned* n;
@@ -99,7 +99,7 @@ __device__ __forceinline__ float sum8(float (&v)[8], int gl, int lanes, unsigned
 
 template <class T, int VB, int PL, bool GW>
 __global__ void __launch_bounds__(GT, PL * VB <= (GW ? 8 : 16) ? 3 : (PL * VB <= 32 ? 2 : 1))
-    k_rows_grad(GradArgs a, const T* __restrict__ table, const T* __restrict__ gout, T* __restrict__ gtable) {
+    k_rows_grad(RowsGradArgs a, const T* __restrict__ table, const T* __restrict__ gout, T* __restrict__ gtable) {
   using U = Unit<T, VB>;
   using W = typename U::W;
   constexpr int E = U::E, UN = PL * VB > (GW ? 16 : 32) ? 4 : 8;
@@ -306,7 +306,7 @@ __device__ __forceinline__ float add_parts(const float* p, long long C, long lon
 
 // Zeros for the rows without a use, a group of lanes for each; the bits of 0 are the same in every type.
 template <class W>
-__device__ __forceinline__ void zero_rows(const GradArgs& a, void* gtable, long long block, long long blocks) {
+__device__ __forceinline__ void zero_rows(const RowsGradArgs& a, void* gtable, long long block, long long blocks) {
   constexpr int UN = 4;
   const int gl = threadIdx.x % a.lanes;
   const long long groups = blocks * GT / a.lanes;
@@ -329,7 +329,7 @@ __device__ __forceinline__ void zero_rows(const GradArgs& a, void* gtable, long 
 constexpr int JOIN_TEST = 8;        // chunks of a warp
 
 template <class T>
-__global__ void __launch_bounds__(GT, 5) k_rows_join(GradArgs a, int lanes, unsigned test_blocks, unsigned parts,
+__global__ void __launch_bounds__(GT, 5) k_rows_join(RowsGradArgs a, int lanes, unsigned test_blocks, unsigned parts,
                                                      T* __restrict__ gtable) {
   __shared__ JoinItem s_many[JOIN_TEST * JOIN_WARPS];
   __shared__ int s_n;
@@ -430,12 +430,12 @@ int rows_grad(const RowUses& u, const SortSpace& s, const void* table, long long
   const int vb = grad_unit(type, t, table_stride, C, gout, gout_stride, gtable);
   GradShape g = grad_shape(C, elem_bytes(type), vb);
   // wide rows: one unit a lane and column parts, unless the weights' sums need the row in one warp (134k lookups
-  // of 328 fp32: 52 us, 64 with 4 units a lane)
+  // of 328 fp32: 52 us, 64 with 4 units a lane) or the grid has too few parts for it
   if (!gweight && g.per_lane > 1 && (g.units + g.lanes - 1) / g.lanes <= 65535) {
     g.per_lane = 1;
     g.parts = (int)((g.units + g.lanes - 1) / g.lanes);
   }
-  GradArgs a;
+  RowsGradArgs a;
   a.u = u;
   a.s = s.sorted;
   a.n = s.n;
@@ -468,9 +468,7 @@ int rows_grad(const RowUses& u, const SortSpace& s, const void* table, long long
     } else {
       if (g.per_lane == 1)
         k_rows_grad<T, VB, 1, false><<<grid, GT, 0, st>>>(a, tb, go, gt);
-      else if (g.per_lane == 2)
-        k_rows_grad<T, VB, 2, false><<<grid, GT, 0, st>>>(a, tb, go, gt);
-      else
+      else      // (4: two units a lane are one column part more)
         k_rows_grad<T, VB, 4, false><<<grid, GT, 0, st>>>(a, tb, go, gt);
     }
     if (a.chunks > 2 || a.used) {      // (a split row covers a chunk whole)
