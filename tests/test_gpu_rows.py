@@ -83,7 +83,7 @@ def test_widths(C, dt):
 
 
 def test_the_widest_rows():
-    """A width with more column parts of one unit a lane than a grid has, and the widest there is."""
+    """Rows of more column parts than any other test has, and the widest there are."""
     for C in (2 ** 21 + 1, 2 ** 22):
         _check(_inputs(3, C, (5,), seed=1, weight=False))
 

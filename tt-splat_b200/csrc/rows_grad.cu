@@ -9,34 +9,54 @@
 // partial sum, and a second kernel adds the parts in order.  A block brings its chunks' (row, use) pairs and
 // factors into shared memory first, so that nothing but gradient rows is waited for afterwards; they are read
 // once, in units of up to 16 bytes, several uses in flight.
+#include <algorithm>
+
 #include "rows.cuh"
 
 namespace tts {
 
 constexpr int GT = 256;
 
-// Uses of a chunk: few where there are few, so that they still spread over the SMs (100k lookups of 45 fp16: sums
-// and joining 22 us at 16 uses, 31 at 64; 845k of 41 bf16 from 526 rows: 104 us at 32, 88 at 64), and at most 8
-// for each lane of a group, which bounds a block's uses by BLOCK_USES.
-constexpr int L_MAX = 64;
-constexpr int BLOCK_USES = 8 * GT;
-static int chunk_len(long long N, int lanes) {
-  const int l = N <= (1 << 14) ? 8 : (N <= (1 << 17) ? 16 : L_MAX);
-  return l < 8 * lanes ? l : 8 * lanes;
+// Blocks to an SM for rows of per_lane units of vb bytes to a lane, with or without the weights' gradient, which
+// also holds the table's row: as many as the registers allow.
+constexpr int grad_blocks(int per_lane, int vb, bool weights) {
+  return per_lane * vb <= (weights ? 8 : 16) ? 3 : (per_lane * vb <= 32 ? 2 : 1);
 }
-static long long chunks_of(long long N, int lanes) { return (N + chunk_len(N, lanes) - 1) / chunk_len(N, lanes); }
+
+// Uses of a chunk: the waves of blocks that make it nearest to L_MEAN, and then what fills them, in whole steps
+// of 8 (320000 lookups of 45 fp32: 33 us in one wave, 41 at 64 uses and 1.1 waves).  At most 8 for each lane of a
+// group, which bounds a block's uses by BLOCK_USES.
+constexpr int L_MIN = 8, L_MEAN = 96, L_MAX = 128;
+constexpr int BLOCK_USES = 8 * GT;
+static int chunk_len(long long N, int lanes, int blocks) {
+  const long long wave = 148ll * blocks * (GT / lanes);
+  const long long waves = std::max(1ll, (N + wave * L_MEAN / 2) / (wave * L_MEAN));
+  const long long l = ((N + waves * wave - 1) / (waves * wave) + 7) / 8 * 8;
+  return (int)std::min<long long>(std::min(8 * lanes, L_MAX), std::max<long long>(L_MIN, l));
+}
+static long long chunks_of(long long N, int l) { return (N + l - 1) / l; }
 
 struct GradShape {
   long long units;        // of a row
   int lanes, per_lane;    // of a group; lanes * per_lane units a column part
   int parts;              // column parts
 };
-static GradShape grad_shape(long long C, int elem, int vb) {
+// Small units are packed 2 to 4 to a lane, so that a warp's steps serve two rows or four (without weights, 300000
+// lookups of 63 fp32: 31 us, 44 by one unit a lane in two column parts; with them, 320000 of 31: 27 and 34; fewer
+// lanes yet lose).  Large ones take one a lane, in column parts where that is not enough (134k lookups of 328 fp32:
+// 52 us, 64 with 4 units a lane), unless the weights' sums need the row in one warp.
+static GradShape grad_shape(long long C, int elem, int vb, bool weights) {
   GradShape g;
   g.units = C * elem / vb;
   g.lanes = 1;
   while (g.lanes < 32 && g.lanes < g.units) g.lanes *= 2;
-  g.per_lane = g.units <= 32 ? 1 : (g.units <= 64 ? 2 : 4);
+  g.per_lane = 1;
+  if (vb == 16 && weights && g.units > 32) {
+    g.per_lane = g.units <= 64 ? 2 : 4;
+  } else if (vb < 16 && g.units > 16) {
+    g.lanes = g.units <= 24 ? 8 : (g.units <= 64 ? 16 : 32);
+    g.per_lane = g.units <= 32 && g.units > 24 ? 2 : (g.units <= 24 || (g.units > 32 && g.units <= 48) ? 3 : 4);
+  }
   g.parts = (int)((g.units + g.lanes * g.per_lane - 1) / (g.lanes * g.per_lane));
   return g;
 }
@@ -98,7 +118,7 @@ __device__ __forceinline__ float sum8(float (&v)[8], int gl, int lanes, unsigned
 }
 
 template <class T, int VB, int PL, bool GW>
-__global__ void __launch_bounds__(GT, PL * VB <= (GW ? 8 : 16) ? 3 : (PL * VB <= 32 ? 2 : 1))
+__global__ void __launch_bounds__(GT, grad_blocks(PL, VB, GW))
     k_rows_grad(RowsGradArgs a, const T* __restrict__ table, const T* __restrict__ gout, T* __restrict__ gtable) {
   using U = Unit<T, VB>;
   using W = typename U::W;
@@ -401,10 +421,12 @@ __global__ void __launch_bounds__(GT, 5) k_rows_join(RowsGradArgs a, int lanes, 
 }
 
 size_t grad_space(long long N, long long C) {
-  // for the fewest lanes that a group can have, which are those of 16-byte units of two bytes' elements
-  int lanes = 1;
-  while (lanes < 32 && lanes * 8 < C) lanes *= 2;
-  return align256((size_t)chunks_of(N, lanes) * 2 * (size_t)C * sizeof(float));
+  // for the most chunks of any kernel that may run
+  long long chunks = 0;
+  for (int lanes = 1; lanes <= 32; lanes *= 2)
+    if (lanes == 32 || lanes * 16 >= C)
+      for (int blocks = 1; blocks <= 3; ++blocks) chunks = std::max(chunks, chunks_of(N, chunk_len(N, lanes, blocks)));
+  return align256((size_t)chunks * 2 * (size_t)C * sizeof(float));
 }
 
 template <class T>
@@ -420,7 +442,8 @@ static int elem_bytes(int type) { return type == TTS_ROW_F32 ? 4 : 2; }
 
 bool grad_takes_weights(const void* table, long long table_stride, int type, long long C, const void* gout,
                         long long gout_stride, const void* gtable) {
-  return grad_shape(C, elem_bytes(type), grad_unit(type, table, table_stride, C, gout, gout_stride, gtable)).parts == 1;
+  const int vb = grad_unit(type, table, table_stride, C, gout, gout_stride, gtable);
+  return grad_shape(C, elem_bytes(type), vb, true).parts == 1;
 }
 
 int rows_grad(const RowUses& u, const SortSpace& s, const void* table, long long table_stride, int type,
@@ -428,13 +451,7 @@ int rows_grad(const RowUses& u, const SortSpace& s, const void* table, long long
               cudaStream_t st) {
   const void* t = gweight ? table : nullptr;
   const int vb = grad_unit(type, t, table_stride, C, gout, gout_stride, gtable);
-  GradShape g = grad_shape(C, elem_bytes(type), vb);
-  // wide rows: one unit a lane and column parts, unless the weights' sums need the row in one warp (134k lookups
-  // of 328 fp32: 52 us, 64 with 4 units a lane) or the grid has too few parts for it
-  if (!gweight && g.per_lane > 1 && (g.units + g.lanes - 1) / g.lanes <= 65535) {
-    g.per_lane = 1;
-    g.parts = (int)((g.units + g.lanes - 1) / g.lanes);
-  }
+  const GradShape g = grad_shape(C, elem_bytes(type), vb, gweight != nullptr);
   RowsGradArgs a;
   a.u = u;
   a.s = s.sorted;
@@ -443,8 +460,8 @@ int rows_grad(const RowUses& u, const SortSpace& s, const void* table, long long
   a.C = C;
   a.table_stride = table_stride;
   a.gout_stride = gout_stride;
-  a.chunks = chunks_of(u.N, g.lanes);
-  a.L = chunk_len(u.N, g.lanes);
+  a.L = chunk_len(u.N, g.lanes, grad_blocks(g.per_lane, vb, gweight != nullptr));
+  a.chunks = chunks_of(u.N, a.L);
   a.lanes = g.lanes;
   a.units = (int)g.units;
   a.unit = vb;
@@ -458,19 +475,23 @@ int rows_grad(const RowUses& u, const SortSpace& s, const void* table, long long
     const T* tb = static_cast<const T*>(t);
     const T* go = static_cast<const T*>(gout);
     T* gt = static_cast<T*>(gtable);
-    if (gweight) {
-      if (g.per_lane == 1)
-        k_rows_grad<T, VB, 1, true><<<grid, GT, 0, st>>>(a, tb, go, gt);
-      else if (g.per_lane == 2)
-        k_rows_grad<T, VB, 2, true><<<grid, GT, 0, st>>>(a, tb, go, gt);
-      else
-        k_rows_grad<T, VB, 4, true><<<grid, GT, 0, st>>>(a, tb, go, gt);
-    } else {
-      if (g.per_lane == 1)
-        k_rows_grad<T, VB, 1, false><<<grid, GT, 0, st>>>(a, tb, go, gt);
-      else      // (4: two units a lane are one column part more)
-        k_rows_grad<T, VB, 4, false><<<grid, GT, 0, st>>>(a, tb, go, gt);
-    }
+    const auto launch = [&](auto per_lane, auto weights) {
+      k_rows_grad<T, VB, decltype(per_lane)::value, decltype(weights)::value><<<grid, GT, 0, st>>>(a, tb, go, gt);
+    };
+    const auto with_weights = [&](auto per_lane) {
+      if (gweight)
+        launch(per_lane, std::true_type());
+      else if constexpr (VB < 16 || decltype(per_lane)::value == 1)
+        launch(per_lane, std::false_type());
+    };
+    if (g.per_lane == 1)
+      with_weights(std::integral_constant<int, 1>());
+    else if (g.per_lane == 2)
+      with_weights(std::integral_constant<int, 2>());
+    else if (g.per_lane == 4)
+      with_weights(std::integral_constant<int, 4>());
+    else if constexpr (VB < 16)
+      with_weights(std::integral_constant<int, 3>());
     if (a.chunks > 2 || a.used) {      // (a split row covers a chunk whole)
       int lanes = 1;
       while (lanes < 32 && lanes < C) lanes *= 2;
