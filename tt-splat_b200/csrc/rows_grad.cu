@@ -43,7 +43,7 @@ struct GradShape {
 };
 // Small units are packed 2 to 4 to a lane, so that a warp's steps serve two rows or four (without weights, 300000
 // lookups of 63 fp32: 31 us, 44 by one unit a lane in two column parts; with them, 320000 of 31: 27 and 34; fewer
-// lanes yet lose).  Large ones take one a lane, in column parts where that is not enough (134k lookups of 328 fp32:
+// lanes yet lose; 700000 of 9: 38 and 43).  Large ones take one a lane, in column parts where that is not enough (134k lookups of 328 fp32:
 // 52 us, 64 with 4 units a lane), unless the weights' sums need the row in one warp.
 static GradShape grad_shape(long long C, int elem, int vb, bool weights) {
   GradShape g;
@@ -53,9 +53,10 @@ static GradShape grad_shape(long long C, int elem, int vb, bool weights) {
   g.per_lane = 1;
   if (vb == 16 && weights && g.units > 32) {
     g.per_lane = g.units <= 64 ? 2 : 4;
-  } else if (vb < 16 && g.units > 16) {
+  } else if (vb < 16 && g.units > 8) {
     g.lanes = g.units <= 24 ? 8 : (g.units <= 64 ? 16 : 32);
-    g.per_lane = g.units <= 32 && g.units > 24 ? 2 : (g.units <= 24 || (g.units > 32 && g.units <= 48) ? 3 : 4);
+    const long long per = (g.units + g.lanes - 1) / g.lanes;
+    g.per_lane = per < 4 ? (int)per : 4;
   }
   g.parts = (int)((g.units + g.lanes * g.per_lane - 1) / (g.lanes * g.per_lane));
   return g;
@@ -115,6 +116,23 @@ __device__ __forceinline__ float sum8(float (&v)[8], int gl, int lanes, unsigned
   }
   for (; d > 0; d >>= 1) v[0] += __shfl_xor_sync(mask, v[0], d);
   return v[0];
+}
+
+// The same for groups of 1, 2 or 4 lanes, which end with 8 / lanes sums each, in v[0 ...]: those of the values from
+// gl * 8 / lanes on (2M weighted lookups of 3 fp32: 65 us, 99 by a sum over the group for each value).
+__device__ __forceinline__ void sum8_narrow(float (&v)[8], int gl, int lanes, unsigned mask) {
+  int d = lanes / 2;
+#pragma unroll
+  for (int n = 4; n > 1; n >>= 1, d >>= 1)
+    if (d > 0) {
+      const bool up = gl & d;
+#pragma unroll
+      for (int j = 0; j < n; ++j) {
+        const float send = up ? v[j] : v[j + n];
+        const float keep = up ? v[j + n] : v[j];
+        v[j] = keep + __shfl_xor_sync(mask, send, d);
+      }
+    }
 }
 
 template <class T, int VB, int PL, bool GW>
@@ -259,11 +277,17 @@ __global__ void __launch_bounds__(GT, grad_blocks(PL, VB, GW))
       }
     }
     if constexpr (GW) {
-      if (UN == 8 && a.lanes >= 8) {
-        if constexpr (UN == 8) {
+      if constexpr (UN == 8) {
+        if (a.lanes >= 8) {
           const float sum = sum8(dot, gl, a.lanes, mask);
           const int q = gl / (a.lanes / 8);
           if (gl % (a.lanes / 8) == 0 && (ALL || q < n)) a.gweight[s_use[j + q]] = a.u.scale * sum;
+        } else {
+          sum8_narrow(dot, gl, a.lanes, mask);
+          const int held = 8 / a.lanes, q = gl * held;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i < held && (ALL || q + i < n)) a.gweight[s_use[j + q + i]] = a.u.scale * dot[i];
         }
       } else {
 #pragma unroll
