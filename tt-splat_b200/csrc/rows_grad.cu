@@ -42,9 +42,9 @@ struct GradShape {
   int parts;              // column parts
 };
 // Small units are packed 2 to 4 to a lane, so that a warp's steps serve two rows or four (without weights, 300000
-// lookups of 63 fp32: 31 us, 44 by one unit a lane in two column parts; with them, 320000 of 31: 27 and 34; fewer
-// lanes yet lose; 700000 of 9: 38 and 43).  Large ones take one a lane, in column parts where that is not enough (134k lookups of 328 fp32:
-// 52 us, 64 with 4 units a lane), unless the weights' sums need the row in one warp.
+// lookups of 63 fp32: 31 us, 44 by one unit a lane in two column parts; with them, 320000 of 31: 27 and 34, 700000
+// of 9: 37 and 43; fewer lanes yet lose).  Large ones take one a lane, in column parts where that is not enough
+// (134k lookups of 328 fp32: 52 us, 64 with 4 units a lane), unless the weights' sums need the row in one warp.
 static GradShape grad_shape(long long C, int elem, int vb, bool weights) {
   GradShape g;
   g.units = C * elem / vb;
@@ -420,7 +420,8 @@ __global__ void __launch_bounds__(GT, 5) k_rows_join(RowsGradArgs a, int lanes, 
       float sum = 0.f;
       if (col < C) sum = add_parts(a.partial + col, C, f.chunk + 1 + q, f.last + 1, nq);
       for (int d = 16; d >= lanes; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      if (q == 0 && col < C) gtable[(long long)f.row * C + col] = from_f32<T>(a.partial[(2 * f.chunk + 1) * C + col] + sum);
+      if (q == 0 && col < C)
+        gtable[(long long)f.row * C + col] = from_f32<T>(a.partial[(2 * f.chunk + 1) * C + col] + sum);
     }
   }
   __syncthreads();
