@@ -109,6 +109,14 @@ def test_row_with_most_uses(hot, N, C):
     _check(_inputs(1000, C, (N,), torch.bfloat16, seed=N, hot=hot))
 
 
+@pytest.mark.parametrize("weight", [False, True])
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("C", [3, 11, 21, 31, 45, 63, 125])
+def test_many_lookups_of_odd_rows(C, dt, weight):
+    """Rows packed several units to a lane, in the longest chunks."""
+    _check(_inputs(4000, C, (300001,), dt, seed=C, hot=0.1, weight=weight))
+
+
 @pytest.mark.parametrize("valid,weight", [(False, False), (True, False), (False, True)])
 def test_without_mask_or_weight(valid, weight):
     _check(_inputs(50, 9, (40, 16), seed=3, valid=valid, weight=weight), scale=-3.5)
