@@ -555,11 +555,12 @@ __global__ void __launch_bounds__(128) k_scores_tile(const T* __restrict__ logit
   }
 }
 
-// ---- one warp per row: rows of up to 1024 labels that no tile takes -------------------------------------
-// The row stays in registers, SLOTS logits a lane.  The k-th largest of the lanes' maxima is a bound that at
+// ---- one warp per row: rows of up to 512 labels that no tile takes -------------------------------------
+// The row stays in registers, SLOTS logits a lane (twice as many labels: 73 us for 40000 x 1000 fp32, 58 by the
+// kernel for longer rows; 39 and 42 for 40000 x 500).  The k-th largest of the lanes' maxima is a bound that at
 // least k logits reach and few more; those are gathered, a lane for each, and placed by counting how many
 // come before.  More than 32 of them (equal values): one round over the registers for each alternative.
-constexpr long long WARP_ROW_MAX = 1024;
+constexpr long long WARP_ROW_MAX = 512;
 
 // Unsigned numbers in the order of the floats (no NaN; -0 counts as 0).
 __device__ __forceinline__ unsigned order_key(float x) {
@@ -676,10 +677,12 @@ __global__ void __launch_bounds__(256) k_scores_warp(const T* __restrict__ logit
 
 // Longer rows of a warp stay in memory: one pass with each lane's own running sums, then the lanes whose maximum
 // reaches the bound read theirs again (from a cache, mostly) for the candidates.
-// Rows of up to 4096 labels where there are enough to keep the SMs busy; longer or fewer ones take a block each
+// Rows of up to 1024 labels, and of up to 4096 where there are enough to keep the SMs busy; others take a block each
 // (20000 x 1100 fp16 top 8: 34 us, 99 by blocks; 4000 x 8000 fp32: 47 and 35; 1200 x 2000 fp32: 9 and 8).
+constexpr long long WARP_LONG_FEW = 1024;
 constexpr long long WARP_LONG_MAX = 4096;
 constexpr long long WARP_LONG_ROWS = 148 * 12;
+static bool warp_rows(long long P, long long C) { return C <= WARP_LONG_FEW || (C <= WARP_LONG_MAX && P >= WARP_LONG_ROWS); }
 
 template <class T>
 __global__ void __launch_bounds__(256, 4) k_scores_warp_long(const T* __restrict__ logits, long long P, long long stride,
@@ -1134,11 +1137,9 @@ extern "C" int tts_label_log_probs(const void* logits, long long P, long long C,
       const unsigned grid = (unsigned)((P + 7) / 8);
       if (C <= 256)
         k_scores_warp<T, 8><<<grid, 256, 0, as_stream(stream)>>>(x, P, row_stride, a);
-      else if (C <= 512)
-        k_scores_warp<T, 16><<<grid, 256, 0, as_stream(stream)>>>(x, P, row_stride, a);
       else
-        k_scores_warp<T, 32><<<grid, 256, 0, as_stream(stream)>>>(x, P, row_stride, a);
-    } else if (C <= WARP_LONG_MAX && P >= WARP_LONG_ROWS) {
+        k_scores_warp<T, 16><<<grid, 256, 0, as_stream(stream)>>>(x, P, row_stride, a);
+    } else if (warp_rows(P, C)) {
       k_scores_warp_long<T><<<(unsigned)((P + 7) / 8), 256, 0, as_stream(stream)>>>(x, P, row_stride, a);
     } else if (int rc = launch_scores_block<T>(x, P, row_stride, a, as_stream(stream))) {
       return rc;
@@ -1174,7 +1175,7 @@ extern "C" int tts_label_log_probs_bwd(const void* logits, long long P, long lon
       // the logits' 16-byte vectors line up with the gradient's when both start on the same offset in every row
       const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(gx)) & 15u) == 0 &&
                         (row_stride - C) * (long long)sizeof(T) % 16 == 0;
-      if (C <= WARP_ROW_MAX || (C <= WARP_LONG_MAX && P >= WARP_LONG_ROWS)) {
+      if (warp_rows(P, C)) {
         const unsigned grid = (unsigned)((P + 7) / 8);
         if (same)
           k_scores_grad_warp<T, true><<<grid, 256, 0, st>>>(x, P, row_stride, a, gx);
