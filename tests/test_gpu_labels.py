@@ -463,3 +463,22 @@ def test_rendered_labels_train_the_rows():
     tol = uses / 4096 * (2 * e + 1.2 * (256 + 64 + 128) * U)
     assert ((grad.double() - gref).abs() <= tol[:, None] + 1e-12).all()
     assert gref.abs().max() > 100 * tol.max()
+
+
+def test_forward_mode_is_refused():
+    """A tangent of the logits or of an incoming gradient raises; plain tensors beside a dual level do not."""
+    import torch.autograd.forward_ad as fw
+    from tt_splat_b200 import metrics
+    x, t = torch.randn(6, 3, device=DEV, requires_grad=True), torch.zeros(6, dtype=torch.int64, device=DEV)
+    dual = lambda y: fw.make_dual(y.detach(), torch.ones_like(y))  # noqa: E731
+    with fw.dual_level():
+        for grad in (False, True):
+            with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
+                metrics.label_log_probs(dual(x), t)
+        s = metrics.label_log_probs(x, t, top=2)
+        for out in (s.logp, s.entropy, s.top_logp):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(out, x, dual(out), retain_graph=True)
+        assert torch.isfinite(torch.autograd.grad(s.logp.sum(), x)[0]).all()
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda y: metrics.label_log_probs(y, t).logp, (x.detach(),), (torch.ones(6, 3, device=DEV),))

@@ -331,3 +331,23 @@ def test_second_derivative_is_refused():
     (g,) = torch.autograd.grad((out * out).sum(), t, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), t)
+
+
+def test_forward_mode_is_refused():
+    """A tangent of an input or of an incoming gradient raises; plain tensors beside a dual level do not."""
+    import torch.autograd.forward_ad as fw
+    from tt_splat_b200 import binned
+    t, w = torch.randn(6, 3, device=DEV, requires_grad=True), torch.rand(4, device=DEV)
+    i = torch.tensor([1, 2, 5, 1], device=DEV)
+    dual = lambda x: fw.make_dual(x.detach(), torch.ones_like(x))  # noqa: E731
+    with fw.dual_level():
+        for args in ((dual(t), i), (t, i, None, dual(w))):
+            for grad in (False, True):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
+                    binned.gather_rows(*args)
+        out = binned.gather_rows(t, i, weight=w)
+        assert torch.equal(out, w[:, None] * t[i])
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(out, t, dual(out))
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: binned.gather_rows(x, i), (t.detach(),), (torch.ones(6, 3, device=DEV),))

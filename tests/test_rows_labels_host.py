@@ -77,3 +77,23 @@ def test_c_entry_points_refuse(pkg):
     assert score(0, 7, 0, 0) == 0
     assert lib.tts_label_log_probs_bwd(None, 5, 7, 7, 0, None, 0, 0, None, None, None, None, None, None, None, None) == 1
     assert "null" in err()
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(pkg, grad):
+    """A dual tensor raises whether or not a graph is recorded: a result without a tangent would read as a
+    derivative of zero."""
+    import torch.autograd.forward_ad as fw
+    from tt_splat_b200 import binned, metrics
+    table, idx, labels = torch.zeros(4, 3), torch.zeros(5, dtype=torch.int64), torch.zeros(4, dtype=torch.int64)
+    weight = torch.ones(5)
+    with fw.dual_level(), torch.set_grad_enabled(grad):
+        dual = lambda t: fw.make_dual(t.clone().requires_grad_(grad), torch.ones_like(t))  # noqa: E731
+        with pytest.raises(NotImplementedError, match="table has a forward-mode tangent"):
+            binned.gather_rows(dual(table), idx)
+        with pytest.raises(NotImplementedError, match="weight has a forward-mode tangent"):
+            binned.gather_rows(table, idx, weight=dual(weight))
+        with pytest.raises(NotImplementedError, match="logits has a forward-mode tangent"):
+            metrics.label_log_probs(dual(table), labels)
+        with pytest.raises(RuntimeError, match="CUDA"):
+            binned.gather_rows(table, idx, weight=weight)

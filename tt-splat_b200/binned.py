@@ -94,7 +94,8 @@ def gather_rows(table, idx, valid=None, weight=None, scale=1.0):
     negative, gets zeros; an id past the last row is never read and gets NaN.  ``weight`` is
     float32 with idx's shape.  The table is float32, bfloat16 or float16 with any row stride.
 
-    Differentiable once in ``table`` and ``weight``: a row's gradient is the sum over its uses in a
+    Differentiable once in ``table`` and ``weight``, in reverse mode only (a forward-mode tangent
+    raises): a row's gradient is the sum over its uses in a
     fixed order (fp32 sums, the same bits on every run), [R, ...] in full with zeros for rows that
     nothing looks up.  To capture a training step in a CUDA graph, take its gradients with
     ``torch.autograd.grad`` and drop the outputs of eager calls on the same leaves first: torch ties

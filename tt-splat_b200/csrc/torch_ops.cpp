@@ -31,6 +31,11 @@ void same_device(const Tensor& t, const Tensor& as, const char* what) {
   need_cuda(t);
   TORCH_CHECK_VALUE(t.device() == as.device(), what, " is on ", t.device(), ", expected ", as.device());
 }
+// There are no forward-mode formulas: a tangent that went unseen would read as a derivative of zero.
+void no_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), what,
+                              " has a forward-mode tangent: this function is differentiable in reverse mode only");
+}
 int row_type(const Tensor& t, const char* what) {
   switch (t.scalar_type()) {
     case at::kFloat: return TTS_ROW_F32;
@@ -146,6 +151,7 @@ struct GatherRows : torch::autograd::Function<GatherRows> {
     for (size_t i = 1; i < shape.size(); ++i) C *= shape[i];
     variable_list out(5);
     if (!grads[0].defined()) return out;
+    no_tangent(grads[0], "the rows' gradient");
     std::tie(out[0], out[1]) = rows_backward(s[0], shape[0], C, s[2], s[3], s[1], ctx->saved_data["scale"].toDouble(),
                                              grads[0], want & 1, want & 2);
     if (out[0].defined() && shape.size() != 2) out[0] = out[0].view(shape);
@@ -169,6 +175,8 @@ Tensor gather_rows(const Tensor& table, const Tensor& idx_, const OptTensor& val
     TORCH_CHECK_VALUE(same_shape(weight.sizes(), idx_.sizes()), "weight must have the shape of idx ",
                       shape_text(idx_.sizes()), ", got ", shape_text(weight.sizes()));
   }
+  no_tangent(table, "table");
+  no_tangent(weight, "weight");
   need_cuda(table);
   same_device(idx_, table, "idx");
   if (valid.defined()) same_device(valid, table, "valid");
@@ -224,8 +232,10 @@ struct LabelLogProbs : torch::autograd::Function<LabelLogProbs> {
     const c10::cuda::CUDAGuard guard(logits.device());
     const int64_t C = logits.size(-1), P = s[1].numel();
     const Tensor x = rows2d(logits, P, C);
-    for (int i = 0; i < 3; ++i)
+    for (int i = 0; i < 3; ++i) {
+      no_tangent(grads[i], "a gradient of the scores");
       if (grads[i].defined()) grads[i] = grads[i].contiguous();
+    }
     out[0] = at::empty(logits.sizes(), logits.options().requires_grad(false));
     check(tts_label_log_probs_bwd(ptr<void>(x), P, C, row_stride(x), row_type(logits, "logits"), ptr<void>(s[1]),
                                   index_type(s[1], "labels"), static_cast<int>(s[4].size(-1)), ptr<float>(s[2]),
@@ -245,6 +255,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> label_log_probs(const Tensor& logits,
   TORCH_CHECK_VALUE(same_shape(labels_.sizes(), rows), "labels must have the shape ", shape_text(rows), ", got ",
                     shape_text(labels_.sizes()));
   TORCH_CHECK_VALUE(top >= 0 && top <= 16, "top must be 0 to 16, got ", top);
+  no_tangent(logits, "logits");
   need_cuda(logits);
   same_device(labels_, logits, "labels");
   const Tensor labels = labels_.contiguous();

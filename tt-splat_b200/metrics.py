@@ -69,7 +69,8 @@ def label_log_probs(logits, labels, top=0):
     left), and a row of nothing else has log probability -inf, entropy 0 and no gradient.  Ties go
     to the lowest id.  A row with NaN or +inf has NaN results.
 
-    Differentiable once in the logits through all three; a row whose incoming gradients are zero
+    Differentiable once in the logits through all three, in reverse mode only (a forward-mode tangent
+    raises); a row whose incoming gradients are zero
     gets zeros whatever it holds.  To capture a training step in a CUDA graph, take its gradients
     with ``torch.autograd.grad`` and drop the outputs of eager calls on the same leaves first: torch
     ties a leaf's gradient to the stream of the graph that is still alive, and the capture fails."""
