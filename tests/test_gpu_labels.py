@@ -482,3 +482,24 @@ def test_forward_mode_is_refused():
         assert torch.isfinite(torch.autograd.grad(s.logp.sum(), x)[0]).all()
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda y: metrics.label_log_probs(y, t).logp, (x.detach(),), (torch.ones(6, 3, device=DEV),))
+
+
+def test_negated_views():
+    """Tensors that only say that their numbers are negated, as the imaginary part of a conjugate does: the same
+    bits as their copies give, forward and backward (negation rounds nothing)."""
+    from tt_splat_b200 import metrics
+    neg = torch._neg_view
+    for C in (5, 700):
+        x, t = _inputs(30, C, seed=C)
+        _check(neg(x), t, top=3)
+        s, gx = _check(x, t, top=3)
+        leaf = x.clone().requires_grad_(True)
+        g = [torch.randn(30, device=DEV), torch.randn(30, device=DEV), torch.randn(30, 3, device=DEV)]
+        s = metrics.label_log_probs(leaf, t, top=3)
+        outs = [s.logp, s.entropy, s.top_logp]
+        (a,) = torch.autograd.grad(outs, leaf, [neg(q) for q in g], retain_graph=True)
+        (b,) = torch.autograd.grad(outs, leaf, [-q for q in g])
+        assert torch.equal(a, b)
+        y = metrics.label_log_probs(neg(leaf), t, top=3)
+        w = metrics.label_log_probs(-leaf.detach(), t, top=3)
+        assert all(torch.equal(p, q) for p, q in zip(y, w))

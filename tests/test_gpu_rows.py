@@ -351,3 +351,23 @@ def test_forward_mode_is_refused():
             torch.autograd.grad(out, t, dual(out))
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda x: binned.gather_rows(x, i), (t.detach(),), (torch.ones(6, 3, device=DEV),))
+
+
+def test_negated_views():
+    """Tensors that only say that their numbers are negated, as the imaginary part of a conjugate does: the same
+    bits as their copies give, forward and backward (negation rounds nothing)."""
+    from tt_splat_b200 import binned
+    x = _inputs(40, 6, (300,), hot=0.2)
+    neg = torch._neg_view
+    _check(dict(x, table=neg(x["table"])))
+    _check(dict(x, weight=neg(x["weight"])))
+    _check(x, gout=neg(x["gout"]))
+    out = binned.gather_rows(neg(x["table"]), x["idx"], x["valid"], neg(x["weight"]))
+    assert torch.equal(out, binned.gather_rows(x["table"], x["idx"], x["valid"], x["weight"]))
+    z = torch.complex(torch.randn(40, device=DEV), torch.randn(40, device=DEV))
+    i = x["idx"].clamp(min=0)
+    assert z.conj().imag.is_neg() and torch.equal(binned.gather_rows(z.conj().imag, i), -z.imag[i])
+    t = x["table"].clone().requires_grad_(True)
+    (g,) = torch.autograd.grad(binned.gather_rows(neg(t), i), t, x["gout"])
+    (h,) = torch.autograd.grad(binned.gather_rows(t, i), t, x["gout"])
+    assert torch.equal(g, -h)

@@ -63,6 +63,10 @@ T* ptr(const Tensor& t) {
   return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
 }
 
+// The kernels read memory as it is: a tensor that only says that its numbers are negated (the imaginary part of
+// a conjugate, and such gradients) is copied with them negated.
+Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // [n, width] view of a tensor's rows with unit stride along them (the kernels take any distance between rows
 // below 2^30, an expanded row's included); a copy where no such view exists.
 Tensor rows2d(const Tensor& t, int64_t n, int64_t width) {
@@ -153,15 +157,15 @@ struct GatherRows : torch::autograd::Function<GatherRows> {
     if (!grads[0].defined()) return out;
     no_tangent(grads[0], "the rows' gradient");
     std::tie(out[0], out[1]) = rows_backward(s[0], shape[0], C, s[2], s[3], s[1], ctx->saved_data["scale"].toDouble(),
-                                             grads[0], want & 1, want & 2);
+                                             plain(grads[0]), want & 1, want & 2);
     if (out[0].defined() && shape.size() != 2) out[0] = out[0].view(shape);
     return once(std::move(out));
   }
 };
 
-Tensor gather_rows(const Tensor& table, const Tensor& idx_, const OptTensor& valid_, const OptTensor& weight_, double scale) {
-  TORCH_CHECK_VALUE(table.dim() >= 1, "table must have at least one dimension");
-  row_type(table, "table");
+Tensor gather_rows(const Tensor& table_, const Tensor& idx_, const OptTensor& valid_, const OptTensor& weight_, double scale) {
+  TORCH_CHECK_VALUE(table_.dim() >= 1, "table must have at least one dimension");
+  row_type(table_, "table");
   index_type(idx_, "idx");
   Tensor valid = of(valid_), weight = of(weight_);
   if (valid.defined()) {
@@ -175,15 +179,15 @@ Tensor gather_rows(const Tensor& table, const Tensor& idx_, const OptTensor& val
     TORCH_CHECK_VALUE(same_shape(weight.sizes(), idx_.sizes()), "weight must have the shape of idx ",
                       shape_text(idx_.sizes()), ", got ", shape_text(weight.sizes()));
   }
-  no_tangent(table, "table");
+  no_tangent(table_, "table");
   no_tangent(weight, "weight");
-  need_cuda(table);
-  same_device(idx_, table, "idx");
-  if (valid.defined()) same_device(valid, table, "valid");
-  if (weight.defined()) same_device(weight, table, "weight");
-  const Tensor idx = idx_.contiguous();
+  need_cuda(table_);
+  same_device(idx_, table_, "idx");
+  if (valid.defined()) same_device(valid, table_, "valid");
+  if (weight.defined()) same_device(weight, table_, "weight");
+  const Tensor table = plain(table_), idx = plain(idx_).contiguous();
   if (valid.defined()) valid = valid.contiguous();
-  if (weight.defined()) weight = weight.contiguous();
+  if (weight.defined()) weight = plain(weight).contiguous();
   if (at::GradMode::is_enabled() && (table.requires_grad() || (weight.defined() && weight.requires_grad())))
     return GatherRows::apply(table, weight.defined() ? OptTensor(weight) : OptTensor(), idx,
                              valid.defined() ? OptTensor(valid) : OptTensor(), scale);
@@ -234,7 +238,7 @@ struct LabelLogProbs : torch::autograd::Function<LabelLogProbs> {
     const Tensor x = rows2d(logits, P, C);
     for (int i = 0; i < 3; ++i) {
       no_tangent(grads[i], "a gradient of the scores");
-      if (grads[i].defined()) grads[i] = grads[i].contiguous();
+      if (grads[i].defined()) grads[i] = plain(grads[i]).contiguous();
     }
     out[0] = at::empty(logits.sizes(), logits.options().requires_grad(false));
     check(tts_label_log_probs_bwd(ptr<void>(x), P, C, row_stride(x), row_type(logits, "logits"), ptr<void>(s[1]),
@@ -246,19 +250,19 @@ struct LabelLogProbs : torch::autograd::Function<LabelLogProbs> {
   }
 };
 
-std::tuple<Tensor, Tensor, Tensor, Tensor> label_log_probs(const Tensor& logits, const Tensor& labels_, int64_t top) {
-  TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1, "logits must be [..., C] with at least one label, got ",
-                    shape_text(logits.sizes()));
-  row_type(logits, "logits");
+std::tuple<Tensor, Tensor, Tensor, Tensor> label_log_probs(const Tensor& logits_, const Tensor& labels_, int64_t top) {
+  TORCH_CHECK_VALUE(logits_.dim() >= 1 && logits_.size(-1) >= 1, "logits must be [..., C] with at least one label, got ",
+                    shape_text(logits_.sizes()));
+  row_type(logits_, "logits");
   index_type(labels_, "labels");
-  const at::IntArrayRef rows = logits.sizes().slice(0, logits.dim() - 1);
+  const at::IntArrayRef rows = logits_.sizes().slice(0, logits_.dim() - 1);
   TORCH_CHECK_VALUE(same_shape(labels_.sizes(), rows), "labels must have the shape ", shape_text(rows), ", got ",
                     shape_text(labels_.sizes()));
   TORCH_CHECK_VALUE(top >= 0 && top <= 16, "top must be 0 to 16, got ", top);
-  no_tangent(logits, "logits");
-  need_cuda(logits);
-  same_device(labels_, logits, "labels");
-  const Tensor labels = labels_.contiguous();
+  no_tangent(logits_, "logits");
+  need_cuda(logits_);
+  same_device(labels_, logits_, "labels");
+  const Tensor logits = plain(logits_), labels = plain(labels_).contiguous();
   if (at::GradMode::is_enabled() && logits.requires_grad()) {
     variable_list v = LabelLogProbs::apply(logits, labels, top);
     return {v[0], v[1], v[2], v[3]};
