@@ -399,7 +399,8 @@ int tts_label_log_probs(const void* logits, long long P, long long C, long long 
                         void* stream);
 /* glogits[P][C] from the gradients of logp, entropy and top_logp (each NULL when there is none);
  * stats, entropy and top_ids as the forward wrote them.  Zeros for a row whose gradients are all
- * zero and for a row of masked labels only. */
+ * zero and for a row of masked labels only; NaN for a row that holds a NaN or +inf and any gradient
+ * that is not zero (but that of a negative label's logp). */
 int tts_label_log_probs_bwd(const void* logits, long long P, long long C, long long row_stride,
                             int type, const void* labels, int labels64, int top, const float* stats,
                             const float* entropy, const int64_t* top_ids, const float* g_logp,

@@ -503,3 +503,27 @@ def test_negated_views():
         y = metrics.label_log_probs(neg(leaf), t, top=3)
         w = metrics.label_log_probs(-leaf.detach(), t, top=3)
         assert all(torch.equal(p, q) for p, q in zip(y, w))
+
+
+@pytest.mark.parametrize("P,C", [(8, 5), (40000, 21), (8, 150), (40000, 300), (8, 1000), (1900, 3001), (8, 20001), (1300, 9001)])
+def test_bad_rows_reached_by_the_alternatives_alone(P, C):
+    """A row with NaN or +inf has NaN in the place of its alternatives' log probabilities: any gradient that is not
+    zero makes its row NaN, gradients that cancel among them, and zeros leave it zero.  Its neighbours' rows are
+    as they were without it."""
+    from tt_splat_b200 import metrics
+    for dt in TYPES:
+        x, t = _inputs(P, C, dt, seed=C)
+        t[1] = t[2] = t[4] = -1
+        g = torch.randn(P, 3, generator=torch.Generator().manual_seed(3)).to(DEV)
+        leaf = x.clone().requires_grad_(True)
+        (clean,) = torch.autograd.grad(metrics.label_log_probs(leaf, t, top=3).top_logp, leaf, g)
+        x[1, C // 2], x[2, 0], x[3, C - 1], x[4, 1], x[5] = math.nan, math.inf, math.nan, math.inf, -math.inf
+        g[1] = torch.tensor([0.0, 0.0, 1.0])
+        g[2] = torch.tensor([2.0, -2.0, 0.0])
+        g[3:5] = 0.0
+        leaf = x.requires_grad_(True)
+        s = metrics.label_log_probs(leaf, t, top=3)
+        assert s.top_logp[1:5].isnan().all() and (s.top_ids[1:6] == -1).all()
+        (gx,) = torch.autograd.grad(s.top_logp, leaf, g)
+        assert gx[1:3].isnan().all() and (gx[3:6] == 0).all()
+        assert torch.equal(gx[6:], clean[6:]) and torch.equal(gx[0], clean[0])

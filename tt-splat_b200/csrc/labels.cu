@@ -805,24 +805,30 @@ struct RowGrad {
   long long t;
   bool zero;      // nothing comes in: zeros, whatever the row holds
   bool empty;     // masked labels only: zeros
-  // The gradients of the alternatives that there are, summed by one thread, or by a warp that asks together.
+  // What alternative k adds to the total: its gradient if there is one.  A row that holds a NaN or +inf has none,
+  // but NaN log probabilities in their place: a gradient that comes in for one is lost in the NaN.
+  static __device__ __forceinline__ float top_term(const GradArgs& a, long long r, int k, bool bad) {
+    const float g = a.g_top[r * a.top + k];
+    return a.top_ids[r * a.top + k] >= 0 ? g : (bad && g != 0.f ? CUDART_NAN_F : 0.f);
+  }
+  static __device__ __forceinline__ bool bad_row(const GradArgs& a, long long r) {
+    const float log_sum = a.stats[r].y;
+    return log_sum != log_sum;
+  }
+  // The alternatives' gradients, summed by one thread, or by a warp that asks together.
   static __device__ __forceinline__ float tops(const GradArgs& a, long long r) {
     float sum = 0.f;
-    if (a.g_top)
-      for (int k = 0; k < a.top; ++k) {
-        const float g = a.g_top[r * a.top + k];
-        if (a.top_ids[r * a.top + k] >= 0) sum += g;
-      }
+    if (a.g_top) {
+      const bool bad = bad_row(a, r);
+      for (int k = 0; k < a.top; ++k) sum += top_term(a, r, k, bad);
+    }
     return sum;
   }
   static __device__ __forceinline__ float warp_tops(const GradArgs& a, long long r) {
     float sum = 0.f;
     if (a.g_top) {
       const int lane = threadIdx.x & 31;
-      if (lane < a.top) {
-        const float g = a.g_top[r * a.top + lane];
-        if (a.top_ids[r * a.top + lane] >= 0) sum = g;
-      }
+      if (lane < a.top) sum = top_term(a, r, lane, bad_row(a, r));
 #pragma unroll
       for (int d = TOP_MAX / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
       sum = __shfl_sync(0xffffffffu, sum, 0);

@@ -71,7 +71,7 @@ def label_log_probs(logits, labels, top=0):
 
     Differentiable once in the logits through all three, in reverse mode only (a forward-mode tangent
     raises); a row whose incoming gradients are zero
-    gets zeros whatever it holds.  To capture a training step in a CUDA graph, take its gradients
+    gets zeros whatever it holds, one with NaN or +inf that any gradient reaches gets NaN.  To capture a training step in a CUDA graph, take its gradients
     with ``torch.autograd.grad`` and drop the outputs of eager calls on the same leaves first: torch
     ties a leaf's gradient to the stream of the graph that is still alive, and the capture fails."""
     return LabelLogProbs(*torch_ops().label_log_probs(logits, labels, top))
