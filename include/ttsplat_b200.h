@@ -53,7 +53,8 @@ int tts_version(void);
 const char* tts_last_error(void);
 
 /* Device status word written by kernels instead of trapping (bounded waits that gave up):
- * 1 = a bulk-copy wait of the forward, 2 = a relocation grid barrier, 4 = a peer barrier;
+ * 1 = a bulk-copy wait of the forward or of the label scores (whose rows' results and gradients are
+ * then NaN, their ids -1), 2 = a relocation grid barrier, 4 = a peer barrier;
  * 8 = a cached binning table that spreads a gaussian over more than its stencil.
  * Synchronous read + clear.  A non-zero word means a step skipped work: the Python train step
  * reads it at check_status / check_replicas and at the end of fit / train_mcmc, and raises. */

@@ -97,3 +97,9 @@ def test_forward_mode_is_refused(pkg, grad):
             metrics.label_log_probs(dual(table), labels)
         with pytest.raises(RuntimeError, match="CUDA"):
             binned.gather_rows(table, idx, weight=weight)
+
+
+def test_a_lost_tile_is_named(pkg):
+    """The status bit of a bulk copy that never arrived names the label scores beside the render's tiles."""
+    from tt_splat_b200 import train
+    assert "label scores" in train.status_message(1) and "per-tile forward" in train.status_message(1)

@@ -460,7 +460,8 @@ struct Best {
 };
 
 // Copies rows [r0, r0 + n) into s (16-byte pieces by the bulk copy, the few bytes behind them by threads);
-// false when the copy did not arrive (recorded in the status word).
+// false when the copy did not arrive (recorded in the status word): the results are then NaN and their ids -1,
+// not what the memory held.
 template <class T>
 __device__ __forceinline__ bool load_tile(const T* logits, long long first, int count, T* s, uint64_t* bar) {
   const unsigned bytes = (unsigned)count * (unsigned)sizeof(T), whole = bytes & ~15u;
@@ -476,6 +477,12 @@ __device__ __forceinline__ bool load_tile(const T* logits, long long first, int 
   return whole == 0 || mbar_wait_bounded(bar, 0);
 }
 
+__device__ __forceinline__ void write_lost(const ScoreArgs& a, long long r) {
+  a.logp[r] = a.entropy[r] = CUDART_NAN_F;
+  if (a.stats) a.stats[r] = make_float2(CUDART_NAN_F, CUDART_NAN_F);
+  for (int k = 0; k < a.top; ++k) write_top(a, r, k, 0.f, -1, make_float2(CUDART_NAN_F, CUDART_NAN_F));
+}
+
 constexpr int TILE_BEST = 4;      // alternatives kept in registers (K of them; K = 0: none or more than these)
 
 template <class T, int VB, bool TURN, int K>
@@ -489,8 +496,12 @@ __global__ void __launch_bounds__(128) k_scores_tile(const T* __restrict__ logit
   T* s = reinterpret_cast<T*>(smem);
   const long long r = r0 + threadIdx.x;
   const long long label = threadIdx.x < rows ? load_index(a.labels, a.labels64, r) : -1;
-  if (!load_tile(logits, r0 * C, rows * C, s, &bar)) return;
+  const bool arrived = load_tile(logits, r0 * C, rows * C, s, &bar);
   if (threadIdx.x >= rows) return;
+  if (!arrived) {
+    write_lost(a, r);
+    return;
+  }
   T* x = s + threadIdx.x * C;
   typename U::W* xu = reinterpret_cast<typename U::W*>(x);
   Soft4 sums;
@@ -1000,8 +1011,8 @@ __global__ void __launch_bounds__(128) k_scores_grad_tile(const T* __restrict__ 
   const long long r = r0 + threadIdx.x;
   const long long mine = threadIdx.x < rows ? r : r0;
   const RowGrad g(a, mine, RowGrad::tops(a, mine));
-  if (!load_tile(logits, r0 * C, rows * C, s, &bar)) return;
-  if (threadIdx.x < rows) {
+  const bool arrived = load_tile(logits, r0 * C, rows * C, s, &bar);
+  if (arrived && threadIdx.x < rows) {
     T* x = s + threadIdx.x * C;
     typename U::W* xu = reinterpret_cast<typename U::W*>(x);
     const bool none = g.zero || g.empty;
@@ -1041,8 +1052,11 @@ __global__ void __launch_bounds__(128) k_scores_grad_tile(const T* __restrict__ 
     }
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  __syncthreads();
   const int count = rows * C;
+  if (!__syncthreads_and(arrived)) {
+    for (int i = threadIdx.x; i < count; i += blockDim.x) glogits[r0 * C + i] = from_f32<T>(CUDART_NAN_F);
+    return;
+  }
   const unsigned whole = ((unsigned)count * (unsigned)sizeof(T)) & ~15u;
   if (threadIdx.x == 0 && whole > 0) {
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(glogits + r0 * C), "r"(smem_u32(s)),

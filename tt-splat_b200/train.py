@@ -32,7 +32,8 @@ DEFAULT_LR = {"means": 5e-3, "scales": 5e-3, "quats": 1e-3, "opacity": 5e-2, "op
 # Bits of the device status word (tts_read_status): the bounded waits and the table check that
 # gave up.  A step that set one of them did not do all of its work.
 STATUS_BITS = {
-    1: "a bulk-copy wait of the per-tile forward timed out (that tile's pixels were not written)",
+    1: "a bulk-copy wait of the per-tile forward timed out (that tile's pixels were not written), or one "
+       "of the label scores (their rows' results or gradients are NaN, the ids -1)",
     2: "a grid barrier of the relocation kernel timed out (the relocation was abandoned)",
     4: "a peer-exchange wait timed out (a rank's gradient or update never arrived; the waiting "
        "blocks skipped their part of the update)",
