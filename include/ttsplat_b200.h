@@ -391,7 +391,7 @@ int tts_gather_rows_bwd(const void* table, long long R, long long C, long long t
  * int32 or (labels64) int64.  logp[P] = log softmax at the label (0 for a negative label, NaN for
  * one >= C), entropy[P] of the softmax, the `top` (0..16) best labels' log probabilities
  * top_logp[P][top] and ids top_ids[P][top], best first, ties to the lowest id, and stats[P][2] =
- * (max, log of the sum of exp(x - max)) for the backward (or NULL).  Logits of -inf are masked labels: never
+ * (max, sum of exp(x - max)) for the backward (or NULL).  Logits of -inf are masked labels: never
  * an alternative (id -1 and -inf where there are fewer than `top`); a row of nothing else has logp
  * -inf and entropy 0; a NaN or +inf in a row makes its results NaN. */
 int tts_label_log_probs(const void* logits, long long P, long long C, long long row_stride,

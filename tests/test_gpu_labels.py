@@ -527,3 +527,14 @@ def test_bad_rows_reached_by_the_alternatives_alone(P, C):
         (gx,) = torch.autograd.grad(s.top_logp, leaf, g)
         assert gx[1:3].isnan().all() and (gx[3:6] == 0).all()
         assert torch.equal(gx[6:], clean[6:]) and torch.equal(gx[0], clean[0])
+
+
+@pytest.mark.parametrize("P,C", [(40000, 21), (40000, 77), (8, 150), (8, 700), (8, 1000), (1900, 3001), (8, 20001), (8, 32001), (3, 100000)])
+def test_probabilities_of_equal_logits(P, C):
+    """Equal logits: every exp is 1 and their sum C, both exactly, so that the gradient -p = -1/C of the labels that
+    are not given has the rounding of one division alone, u relative."""
+    from tt_splat_b200 import metrics
+    x = torch.full((P, C), 0.75, device=DEV, requires_grad=True)
+    s = metrics.label_log_probs(x, torch.zeros(P, dtype=torch.int64, device=DEV))
+    (g,) = torch.autograd.grad(s.logp, x, torch.ones(P, device=DEV))
+    assert (g[:, 1:].double() * -C - 1).abs().max() <= 1.01 * U

@@ -10,7 +10,9 @@
 // +inf has NaN results.  A negative label says unlabelled (logp 0, whatever the row holds), a label past
 // the last one gives NaN and reads nothing.  A row whose incoming gradients are all zero gets zeros.
 //
-// stats[r] = (m, log S); log S = -inf marks a row of masked labels only (a real one is at least 0).
+// stats[r] = (m, S); S = 0 marks a row of masked labels only (a real one is at least 1), NaN a bad row.  The
+// gradient takes p = exp(x - m) / S from S itself: log S, rounded to fp32, would put its rounding (6 of p's own
+// for a row of 32001 equal logits) on every p of the row alike.
 //
 // The running maximum starts at -FLT_MAX, so that x - m is -inf and never NaN for a masked label, and
 // x - m is clamped at D_MIN, where exp is 0 in fp32 already: 0 * D_MIN is 0 in A.  S = 0 then says that
@@ -102,7 +104,7 @@ struct ScoreArgs {
   int labels64, top;
 };
 
-// A row's results but the alternatives; x is the row (global or shared memory).
+// A row's results but the alternatives; x is the row (global or shared memory).  Returns (m, log S).
 template <class T>
 __device__ __forceinline__ float2 write_scores(const ScoreArgs& a, long long r, const Soft& s, const T* x, long long t) {
   const bool bad = s.bad(), empty = !bad && s.S == 0.f;
@@ -115,7 +117,7 @@ __device__ __forceinline__ float2 write_scores(const ScoreArgs& a, long long r, 
     lp = empty ? -CUDART_INF_F : (to_f32(x[t]) - m) - logS;
   a.logp[r] = lp;
   a.entropy[r] = bad ? nan : (empty ? 0.f : logS - s.A / s.S);
-  if (a.stats) a.stats[r] = make_float2(m, logS);
+  if (a.stats) a.stats[r] = make_float2(m, bad ? nan : s.S);
   return make_float2(m, logS);
 }
 
@@ -810,9 +812,10 @@ struct GradArgs {
   int labels64, top;
 };
 
-// With d = x - m:  dx = p (alpha - g_H d),  p = exp(d - log S),  alpha = -total - g_H (H - log S).
+// With d = x - m:  dx = p (alpha - g_H d),  p = exp(d) / S,  alpha = -total - g_H (H - log S); alpha and g_H are
+// held divided by S.
 struct RowGrad {
-  float m, c, alpha, gh, gl;
+  float m, alpha, gh, gl;
   long long t;
   bool zero;      // nothing comes in: zeros, whatever the row holds
   bool empty;     // masked labels only: zeros
@@ -822,52 +825,42 @@ struct RowGrad {
     const float g = a.g_top[r * a.top + k];
     return a.top_ids[r * a.top + k] >= 0 ? g : (bad && g != 0.f ? CUDART_NAN_F : 0.f);
   }
-  static __device__ __forceinline__ bool bad_row(const GradArgs& a, long long r) {
-    const float log_sum = a.stats[r].y;
-    return log_sum != log_sum;
-  }
-  // The alternatives' gradients, summed by one thread, or by a warp that asks together.
-  static __device__ __forceinline__ float tops(const GradArgs& a, long long r) {
-    float sum = 0.f;
-    if (a.g_top) {
-      const bool bad = bad_row(a, r);
-      for (int k = 0; k < a.top; ++k) sum += top_term(a, r, k, bad);
-    }
-    return sum;
-  }
-  static __device__ __forceinline__ float warp_tops(const GradArgs& a, long long r) {
-    float sum = 0.f;
-    if (a.g_top) {
-      const int lane = threadIdx.x & 31;
-      if (lane < a.top) sum = top_term(a, r, lane, bad_row(a, r));
-#pragma unroll
-      for (int d = TOP_MAX / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      sum = __shfl_sync(0xffffffffu, sum, 0);
-    }
-    return sum;
-  }
-  __device__ __forceinline__ RowGrad(const GradArgs& a, long long r, float of_tops) {
+  // By one thread, or by a warp that asks together (the alternatives' gradients a lane each).
+  template <bool WARP>
+  __device__ __forceinline__ RowGrad(const GradArgs& a, long long r, std::bool_constant<WARP>) {
     const float2 st = a.stats[r];
-    const float H = a.entropy[r];
+    const float H = a.entropy[r], S = st.y;
+    const bool bad = S != S;
     gh = a.g_entropy ? a.g_entropy[r] : 0.f;
     t = load_index(a.labels, a.labels64, r);
-    gl = 0.f;
-    if (a.g_logp && t >= 0) {
-      gl = a.g_logp[r];
-      if (t >= a.C && gl != 0.f) gl = CUDART_NAN_F;
+    gl = a.g_logp ? a.g_logp[r] : 0.f;
+    float of_tops = 0.f;
+    if (a.g_top) {
+      if constexpr (WARP) {
+        const int lane = threadIdx.x & 31;
+        if (lane < a.top) of_tops = top_term(a, r, lane, bad);
+#pragma unroll
+        for (int d = TOP_MAX / 2; d > 0; d >>= 1) of_tops += __shfl_xor_sync(0xffffffffu, of_tops, d);
+        of_tops = __shfl_sync(0xffffffffu, of_tops, 0);
+      } else {
+        for (int k = 0; k < a.top; ++k) of_tops += top_term(a, r, k, bad);
+      }
     }
+    if (t < 0) gl = 0.f;
+    if (t >= a.C && gl != 0.f) gl = CUDART_NAN_F;
     const float total = gl + of_tops;
     m = st.x;
-    c = -st.y * LOG2E;
-    alpha = st.y != st.y ? CUDART_NAN_F : -total - gh * (H - st.y);
     zero = total == 0.f && gh == 0.f;
-    empty = st.y == -CUDART_INF_F;
+    empty = S == 0.f;
+    const float over = __frcp_rn(S);
+    alpha = bad ? CUDART_NAN_F : (gh != 0.f ? -total - gh * (H - logf(S)) : -total) * over;
+    gh *= over;
     if (empty) gl = 0.f;
-    if (zero || empty) m = 0.f, c = 0.f, alpha = 0.f, gh = 0.f;
+    if (zero || empty) m = 0.f, alpha = 0.f, gh = 0.f;
   }
   __device__ __forceinline__ float operator()(float x) const {
     const float d = fmaxf(x - m, D_MIN);
-    return exp2_fast(fmaf(d, LOG2E, c)) * fmaf(-gh, d, alpha);
+    return exp2_fast(d * LOG2E) * fmaf(-gh, d, alpha);
   }
   // The gradient at label j, which the given label or alternatives hit.
   __device__ __forceinline__ float special(const GradArgs& a, long long r, long long j, float x) const {
@@ -919,7 +912,7 @@ __global__ void __launch_bounds__(GB_THREADS) k_scores_grad_block(const T* __res
   };
   // the first step's vectors and the row's numbers are on their way together
   fetch(lo + threadIdx.x);
-  const RowGrad g(a, r, RowGrad::warp_tops(a, r));
+  const RowGrad g(a, r, std::true_type());
   const bool none = g.zero || g.empty;
   for (long long v0 = lo + threadIdx.x; v0 < hi; v0 += GB_STEP) {
     Vec16<T> w[GB_UNROLL];
@@ -963,7 +956,7 @@ __global__ void __launch_bounds__(256) k_scores_grad_warp(const T* __restrict__ 
   const T* x = logits + r * stride;
   T* gx = glogits + r * a.C;
   const int C = (int)a.C;
-  const RowGrad g(a, r, RowGrad::warp_tops(a, r));
+  const RowGrad g(a, r, std::true_type());
   const bool none = g.zero || g.empty;
   if constexpr (SAME) {
     const RowSplit<T> rs(gx, C);
@@ -1010,7 +1003,7 @@ __global__ void __launch_bounds__(128) k_scores_grad_tile(const T* __restrict__ 
   T* s = reinterpret_cast<T*>(smem);
   const long long r = r0 + threadIdx.x;
   const long long mine = threadIdx.x < rows ? r : r0;
-  const RowGrad g(a, mine, RowGrad::tops(a, mine));
+  const RowGrad g(a, mine, std::false_type());
   const bool arrived = load_tile(logits, r0 * C, rows * C, s, &bar);
   if (arrived && threadIdx.x < rows) {
     T* x = s + threadIdx.x * C;
