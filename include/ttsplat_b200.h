@@ -366,7 +366,7 @@ int tts_unit_from_u8(const uint8_t* src, long long n, float* dst, void* stream);
  * of tools/m4_train_binned.py:203-211, for rows of any width, and its transpose.
  * table [R] rows of C elements of `type`, table_stride elements apart; idx [N] int32 or (idx64)
  * int64; valid [N] uint8 or NULL; weight [N] fp32 or NULL; N < 2^30, R < 2^31 - 1, C <= 2^22,
- * strides below 2^30.
+ * strides below 2^30.  Pointers must be aligned to their elements (refused otherwise).
  * out[N][C] = scale * weight[n] * table[idx[n]], rounded once; a slot with valid 0 or a negative
  * idx gives zeros, an idx >= R is not read and gives NaN. */
 #define TTS_ROW_F32 0
@@ -393,7 +393,8 @@ int tts_gather_rows_bwd(const void* table, long long R, long long C, long long t
  * top_logp[P][top] and ids top_ids[P][top], best first, ties to the lowest id, and stats[P][2] =
  * (max, sum of exp(x - max)) for the backward (or NULL).  Logits of -inf are masked labels: never
  * an alternative (id -1 and -inf where there are fewer than `top`); a row of nothing else has logp
- * -inf and entropy 0; a NaN or +inf in a row makes its results NaN. */
+ * -inf and entropy 0; a NaN or +inf in a row makes its results NaN.  Pointers must be aligned to their
+ * elements, stats to 8 bytes (refused otherwise). */
 int tts_label_log_probs(const void* logits, long long P, long long C, long long row_stride,
                         int type, const void* labels, int labels64, int top, float* logp,
                         float* entropy, float* top_logp, int64_t* top_ids, float* stats,

@@ -103,3 +103,36 @@ def test_a_lost_tile_is_named(pkg):
     """The status bit of a bulk copy that never arrived names the label scores beside the render's tiles."""
     from tt_splat_b200 import train
     assert "label scores" in train.status_message(1) and "per-tile forward" in train.status_message(1)
+
+
+def test_c_entry_points_refuse_misaligned_pointers(pkg):
+    """Addresses between two elements, and stats between two pairs, are refused before a launch (the addresses are
+    made up: nothing reads them)."""
+    from tt_splat_b200 import _lib
+    lib = _lib.lib()
+    refused = lambda rc: rc == 1 and "aligned" in lib.tts_last_error().decode()  # noqa: E731
+    ok = 4096
+    for type, e in ((0, 4), (1, 2), (2, 2)):
+        def gather(table=ok, idx=ok, idx64=0, weight=None, out=ok):
+            return lib.tts_gather_rows(table, 4, 3, 3, type, idx, idx64, None, weight, 1.0, 5, out, None)
+        for bad in (dict(table=ok + e // 2), dict(out=ok + e // 2), dict(idx=ok + 2), dict(idx=ok + 4, idx64=1), dict(weight=ok + 2)):
+            assert refused(gather(**bad)), bad
+
+        def gather_bwd(table=ok, idx=ok, idx64=0, weight=None, gout=ok, gtable=None, gweight=None):
+            return lib.tts_gather_rows_bwd(table, 4, 3, 3, type, idx, idx64, None, weight, 1.0, 5, gout, 3, gtable, gweight,
+                                           ok, 1 << 30, None)
+        for bad in (dict(table=ok + e // 2, gweight=ok), dict(gout=ok + e // 2, gtable=ok), dict(gtable=ok + e // 2),
+                    dict(gweight=ok + 2), dict(idx=ok + 2, gtable=ok), dict(idx=ok + 4, idx64=1, gtable=ok), dict(weight=ok + 1, gtable=ok)):
+            assert refused(gather_bwd(**bad)), bad
+
+        def score(x=ok, t=ok, t64=0, logp=ok, ent=ok, tl=ok, ti=ok, stats=ok):
+            return lib.tts_label_log_probs(x, 5, 7, 7, type, t, t64, 2, logp, ent, tl, ti, stats, None)
+        for bad in (dict(x=ok + e // 2), dict(t=ok + 2), dict(t=ok + 4, t64=1), dict(logp=ok + 2), dict(ent=ok + 2), dict(tl=ok + 1),
+                    dict(ti=ok + 4), dict(stats=ok + 4)):
+            assert refused(score(**bad)), bad
+
+        def score_bwd(x=ok, t=ok, t64=0, stats=ok, ent=ok, ti=ok, gl=ok, gh=ok, gt=ok, gx=ok):
+            return lib.tts_label_log_probs_bwd(x, 5, 7, 7, type, t, t64, 2, stats, ent, ti, gl, gh, gt, gx, None)
+        for bad in (dict(x=ok + e // 2), dict(gx=ok + e // 2), dict(t=ok + 2), dict(t=ok + 4, t64=1), dict(stats=ok + 4), dict(ent=ok + 2),
+                    dict(ti=ok + 4), dict(gl=ok + 2), dict(gh=ok + 2), dict(gt=ok + 2)):
+            assert refused(score_bwd(**bad)), bad

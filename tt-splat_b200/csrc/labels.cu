@@ -1122,6 +1122,9 @@ extern "C" int tts_label_log_probs(const void* logits, long long P, long long C,
   if (P == 0) return TTS_OK;
   TTS_REQUIRE(logits && labels && logp && entropy && (top == 0 || (top_logp && top_ids)),
               "null label_log_probs argument");
+  TTS_REQUIRE(aligned_to(row_elem(type), {logits}) && aligned_to(labels64 ? 8 : 4, {labels}) &&
+                  aligned_to(4, {logp, entropy, top_logp}) && aligned_to(8, {top_ids, stats}),
+              "logits, labels and results must be aligned to their elements, stats to 8 bytes");
   const ScoreArgs a{labels, logp, entropy, top_logp, reinterpret_cast<long long*>(top_ids), reinterpret_cast<float2*>(stats),
                     C, labels64, top};
   return with_row_type(type, [&](auto t) {
@@ -1169,6 +1172,9 @@ extern "C" int tts_label_log_probs_bwd(const void* logits, long long P, long lon
   if (P == 0) return TTS_OK;
   TTS_REQUIRE(logits && labels && stats && entropy && glogits && (!g_top || top == 0 || top_ids),
               "null label_log_probs_bwd argument");
+  TTS_REQUIRE(aligned_to(row_elem(type), {logits, glogits}) && aligned_to(labels64 ? 8 : 4, {labels}) &&
+                  aligned_to(4, {entropy, g_logp, g_entropy, g_top}) && aligned_to(8, {top_ids, stats}),
+              "logits, labels and gradients must be aligned to their elements, stats to 8 bytes");
   const GradArgs a{labels, reinterpret_cast<const float2*>(stats), entropy, reinterpret_cast<const long long*>(top_ids),
                    g_logp, g_entropy, top > 0 ? g_top : nullptr, C, labels64, top};
   cudaStream_t st = as_stream(stream);

@@ -187,7 +187,12 @@ static int check_rows(long long R, long long C, int type, long long N, long long
   TTS_REQUIRE(stride >= 0 && stride < (1ll << 30), "the distance between rows must be below 2^30");
   return TTS_OK;
 }
-static size_t elem(int type) { return type == TTS_ROW_F32 ? 4 : 2; }
+static int check_alignment(int type, const void* idx, int idx64, std::initializer_list<const void*> rows,
+                           std::initializer_list<const void*> floats) {
+  TTS_REQUIRE(aligned_to(row_elem(type), rows) && aligned_to(4, floats) && aligned_to(idx64 ? 8 : 4, {idx}),
+              "rows, indices and weights must be aligned to their elements");
+  return TTS_OK;
+}
 
 }  // namespace tts
 
@@ -199,9 +204,10 @@ extern "C" int tts_gather_rows(const void* table, long long R, long long C, long
   if (int rc = check_rows(R, C, type, N, table_stride)) return rc;
   if (N == 0 || C == 0) return TTS_OK;
   TTS_REQUIRE((table || R == 0) && idx && out, "null gather_rows argument");
+  if (int rc = check_alignment(type, idx, idx64, {table, out}, {weight})) return rc;
   const RowUses u{idx, valid, weight, scale, idx64, N, R};
   const int vb = with_row_type(type, [&](auto t) { return unit_bytes<decltype(t)>({table, out}, {C, table_stride}); });
-  const long long units = C * (long long)elem(type) / vb;
+  const long long units = C * (long long)row_elem(type) / vb;
   long long rows = GATHER_UNITS / units;
   rows = rows < 1 ? 1 : (rows > GATHER_THREADS ? GATHER_THREADS : rows);
   const int step = 16 / vb;
@@ -241,6 +247,7 @@ extern "C" int tts_gather_rows_bwd(const void* table, long long R, long long C, 
   if (int rc = check_rows(R, C, type, N, gout_stride)) return rc;
   TTS_REQUIRE(N == 0 || (idx && (gout || C == 0)), "null gather_rows_bwd argument");
   TTS_REQUIRE(!gweight || table || R == 0 || C == 0, "the weight gradient needs the table");
+  if (int rc = check_alignment(type, idx, idx64, {table, gout, gtable}, {weight, gweight})) return rc;
   if (R == 0 || C == 0) gtable = nullptr;      // nothing to write
   if (gtable && workspace_bytes < tts_gather_rows_bwd_workspace_bytes(N, R, C))
     return fail(TTS_ERR_CAPACITY, "gather_rows_bwd workspace too small");
@@ -249,12 +256,12 @@ extern "C" int tts_gather_rows_bwd(const void* table, long long R, long long C, 
   const RowUses u{idx, valid, weight, scale, idx64, N, R};
   const bool fused = gtable && gweight && grad_takes_weights(table, table_stride, type, C, gout, gout_stride, gtable);
   if (gtable && N == 0) {
-    if (cudaMemsetAsync(gtable, 0, (size_t)R * C * elem(type), st) != cudaSuccess) return check_launch("memset of the gradient");
+    if (cudaMemsetAsync(gtable, 0, (size_t)R * C * row_elem(type), st) != cudaSuccess) return check_launch("memset of the gradient");
   } else if (gtable) {
     char* w = reinterpret_cast<char*>(align256(reinterpret_cast<size_t>(workspace)));
     SortSpace s;
     const size_t at = sort_space(N, R, w, &s);
-    if (int rc = sort_uses(u, s, gtable, (size_t)R * C * elem(type), fused ? gweight : nullptr, st)) return rc;
+    if (int rc = sort_uses(u, s, gtable, (size_t)R * C * row_elem(type), fused ? gweight : nullptr, st)) return rc;
     if (int rc = rows_grad(u, s, table, table_stride, type, C, gout, gout_stride, gtable,
                            fused ? gweight : nullptr, reinterpret_cast<float*>(w + at), st))
       return rc;
@@ -263,7 +270,7 @@ extern "C" int tts_gather_rows_bwd(const void* table, long long R, long long C, 
     const int vb = with_row_type(type, [&](auto t) {
       return unit_bytes<decltype(t)>({table, gout}, {C, table_stride, gout_stride});
     });
-    const long long units = C * (long long)elem(type) / vb;
+    const long long units = C * (long long)row_elem(type) / vb;
     return with_unit(type, vb, [&](auto t, auto b) {
       using T = decltype(t);
       k_weight_grad<T, decltype(b)::value><<<(unsigned)((N + 7) / 8), 256, 0, st>>>(u, static_cast<const T*>(table), table_stride, units,

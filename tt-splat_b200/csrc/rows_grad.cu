@@ -465,12 +465,11 @@ static int grad_unit(int type, const void* table, long long ts, long long C, con
                      const void* gtable) {
   return with_row_type(type, [&](auto t) { return grad_unit<decltype(t)>(table, ts, C, gout, gs, gtable); });
 }
-static int elem_bytes(int type) { return type == TTS_ROW_F32 ? 4 : 2; }
 
 bool grad_takes_weights(const void* table, long long table_stride, int type, long long C, const void* gout,
                         long long gout_stride, const void* gtable) {
   const int vb = grad_unit(type, table, table_stride, C, gout, gout_stride, gtable);
-  return grad_shape(C, elem_bytes(type), vb, true).parts == 1;
+  return grad_shape(C, (int)row_elem(type), vb, true).parts == 1;
 }
 
 int rows_grad(const RowUses& u, const SortSpace& s, const void* table, long long table_stride, int type,
@@ -478,7 +477,7 @@ int rows_grad(const RowUses& u, const SortSpace& s, const void* table, long long
               cudaStream_t st) {
   const void* t = gweight ? table : nullptr;
   const int vb = grad_unit(type, t, table_stride, C, gout, gout_stride, gtable);
-  const GradShape g = grad_shape(C, elem_bytes(type), vb, gweight != nullptr);
+  const GradShape g = grad_shape(C, (int)row_elem(type), vb, gweight != nullptr);
   RowsGradArgs a;
   a.u = u;
   a.s = s.sorted;

@@ -3,6 +3,8 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <initializer_list>
+
 #include "common.cuh"
 
 namespace tts {
@@ -111,6 +113,15 @@ inline int with_row_type(int type, F f) {
   if (type == TTS_ROW_BF16) return f(__nv_bfloat16());
   return f(__half());
 }
+
+// Whether each pointer lies on a multiple of n bytes: a misaligned access ends the context, so that the entry
+// points refuse it.
+inline bool aligned_to(size_t n, std::initializer_list<const void*> ptrs) {
+  for (const void* p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) % n) return false;
+  return true;
+}
+inline size_t row_elem(int type) { return type == TTS_ROW_F32 ? 4 : 2; }
 
 // An index or label as given (int32 or int64).
 __device__ __forceinline__ long long load_index(const void* p, int is64, long long n) {
