@@ -1,14 +1,16 @@
-"""Build ``libttsplat_b200.so`` (sm_100a) in-tree with nvcc.
+"""Build ``libttsplat_b200.so`` (sm_100a) and the torch functions over it in-tree, with nvcc and g++.
 
 Each ``csrc/*.cu`` compiles to an object with relocatable device code (the device status word
 is shared across translation units), then nvcc links them into one shared library next to this
-file.  ``csrc/torch_ops.cpp`` (torch functions over the C entry points) compiles with g++ against the
-installed torch into ``_torch_ops.so``, which links to that library.  Objects are rebuilt only when a
-source or header is newer.  Usage:
+file: ``build_library``, which needs neither torch nor Python's headers.  ``csrc/torch_ops.cpp`` (torch
+functions over the C entry points) compiles with g++ against the installed torch into
+``_torch_ops.so``, which links to that library: ``build_torch_ops``.  Objects are rebuilt only when a
+source or header is newer.  Usage (without torch it builds the library alone):
 
     python tt-splat_b200/build.py            # or __graft_entry__.build()
 """
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -102,9 +104,18 @@ def build_library(verbose=True, extra_flags=()):
         if res.returncode != 0:
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError("nvcc link failed")
-    build_torch_ops(verbose)
+    return LIB
+
+
+def build_all(verbose=True):
+    """The CUDA library, and the torch functions where torch is installed."""
+    build_library(verbose)
+    if importlib.util.find_spec("torch") is not None:
+        build_torch_ops(verbose)
+    elif verbose:
+        print("torch is not installed: built the CUDA library without the torch functions", flush=True)
     return LIB
 
 
 if __name__ == "__main__":
-    print(build_library())
+    print(build_all())
