@@ -48,3 +48,34 @@ def test_the_whole_build_has_the_torch_functions(build):
     n = len(build.ran)
     build.build_all(verbose=False)
     assert len(build.ran) == n                     # nothing is newer
+
+
+def test_torch_functions_follow_what_they_are_built_against(build, monkeypatch):
+    """Another torch, Python or command rebuilds them; a build that fails leaves the old file, and the next one
+    tries again."""
+    import torch
+    build.build_torch_ops(verbose=False)
+    assert len(build.ran) == 1
+    build.build_torch_ops(verbose=False)
+    assert len(build.ran) == 1
+    changes = [(torch, "__version__", "9.9.9"), (sys, "version", "3.99"),
+               (build, "_torch_ops_command", lambda old=build._torch_ops_command: old() + ["-DOTHER"])]
+    for n, (obj, name, value) in enumerate(changes):
+        monkeypatch.setattr(obj, name, value)
+        build.build_torch_ops(verbose=False)
+        assert len(build.ran) == n + 2
+        build.build_torch_ops(verbose=False)
+        assert len(build.ran) == n + 2
+    with open(build.TORCH_OPS) as f:
+        old = f.read()
+    monkeypatch.setattr(torch, "__version__", "9.9.10")
+    build.rc = 1
+    for n in (5, 6):
+        with pytest.raises(RuntimeError, match="torch_ops.cpp"):
+            build.build_torch_ops(verbose=False)
+        assert len(build.ran) == n
+        with open(build.TORCH_OPS) as f:
+            assert f.read() == old
+    build.rc = 0
+    build.build_torch_ops(verbose=False)
+    assert len(build.ran) == 7

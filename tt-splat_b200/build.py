@@ -63,17 +63,38 @@ def _torch_ops_command():
             *(f"-L{p}" for p in lib), f"-L{HERE}", "-lttsplat_b200", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
 
 
+def _torch_ops_key(cmd):
+    """What the extension is built against, beside its sources: the command (paths, C++ ABI), torch and
+    Python."""
+    import torch
+    return "\n".join([torch.__version__, sys.version, *cmd])
+
+
 def build_torch_ops(verbose=True):
-    """``_torch_ops.so``; needs the CUDA library to link to."""
+    """``_torch_ops.so``; needs the CUDA library to link to.  Rebuilt when a source or header is newer, or when
+    torch, Python or the command are others than it was built with."""
     src = os.path.join(CSRC, "torch_ops.cpp")
     newest = max(os.path.getmtime(src), _headers_mtime())
-    if not os.path.exists(TORCH_OPS) or os.path.getmtime(TORCH_OPS) < newest:
+    cmd = _torch_ops_command()
+    key, stamp = _torch_ops_key(cmd), os.path.join(BUILD, "torch_ops.stamp")
+    built = None
+    if os.path.exists(TORCH_OPS) and os.path.exists(stamp):
+        with open(stamp) as f:
+            built = f.read()
+    if built != key or os.path.getmtime(TORCH_OPS) < newest:
         if verbose:
             print("torch_ops.cpp -o _torch_ops.so", flush=True)
-        res = subprocess.run(_torch_ops_command(), capture_output=True, text=True)
+        os.makedirs(BUILD, exist_ok=True)
+        # under another name first: a build that fails or is cut off leaves what was there
+        part = os.path.splitext(TORCH_OPS)[0] + ".part.so"
+        cmd[cmd.index("-o") + 1] = part
+        res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError("g++ failed on torch_ops.cpp")
+        os.replace(part, TORCH_OPS)
+        with open(stamp, "w") as f:
+            f.write(key)
     return TORCH_OPS
 
 
