@@ -371,3 +371,61 @@ def test_negated_views():
     (g,) = torch.autograd.grad(binned.gather_rows(neg(t), i), t, x["gout"])
     (h,) = torch.autograd.grad(binned.gather_rows(t, i), t, x["gout"])
     assert torch.equal(g, -h)
+
+
+@pytest.mark.parametrize("op", ["rows", "labels"])
+def test_other_threads_go_on(op):
+    """While calls wait for room in the GPU's queue, which a sleep of about a second blocks, a thread that wakes every
+    millisecond never stands still for half of it."""
+    import threading
+    import time
+
+    from tt_splat_b200 import binned, metrics
+    t, i = torch.randn(100, 16, device=DEV), torch.randint(0, 16, (100,), device=DEV)
+    call = (lambda: binned.gather_rows(t, i)) if op == "rows" else (lambda: metrics.label_log_probs(t, i))
+    call()
+    torch.cuda.synchronize()
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    stop, gaps = threading.Event(), [0.0]
+
+    def tick():
+        last = time.perf_counter()
+        while not stop.is_set():
+            time.sleep(0.001)
+            now = time.perf_counter()
+            gaps.append(now - last)
+            last = now
+
+    thread = threading.Thread(target=tick)
+    thread.start()
+    start.record()
+    torch.cuda._sleep(2_000_000_000)               # clock cycles
+    end.record()
+    n = 0
+    while not end.query() and n < 20000:
+        call()
+        n += 1
+    stop.set()
+    thread.join()
+    torch.cuda.synchronize()
+    assert max(gaps) < 0.5e-3 * start.elapsed_time(end)
+
+
+def test_saved_tensors_through_python_hooks():
+    """Hooks that pack what the functions save, which run Python inside the calls: the same bits."""
+    from tt_splat_b200 import binned, metrics
+    x = _inputs(40, 6, (300,))
+    y, lab = torch.randn(30, 9, device=DEV), torch.randint(0, 9, (30,), device=DEV)
+    packed = []
+
+    def both():
+        t, w = x["table"].clone().requires_grad_(True), x["weight"].clone().requires_grad_(True)
+        rows = torch.autograd.grad(binned.gather_rows(t, x["idx"], x["valid"], w), [t, w], x["gout"])
+        leaf = y.clone().requires_grad_(True)
+        s = metrics.label_log_probs(leaf, lab, top=2)
+        return *rows, *torch.autograd.grad(s.logp.sum() + s.entropy.sum(), leaf)
+
+    want = both()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: packed.append(0) or t.cpu(), lambda t: t.to(DEV)):
+        got = both()
+    assert len(packed) >= 5 and all(torch.equal(a, b) for a, b in zip(got, want))

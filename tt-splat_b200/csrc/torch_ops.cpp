@@ -274,7 +274,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> label_log_probs(const Tensor& logits_
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  // without the interpreter's lock, as torch's own functions run: a launch may wait for room in the GPU's queue
   namespace py = pybind11;
-  m.def("gather_rows", &gather_rows);
-  m.def("label_log_probs", &label_log_probs);
+  m.def("gather_rows", &gather_rows, py::call_guard<py::gil_scoped_release>());
+  m.def("label_log_probs", &label_log_probs, py::call_guard<py::gil_scoped_release>());
 }
