@@ -538,3 +538,53 @@ def test_probabilities_of_equal_logits(P, C):
     s = metrics.label_log_probs(x, torch.zeros(P, dtype=torch.int64, device=DEV))
     (g,) = torch.autograd.grad(s.logp, x, torch.ones(P, device=DEV))
     assert (g[:, 1:].double() * -C - 1).abs().max() <= 1.01 * U
+
+
+@pytest.mark.parametrize("P,C,dt", [(1300, 20001, torch.float32), (1600, 20003, torch.bfloat16), (1600, 20008, torch.float16),
+                                    (2110, 33333, torch.float32), (700, 60001, torch.bfloat16)])
+@pytest.mark.parametrize("aligned", [True, False])
+def test_gradient_in_several_steps(P, C, dt, aligned):
+    """Rows so many and so long that a block of the gradient takes several steps of 1024 16-byte vectors, the last
+    block fewer; logits that line up with their gradient and columns of a wider tensor that do not.  Every element
+    is compared, masked rows among them; rows without a gradient are exactly zero and change no other."""
+    from tt_splat_b200 import metrics
+    x, t = _inputs(P, C, dt, seed=P, masked=0.1)
+    x[5::101] = -math.inf
+    x[7] = 1.0
+    if not aligned:
+        wide = torch.full((P, C + 9), math.nan, device=DEV, dtype=dt)
+        wide[:, 1:C + 1] = x
+        x = wide[:, 1:C + 1]
+    _check(x, t, top=2)
+    torch.cuda.empty_cache()
+    g = [torch.randn(P, device=DEV), torch.randn(P, device=DEV)]
+    leaf = x.detach().requires_grad_(True)
+    s = metrics.label_log_probs(leaf, t)
+    (full,) = torch.autograd.grad([s.logp, s.entropy], leaf, g, retain_graph=True)
+    for q in g:
+        q[::7] = 0.0
+    (some,) = torch.autograd.grad([s.logp, s.entropy], leaf, g)
+    kept = torch.arange(P, device=DEV) % 7 != 0
+    assert (some[~kept] == 0).all() and torch.equal(some[kept], full[kept])
+
+
+def test_gradient_past_32_bits():
+    """The last rows of a gradient of more than 2^31 elements, element by element: equal logits but one, so that
+    p_j = 1 / S with S = C - 1 + e^8, off by 6u for the sum and its parts, and the rounding of the result."""
+    from tt_splat_b200 import metrics
+    C = 65536
+    P = 2 ** 31 // C + 2
+    x = torch.zeros(P, C, dtype=torch.float16, device=DEV)
+    x[-3:, 9] = 8.0
+    t = torch.full((P,), 5, dtype=torch.int64, device=DEV)
+    x.requires_grad_(True)
+    s = metrics.label_log_probs(x, t)
+    (g,) = torch.autograd.grad(s.logp, x, torch.full((P,), 4096.0, device=DEV))
+    S = C - 1 + math.exp(8.0)
+    ref = torch.full((C,), -4096.0 / S, dtype=torch.float64, device=DEV)
+    ref[5] += 4096.0
+    ref[9] *= math.exp(8.0)
+    # beside the rounding: the sum's 2 (8 + 4) u for its one large part, C / 32 + 16 additions, and 6u
+    tol = ref.abs() * (torch.finfo(torch.float16).eps / 2 + (24 + C / 32 + 16 + 6) * U) + 2.0 ** -25
+    assert ((g[-3:].double() - ref).abs() <= tol).all()
+    assert ((g[-4].double() + 4096.0 / C)[torch.arange(C, device=DEV) != 5].abs() <= 4096.0 / C * 2.0 ** -11).all()

@@ -429,3 +429,56 @@ def test_saved_tensors_through_python_hooks():
     with torch.autograd.graph.saved_tensors_hooks(lambda t: packed.append(0) or t.cpu(), lambda t: t.to(DEV)):
         got = both()
     assert len(packed) >= 5 and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# Sums of small whole numbers (and halves) are exact in fp32 whatever their order, as long as they stay below
+# 2^24 steps: a lost or doubled term of a row with many uses shows, which a bound that grows with the uses hides.
+def _check_whole(rows, N, C, dt, weight, seed=0, unused=0):
+    """A table gradient (and the weights') whose uses are `rows` in a random order, N of them after padding with
+    unused slots, against the integers."""
+    from tt_splat_b200 import binned
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    idx = torch.cat([rows, torch.full((N - rows.numel(),), -1, device=DEV)])[torch.randperm(N, generator=g, device=DEV)]
+    R = int(rows.max()) + 2
+    gout = torch.randint(-3, 4, (N, C), generator=g, device=DEV)
+    gout[:, 0] = 1                                            # counts the uses
+    table = torch.randint(-2, 3, (R, C), generator=g, device=DEV).to(dt).requires_grad_(True)
+    twice = torch.randint(1, 5, (N,), generator=g, device=DEV)      # weights of 0.5, 1, 1.5 and 2
+    w = (twice.float() * 0.5).requires_grad_(True) if weight else None
+    out = binned.gather_rows(table, idx, weight=w)
+    grads = torch.autograd.grad(out, [table] + ([w] if weight else []), gout.to(dt))
+    f = twice if weight else torch.full_like(twice, 2)
+    n = idx >= 0
+    ref = torch.zeros(R, C, dtype=torch.float64, device=DEV).index_add_(0, idx[n], (f[n, None] * gout[n]).double())
+    assert ref.abs().max() < 2 ** 24
+    assert torch.equal(grads[0], (ref * 0.5).to(dt))
+    if weight:
+        dots = (gout * table.detach().long()[idx.clamp(min=0)]).sum(1)
+        assert torch.equal(grads[1], torch.where(n, dots, 0).float())
+
+
+@pytest.mark.parametrize("weight", [False, True])
+@pytest.mark.parametrize("dt,C", [(torch.float32, 1), (torch.float32, 6), (torch.float32, 45), (torch.bfloat16, 64),
+                                  (torch.float32, 128), (torch.float16, 45), (torch.float32, 300)])
+@pytest.mark.parametrize("N", [9000, 70001, 300000])
+def test_hot_rows_exactly(N, dt, C, weight):
+    """One row with nearly all uses, first, in the middle and last among the rows, and a few hot rows in turn."""
+    for hot, share in ((0, 0.9), (500, 0.81), (999, 0.99), (3, 1.0)):
+        n = int(N * share)
+        others = torch.randint(0, 1000, (N - n,), device=DEV, generator=torch.Generator(device=DEV).manual_seed(hot))
+        _check_whole(torch.cat([torch.full((n,), hot, device=DEV), others]), N + 17, C, dt, weight, seed=hot)
+    _check_whole(torch.arange(N, device=DEV) % 5 * 7, N, C, dt, weight)
+
+
+@pytest.mark.parametrize("N,C", [(9000, 128), (60000, 32), (60000, 128), (300000, 64), (300000, 128)])
+def test_rows_on_the_borders_of_chunks(N, C):
+    """All rows have the same number of uses: every whole multiple of 8 up to 128, which the chunks' lengths are, so
+    that rows begin and end where chunks do, and one more and less; 2 to 4 of them, where a row is first split, and
+    31 to 35, where its parts are joined in another way."""
+    for L in range(8, 129, 8):
+        for m in (1, 2, 3, 4, 31, 32, 33, 34, 35):
+            for d in (-1, 0, 1):
+                size = L * m + d
+                k = N // size
+                if k and (d == 0 or m in (2, 33)):
+                    _check_whole(torch.arange(k, device=DEV).repeat_interleave(size), k * size, C, torch.float32, (L + m) % 2 == 0, seed=L)
