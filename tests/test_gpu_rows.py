@@ -482,3 +482,33 @@ def test_rows_on_the_borders_of_chunks(N, C):
                 k = N // size
                 if k and (d == 0 or m in (2, 33)):
                     _check_whole(torch.arange(k, device=DEV).repeat_interleave(size), k * size, C, torch.float32, (L + m) % 2 == 0, seed=L)
+
+
+def test_gradients_not_asked_for_are_not_computed():
+    """Where both inputs require gradients and one is asked for, the other one takes no memory, and the one that is
+    asked for has the bits of the same call with the other input constant."""
+    from tt_splat_b200 import binned
+    x = _inputs(1000000, 16, (3000,), unused=0.1)
+    t, w = x["table"].requires_grad_(True), x["weight"].requires_grad_(True)
+
+    def one(table, weight, of):
+        out = binned.gather_rows(table, x["idx"], x["valid"], weight)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        (g,) = torch.autograd.grad(out, of, x["gout"])
+        return g, torch.cuda.max_memory_allocated() - before
+
+    g, peak = one(t, w, w)
+    assert torch.equal(g, one(t.detach(), w, w)[0]) and peak < t.numel()
+    assert torch.equal(one(t, w, t)[0], one(t, w.detach(), t)[0])
+    leaf = torch.zeros((), device=DEV, requires_grad=True)          # inputs that are no leaves themselves
+    out = binned.gather_rows(t + leaf, x["idx"], x["valid"], w * 1)
+    (h,) = torch.autograd.grad(out, w, x["gout"])
+    assert torch.equal(h, g)
+    out = binned.gather_rows(t, x["idx"], x["valid"])
+    assert torch.autograd.grad(out, t, x["gout"])[0].shape == t.shape
+    t.grad = w.grad = None
+    binned.gather_rows(t, x["idx"], x["valid"], w).backward(x["gout"])      # everything
+    both = torch.autograd.grad(binned.gather_rows(t, x["idx"], x["valid"], w), [t, w], x["gout"])
+    assert torch.equal(t.grad, both[0]) and torch.equal(w.grad, both[1])

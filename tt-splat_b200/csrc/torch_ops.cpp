@@ -140,24 +140,24 @@ struct GatherRows : torch::autograd::Function<GatherRows> {
   static Tensor forward(AutogradContext* ctx, const Tensor& table, const OptTensor& weight_, const Tensor& idx,
                         const OptTensor& valid_, double scale) {
     const Tensor weight = of(weight_), valid = of(valid_);
-    const bool gt = table.requires_grad(), gw = weight.defined() && weight.requires_grad();
+    const bool gw = weight.defined() && weight.requires_grad();
     ctx->save_for_backward({gw ? table : Tensor(), weight, idx, valid});
     ctx->saved_data["scale"] = scale;
-    ctx->saved_data["want"] = static_cast<int64_t>(gt) + 2 * static_cast<int64_t>(gw);
     ctx->saved_data["shape"] = table.sizes().vec();
     return rows_forward(table, idx, valid, weight, scale);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list s = ctx->get_saved_variables();
     const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
-    const int64_t want = ctx->saved_data["want"].toInt();
+    // what this call asks for, not all that could be asked for (an absent weight has no place among the inputs)
+    const bool want_table = ctx->needs_input_grad(0), want_weight = s[1].defined() && ctx->needs_input_grad(1);
     int64_t C = 1;
     for (size_t i = 1; i < shape.size(); ++i) C *= shape[i];
     variable_list out(5);
     if (!grads[0].defined()) return out;
     no_tangent(grads[0], "the rows' gradient");
     std::tie(out[0], out[1]) = rows_backward(s[0], shape[0], C, s[2], s[3], s[1], ctx->saved_data["scale"].toDouble(),
-                                             plain(grads[0]), want & 1, want & 2);
+                                             plain(grads[0]), want_table, want_weight);
     if (out[0].defined() && shape.size() != 2) out[0] = out[0].view(shape);
     return once(std::move(out));
   }
