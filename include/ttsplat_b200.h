@@ -366,7 +366,8 @@ int tts_unit_from_u8(const uint8_t* src, long long n, float* dst, void* stream);
  * of tools/m4_train_binned.py:203-211, for rows of any width, and its transpose.
  * table [R] rows of C elements of `type`, table_stride elements apart; idx [N] int32 or (idx64)
  * int64; valid [N] uint8 or NULL; weight [N] fp32 or NULL; N < 2^30, R < 2^31 - 1, C <= 2^22,
- * strides below 2^30.  Pointers must be aligned to their elements (refused otherwise).
+ * strides below 2^30.  Pointers must be aligned to their elements, and results must not overlap the rows
+ * that are read (refused otherwise).
  * out[N][C] = scale * weight[n] * table[idx[n]], rounded once; a slot with valid 0 or a negative
  * idx gives zeros, an idx >= R is not read and gives NaN. */
 #define TTS_ROW_F32 0
@@ -402,7 +403,7 @@ int tts_label_log_probs(const void* logits, long long P, long long C, long long 
 /* glogits[P][C] from the gradients of logp, entropy and top_logp (each NULL when there is none);
  * stats, entropy and top_ids as the forward wrote them.  Zeros for a row whose gradients are all
  * zero and for a row of masked labels only; NaN for a row that holds a NaN or +inf and any gradient
- * that is not zero (but that of a negative label's logp). */
+ * that is not zero (but that of a negative label's logp).  glogits must not overlap the logits (refused). */
 int tts_label_log_probs_bwd(const void* logits, long long P, long long C, long long row_stride,
                             int type, const void* labels, int labels64, int top, const float* stats,
                             const float* entropy, const int64_t* top_ids, const float* g_logp,

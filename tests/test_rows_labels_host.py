@@ -136,3 +136,24 @@ def test_c_entry_points_refuse_misaligned_pointers(pkg):
         for bad in (dict(x=ok + e // 2), dict(gx=ok + e // 2), dict(t=ok + 2), dict(t=ok + 4, t64=1), dict(stats=ok + 4), dict(ent=ok + 2),
                     dict(ti=ok + 4), dict(gl=ok + 2), dict(gh=ok + 2), dict(gt=ok + 2)):
             assert refused(score_bwd(**bad)), bad
+
+
+def test_c_entry_points_refuse_results_over_their_inputs(pkg):
+    """Results in the memory of the rows that are read, whole or by one element, are refused before a launch (the
+    addresses are made up: nothing reads them)."""
+    from tt_splat_b200 import _lib
+    lib = _lib.lib()
+    refused = lambda rc: rc == 1 and "overlap" in lib.tts_last_error().decode()  # noqa: E731
+    x, R, C, stride, N = 1 << 20, 4, 3, 5, 6
+    for type, e in ((0, 4), (1, 2)):
+        end = x + ((R - 1) * stride + C) * e                # behind the last row
+        for out in (x, end - e, x - N * C * e + e):
+            assert refused(lib.tts_gather_rows(x, R, C, stride, type, x - 4096, 0, None, None, 1.0, N, out, None))
+        bwd = lambda table, gout, gtable: lib.tts_gather_rows_bwd(  # noqa: E731
+            table, R, C, stride, type, x - 4096, 0, None, None, 1.0, N, gout, stride, gtable, None, x - 8192, 1 << 30, None)
+        for gtable in (x, end - e, x - R * C * e + e):
+            assert refused(bwd(x, x + 4096, gtable))
+            assert refused(bwd(None, x, gtable))
+        for gx in (x, end - e, x - R * C * e + e):
+            assert refused(lib.tts_label_log_probs_bwd(x, R, C, stride, type, x - 4096, 0, 0, x - 8192, x - 8192, None,
+                                                       x - 8192, None, None, gx, None))

@@ -1175,6 +1175,8 @@ extern "C" int tts_label_log_probs_bwd(const void* logits, long long P, long lon
   TTS_REQUIRE(aligned_to(row_elem(type), {logits, glogits}) && aligned_to(labels64 ? 8 : 4, {labels}) &&
                   aligned_to(4, {entropy, g_logp, g_entropy, g_top}) && aligned_to(8, {top_ids, stats}),
               "logits, labels and gradients must be aligned to their elements, stats to 8 bytes");
+  TTS_REQUIRE(!rows_overlap(logits, P, C, row_stride, row_elem(type), glogits, P * C * (long long)row_elem(type)),
+              "the gradient must not overlap the logits");
   const GradArgs a{labels, reinterpret_cast<const float2*>(stats), entropy, reinterpret_cast<const long long*>(top_ids),
                    g_logp, g_entropy, top > 0 ? g_top : nullptr, C, labels64, top};
   cudaStream_t st = as_stream(stream);

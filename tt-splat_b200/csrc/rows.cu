@@ -205,6 +205,8 @@ extern "C" int tts_gather_rows(const void* table, long long R, long long C, long
   if (N == 0 || C == 0) return TTS_OK;
   TTS_REQUIRE((table || R == 0) && idx && out, "null gather_rows argument");
   if (int rc = check_alignment(type, idx, idx64, {table, out}, {weight})) return rc;
+  TTS_REQUIRE(!rows_overlap(table, R, C, table_stride, row_elem(type), out, N * C * (long long)row_elem(type)),
+              "the output must not overlap the table");
   const RowUses u{idx, valid, weight, scale, idx64, N, R};
   const int vb = with_row_type(type, [&](auto t) { return unit_bytes<decltype(t)>({table, out}, {C, table_stride}); });
   const long long units = C * (long long)row_elem(type) / vb;
@@ -252,6 +254,9 @@ extern "C" int tts_gather_rows_bwd(const void* table, long long R, long long C, 
   if (gtable && workspace_bytes < tts_gather_rows_bwd_workspace_bytes(N, R, C))
     return fail(TTS_ERR_CAPACITY, "gather_rows_bwd workspace too small");
   TTS_REQUIRE(!gtable || workspace, "null gather_rows_bwd workspace");
+  TTS_REQUIRE(!rows_overlap(table, R, C, table_stride, row_elem(type), gtable, R * C * (long long)row_elem(type)) &&
+                  !rows_overlap(gout, N, C, gout_stride, row_elem(type), gtable, R * C * (long long)row_elem(type)),
+              "the table's gradient must not overlap the table or the incoming gradient");
   cudaStream_t st = as_stream(stream);
   const RowUses u{idx, valid, weight, scale, idx64, N, R};
   const bool fused = gtable && gweight && grad_takes_weights(table, table_stride, type, C, gout, gout_stride, gtable);

@@ -121,6 +121,15 @@ inline bool aligned_to(size_t n, std::initializer_list<const void*> ptrs) {
     if (reinterpret_cast<uintptr_t>(p) % n) return false;
   return true;
 }
+// Whether R rows of C elements, stride apart, share memory with bytes [q, q + n): results are written while other
+// blocks still read the rows.
+inline bool rows_overlap(const void* rows, long long R, long long C, long long stride, size_t elem, const void* q,
+                         long long n) {
+  if (!rows || !q || R <= 0 || C <= 0 || n <= 0) return false;
+  const char *p = static_cast<const char*>(rows), *o = static_cast<const char*>(q);
+  const long long far = (R - 1) * stride * (long long)elem, row = C * (long long)elem;
+  return p + (far < 0 ? far : 0) < o + n && o < p + (far > 0 ? far : 0) + row;
+}
 inline size_t row_elem(int type) { return type == TTS_ROW_F32 ? 4 : 2; }
 
 // An index or label as given (int32 or int64).
