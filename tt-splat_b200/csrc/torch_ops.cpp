@@ -1,7 +1,7 @@
 // The row lookup and the label scores as torch functions: argument checks, allocation on the current stream and
 // the autograd nodes, over the C entry points.  In C++ because small training calls are bound by the host: a
 // backward that torch's engine thread runs without Python takes half the time (4000 lookups of 16 fp32 and
-// their gradient: 101 us by Python autograd functions, 59 us here).
+// their gradient: 101 us by Python autograd functions, 61 us here, of which an empty C++ function takes 41).
 #include <torch/extension.h>
 
 #include <algorithm>
